@@ -31,7 +31,8 @@ enum {
   RT_ERR_STATE = 5         /* call order violated (e.g. forward before prepare)   */
 };
 
-enum { RT_F16 = 0, RT_BF16 = 1 };
+enum { RT_F16 = 0, RT_BF16 = 1, RT_F32 = 2 };  /* RT_F32: logits of rt_token_logprobs only */
+enum { RT_KV_E4M3 = 0, RT_KV_INT8 = 1 };
 enum { RT_PATTERN_BIGBIRD = 0, RT_PATTERN_BAND = 1 };
 enum { RT_EPI_NONE = 0, RT_EPI_BIAS = 1, RT_EPI_BIAS_GELU = 2 };
 /* (3 is the internal QKV scatter of rt_gemm_qkv) */
@@ -227,6 +228,84 @@ rt_status rt_sparse_attention_static(void* ctx_dev, const void* q_dev, const voi
                                      const rt_config* cfg, const int32_t* lens_tokens_host, int n_seq,
                                      const int32_t* kv_ptr_host, const int32_t* kv_idx_host, float scale,
                                      int dtype, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Answering from encoded documents: a cache of keys and values in 8 bits, attention of later tokens over it, scores of
+ * tokens.  No counterpart in the reference, which stops at the encoder's hidden states.
+ *
+ * Indexes in device memory (table entries, lengths, token ids) are checked by the kernels: one that leaves its buffer is
+ * skipped and reported by the next rt_check_device() as RT_ERR_INVALID.  The first call on a device allocates the
+ * word for that: make it before a stream capture.
+ * ---------------------------------------------------------------------------------------- */
+
+/* Blocks of 64 tokens of one head, 64 dimensions each: k / v [blocks][kv_heads][64 tokens][64] code bytes (e4m3 or
+ * int8), k_scale / v_scale fp32 [blocks][kv_heads]; value = code * scale.  Which blocks belong to a sequence, and in which order,
+ * is the caller's block table: int32 [n_seq][table_stride], entry j = block of tokens 64 j .. 64 j + 63; entries behind a
+ * sequence's last token are not read.  Sequences may share blocks that none of them writes to. */
+typedef struct rt_kv_cache {
+  void* k_dev;
+  void* v_dev;
+  float* k_scale_dev;
+  float* v_scale_dev;
+  int32_t blocks;
+  int32_t kv_heads;
+  int32_t format;   /* RT_KV_E4M3 / RT_KV_INT8 */
+  int32_t reserved;
+} rt_kv_cache;
+
+/* Quantises the keys and values of new tokens into the cache.  Sequence s has first_dev[s + 1] - first_dev[s] (at most max_tokens,
+ * none allowed) new tokens, rows first_dev[s] .. of the batch of `tokens` rows; they take the positions from start_dev[s] on.
+ * k / v: 16-bit, element (row, head, d) at row * token_stride + head * head_stride + d (strides in elements, multiples of 8;
+ * columns of a projection's output are fine); token_stride = 0: head-major per sequence, as rt_gemm_qkv and rt_qkv_bias_transpose
+ * write them.  With a = the largest finite |value| that the call brings to a block and head:
+ *   need = e4m3: smallest power of two >= a / 448;  int8: a / 127 rounded up to 8 significant bits;  at least 2^-100.
+ * Where the block holds earlier tokens (positions below start) and need <= its scale, the scale stays; else it becomes need and the
+ * earlier codes c become round(c * old scale / scale).  New codes are round(x / scale), ties to even; infinities take
+ * the largest code, NaN the code 0.  Codes of positions that hold no token stay as they are.  No two sequences of
+ * a call may write to one block. */
+rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k_dev, const void* v_dev, int64_t token_stride,
+                            int64_t head_stride, const int32_t* block_table_dev, int table_stride, const int32_t* start_dev,
+                            const int32_t* first_dev, int n_seq, int tokens, int max_tokens, int dtype, void* stream);
+
+/* The reverse: values of the positions start_dev[s] .. of each sequence, rounded to 16 bits, into rows first_dev[s] .. of
+ * k_out / v_out [tokens][kv_heads * 64]. */
+rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* k_out_dev, void* v_out_dev, const int32_t* block_table_dev,
+                           int table_stride, const int32_t* start_dev, const int32_t* first_dev, int n_seq, int tokens,
+                           int max_tokens, int dtype, void* stream);
+
+/* out[row][head * 64 + d] = softmax(scale * q k^T) v over the cached tokens of the row's sequence.  Sequence s has the query rows
+ * first_dev[s] .. first_dev[s + 1] - 1 (at most max_q, none allowed) and context_dev[s] tokens in the cache.  causal = 0: every row
+ * sees all of them; 1: the query rows are the sequence's last tokens and row i of n sees the first context - n + i + 1.  A row
+ * that sees nothing is 0.  q: 16-bit, element (row, head, d) at row * q_stride + head * 64 + d, q_stride a multiple of 8; out
+ * [tokens][heads * 64] must not overlap q.  heads is a multiple of the cache's kv_heads: query head h reads
+ * key head h / (heads / kv_heads).  Rows behind the last sequence stay as they are.  max_context (0: as wide as the table) only
+ * guides how the work is split, a wrong one costs time. */
+rt_status rt_cached_attention(void* out_dev, const void* q_dev, int64_t q_stride, const rt_kv_cache* cache,
+                              const int32_t* block_table_dev, int table_stride, const int32_t* context_dev,
+                              const int32_t* first_dev, int n_seq, int tokens, int max_q, int max_context, int heads, float scale,
+                              int causal, int dtype, void* stream);
+
+/* Scores of tokens from logits [rows][vocab] (16-bit or RT_F32, row pitch in elements, any alignment of the elements' own
+ * size).  With p = softmax of a row:
+ *   logp_dev [rows]      log p[target]; 0 where the target is negative (no token given); NULL: not wanted
+ *   entropy_dev [rows]   -sum p log p; NULL: not wanted
+ *   stats_dev [rows][2]  {max, log sum e^(z - max)}, what rt_token_logprobs_backward takes; their sum is the log of the normaliser
+ *   top_ids_dev, top_logp_dev [rows][top]  the `top` (0 to 32, at most vocab) most likely tokens, best first, equal logits in order of their ids
+ * All in fp32 from fp32 sums.  A row of nothing but -inf: logp and top_logp -inf, entropy 0.  A row with NaN or +inf: NaN (top_ids
+ * then name the largest that are numbers, -1 where there are none left). */
+rt_status rt_token_logprobs(const void* logits_dev, int64_t pitch, const int32_t* targets_dev, int rows, int vocab, int top,
+                            float* logp_dev, float* entropy_dev, float* stats_dev, int32_t* top_ids_dev, float* top_logp_dev,
+                            int dtype, void* stream);
+
+/* The gradient with respect to the logits, rounded once to their type:
+ *   dz_v = -p_v (g_logp + sum_j g_top_j + g_entropy (log p_v + entropy)) + [v = target] g_logp + sum_j [v = top_ids_j] g_top_j
+ * g_logp_dev / g_entropy_dev fp32 [rows] or NULL (no such term; targets_dev / entropy_dev are then not read), g_top_dev fp32 [rows][top] for
+ * top_ids_dev (top = 0: none; an id may stand there twice, a negative one counts for p alone).  dlogits_dev may be logits_dev itself, with the same
+ * pitch; otherwise the two do not overlap.  Columns behind vocab stay as they are. */
+rt_status rt_token_logprobs_backward(void* dlogits_dev, int64_t out_pitch, const void* logits_dev, int64_t pitch,
+                                     const int32_t* targets_dev, const float* stats_dev, const float* entropy_dev, int rows, int vocab,
+                                     const float* g_logp_dev, const float* g_entropy_dev, int top, const int32_t* top_ids_dev,
+                                     const float* g_top_dev, int dtype, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Encoder object: weights, scratch (the TensorSet), metadata pipeline, streams and events.

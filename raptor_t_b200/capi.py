@@ -10,7 +10,8 @@ import os
 from . import build as _build
 
 RT_OK = 0
-RT_F16, RT_BF16 = 0, 1
+RT_F16, RT_BF16, RT_F32 = 0, 1, 2
+RT_KV_E4M3, RT_KV_INT8 = 0, 1
 RT_PATTERN_BIGBIRD, RT_PATTERN_BAND = 0, 1
 RT_EPI_NONE, RT_EPI_BIAS, RT_EPI_BIAS_GELU = 0, 1, 2
 
@@ -21,6 +22,13 @@ class RtConfig(C.Structure):
         ("block", C.c_int32), ("num_rand", C.c_int32), ("max_pos", C.c_int32), ("vocab", C.c_int32),
         ("type_vocab", C.c_int32), ("pattern", C.c_int32), ("band_half", C.c_int32), ("dtype", C.c_int32),
         ("eps", C.c_float), ("reserved", C.c_int32),
+    ]
+
+
+class RtKvCache(C.Structure):
+    _fields_ = [
+        ("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("k_scale_dev", C.c_void_p), ("v_scale_dev", C.c_void_p),
+        ("blocks", C.c_int32), ("kv_heads", C.c_int32), ("format", C.c_int32), ("reserved", C.c_int32),
     ]
 
 
@@ -41,6 +49,7 @@ lib = _load()
 
 _vp, _i32p, _i64p = C.c_void_p, C.POINTER(C.c_int32), C.POINTER(C.c_int64)
 _cfgp = C.POINTER(RtConfig)
+_kvp = C.POINTER(RtKvCache)
 
 _SIGS = {
     "rt_last_error": (C.c_char_p, []),
@@ -73,6 +82,14 @@ _SIGS = {
     "rt_sparse_attention": (C.c_int, [_vp, _vp, _vp, _vp, _vp, C.c_float, C.c_int, _vp]),
     "rt_sparse_attention_static": (C.c_int, [_vp, _vp, _vp, _vp, _cfgp, _i32p, C.c_int, _i32p, _i32p, C.c_float, C.c_int,
                                              _vp]),
+    "rt_kv_cache_write": (C.c_int, [_kvp, _vp, _vp, C.c_int64, C.c_int64, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int,
+                                    C.c_int, _vp]),
+    "rt_kv_cache_read": (C.c_int, [_kvp, _vp, _vp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int, _vp]),
+    "rt_cached_attention": (C.c_int, [_vp, _vp, C.c_int64, _kvp, _vp, C.c_int, _vp, _vp, C.c_int, C.c_int, C.c_int, C.c_int,
+                                      C.c_int, C.c_float, C.c_int, C.c_int, _vp]),
+    "rt_token_logprobs": (C.c_int, [_vp, C.c_int64, _vp, C.c_int, C.c_int, C.c_int, _vp, _vp, _vp, _vp, _vp, C.c_int, _vp]),
+    "rt_token_logprobs_backward": (C.c_int, [_vp, C.c_int64, _vp, C.c_int64, _vp, _vp, _vp, C.c_int, C.c_int, _vp, _vp, C.c_int,
+                                             _vp, _vp, C.c_int, _vp]),
     "rt_encoder_create": (C.c_int, [_cfgp, C.POINTER(_vp)]),
     "rt_encoder_destroy": (C.c_int, [_vp]),
     "rt_encoder_set_layer": (C.c_int, [_vp, C.c_int, C.c_uint32, C.c_int] + [_vp] * 12),

@@ -1,0 +1,319 @@
+// Writing keys and values of new tokens into the 8-bit cache, and reading them back (layout: kv_cache.cuh).
+//
+// A block's scale follows its tokens.  With a = the largest finite |value| that a call adds to the block,
+//   need = e4m3: the smallest power of two >= a / 448;  int8: a / 127 rounded up to eight significant bits;  at least 2^-100.
+// A block that holds earlier tokens keeps its scale if it is >= need; otherwise the scale becomes `need` and the earlier codes c
+// become round(c * old / need).  New codes are round(x / scale), ties to even.
+// The scale's few bits cost int8 at most 1/128 of its range and e4m3 none of its precision (a power of two moves the
+// exponent), and they make every code exact: x has at most 11 significant bits and the scale 8, so a quotient that is not itself on a border
+// between two codes is at least 2^-17 away from it, more than a correctly rounded fp32 division moves it (2^-18 at 127).  So every
+// implementation of the definition gets the same codes.
+//
+// Both kernels move bytes: 2 in and 1 out a value, or the reverse.  A warp takes one block of one head, keys or values: its
+// 64 rows of 128 bytes stay in registers between the maximum and the rounding, one pass over the data.
+#include "kv_cache.cuh"
+
+#include "device_error.h"
+#include "launch.h"
+#include "launch_count.h"
+
+namespace rt {
+
+rt_status check_kv_cache(const char* what, const rt_kv_cache* c, KvView* view) {
+  RT_REQUIRE(c != nullptr, RT_ERR_INVALID, "%s: null cache", what);
+  RT_REQUIRE(c->k_dev && c->v_dev && c->k_scale_dev && c->v_scale_dev, RT_ERR_INVALID, "%s: null pointer in the cache", what);
+  RT_REQUIRE(c->blocks > 0 && c->kv_heads > 0 && c->kv_heads <= 1024, RT_ERR_INVALID,
+             "%s: a cache needs blocks > 0 and 1 to 1024 heads (got %d, %d)", what, c->blocks, c->kv_heads);
+  RT_REQUIRE(c->format == RT_KV_E4M3 || c->format == RT_KV_INT8, RT_ERR_INVALID, "%s: unknown cache format %d", what, c->format);
+  RT_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_dev) | reinterpret_cast<uintptr_t>(c->v_dev)) & 15u) == 0, RT_ERR_INVALID,
+             "%s: cache buffers must be 16-byte aligned", what);
+  RT_REQUIRE(((reinterpret_cast<uintptr_t>(c->k_scale_dev) | reinterpret_cast<uintptr_t>(c->v_scale_dev)) & 3u) == 0, RT_ERR_INVALID,
+             "%s: scales must be 4-byte aligned", what);
+  *view = KvView{static_cast<uint8_t*>(c->k_dev), static_cast<uint8_t*>(c->v_dev), c->k_scale_dev, c->v_scale_dev, c->blocks,
+                 c->kv_heads};
+  return RT_OK;
+}
+
+namespace {
+
+// What one warp works on: tokens [lo, hi) (positions in the sequence) of one block.
+struct Span {
+  int page;          // block of the cache, < 0: nothing to do
+  int64_t base, lo, hi;
+  int64_t row0;      // packed row of position 0 (may be negative: only positions >= start are used)
+  int first, len;    // of the sequence in the packed rows
+};
+
+__device__ __forceinline__ Span span_of(int seq, int nth, const int32_t* __restrict__ table, int table_stride,
+                                        const int32_t* __restrict__ start, const int32_t* __restrict__ first, int tokens, int max_tokens,
+                                        int blocks, int* err, int site) {
+  Span s;
+  s.page = -1;
+  const int f0 = first[seq], f1 = first[seq + 1], p0 = start[seq];
+  if (f1 <= f0) return s;
+  if (f0 < 0 || f1 > tokens || p0 < 0 || f1 - f0 > max_tokens) {
+    kv::index_error(err, site);
+    return s;
+  }
+  s.first = f0;
+  s.len = f1 - f0;
+  s.row0 = static_cast<int64_t>(f0) - p0;
+  const int64_t b = p0 / 64 + nth, end = static_cast<int64_t>(p0) + s.len;
+  s.base = b * 64;
+  s.lo = s.base > p0 ? s.base : p0;
+  s.hi = s.base + 64 < end ? s.base + 64 : end;
+  if (s.lo >= s.hi) return s;
+  const int page = b < table_stride ? table[static_cast<int64_t>(seq) * table_stride + b] : -1;
+  if (page < 0 || page >= blocks) {
+    kv::index_error(err, site);
+    return s;
+  }
+  s.page = page;
+  return s;
+}
+
+// The packed row of 64 values of token `t` (row of the batch): token-major with strides, or head-major per sequence
+// (rt_qkv_bias_transpose).
+__device__ __forceinline__ int64_t value_offset(const Span& s, int64_t t, int head, int heads, int64_t token_stride,
+                                                int64_t head_stride) {
+  if (token_stride == 0) return (static_cast<int64_t>(s.first) * heads + static_cast<int64_t>(head) * s.len + (t - s.first)) * 64;
+  return t * token_stride + head * head_stride;
+}
+
+template <bool INT8>
+__device__ __forceinline__ float scale_for(float most) {
+  const uint32_t low = INT8 ? 0xffffu : 0x7fffffu;  // mantissa bits that a scale does not have
+  const uint32_t bits = __float_as_uint(most / (INT8 ? kv::kInt8Max : kv::kE4m3Max));
+  return fmaxf(__uint_as_float((bits + low) & ~low), kv::kMinScale);
+}
+
+// four codes of x / scale
+template <bool INT8>
+__device__ __forceinline__ uint32_t codes4(const float* x, float scale) {
+  if constexpr (INT8) {
+    uint32_t r = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float q = x[i] / scale;
+      const int c = __float2int_rn(q == q ? fminf(fmaxf(q, -kv::kInt8Max), kv::kInt8Max) : 0.f);
+      r |= static_cast<uint32_t>(c & 0xff) << (8 * i);
+    }
+    return r;
+  } else {
+    const float inv = 1.0f / scale;  // exact: a power of two
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = x[i] == x[i] ? x[i] * inv : 0.f;
+    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
+    return a | (b << 16);
+  }
+}
+
+// values of four codes, times `scale`
+template <bool INT8>
+__device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
+  using C = kv::Codes<INT8>;
+  const uint32_t p = C::prepare(w);
+  const float2 a = kv::unpack16<false>(C::template pair<0>(p)), b = kv::unpack16<false>(C::template pair<2>(p));
+  const float s = scale * C::kUnit;  // an exact product: a power of two
+  x[0] = a.x * s;
+  x[1] = a.y * s;
+  x[2] = b.x * s;
+  x[3] = b.y * s;
+}
+
+// grid: (block of the sequence, head) pairs of every sequence; warp 0 takes the keys, warp 1 the values.
+template <bool BF16, bool INT8>
+__global__ void __launch_bounds__(64)
+kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t token_stride, int64_t head_stride,
+                const int32_t* __restrict__ table, int table_stride, const int32_t* __restrict__ start,
+                const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
+  RT_PDL_LAUNCH_DEPENDENTS();
+  RT_PDL_WAIT();
+  const int head = blockIdx.x % c.heads;
+  const int nth = blockIdx.x / c.heads % spans;
+  const int seq = blockIdx.x / c.heads / spans;
+  const int lane = threadIdx.x & 31;
+  const bool values = threadIdx.x >= 32;
+  const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheWrite);
+  if (s.page < 0) return;
+  const uint16_t* x = values ? v : k;
+  const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
+  uint8_t* dst = (values ? c.v : c.k) + slot * 4096;
+  float* scale_at = (values ? c.v_scale : c.k_scale) + slot;
+
+  // eight lanes a row, four rows an instruction
+  uint4 w[16];
+  const int sub = lane >> 3, col = (lane & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t pos = s.base + 4 * i + sub;
+    w[i] = make_uint4(0, 0, 0, 0);
+    if (pos >= s.lo && pos < s.hi)
+      w[i] = __ldg(reinterpret_cast<const uint4*>(x + value_offset(s, s.row0 + pos, head, c.heads, token_stride, head_stride) + col));
+  }
+  const bool older = s.lo > s.base;
+  const float was = older ? *scale_at : 0.f;
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 f = kv::unpack16<BF16>(p[j]);
+      const float a = fabsf(f.x), b = fabsf(f.y);
+      if (a < INFINITY) most = fmaxf(most, a);
+      if (b < INFINITY) most = fmaxf(most, b);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+  const float need = scale_for<INT8>(most);
+  const bool grow = older && !(need <= was);
+  const float scale = older && !grow ? was : need;
+  if (grow) {  // the earlier tokens' codes, four lanes a row
+    for (int r = lane >> 2; r < s.lo - s.base; r += 8) {
+      uint4* at = reinterpret_cast<uint4*>(dst + r * 64 + (lane & 3) * 16);
+      uint4 old = *at;
+      uint32_t* p = reinterpret_cast<uint32_t*>(&old);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        float f[4];
+        values4<INT8>(p[j], was, f);
+        p[j] = codes4<INT8>(f, scale);
+      }
+      *at = old;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t pos = s.base + 4 * i + sub;
+    if (pos < s.lo || pos >= s.hi) continue;
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
+    uint2 out;
+    float f[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 t = kv::unpack16<BF16>(p[j]);
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
+    }
+    out.x = codes4<INT8>(f, scale);
+    out.y = codes4<INT8>(f + 4, scale);
+    *reinterpret_cast<uint2*>(dst + (4 * i + sub) * 64 + col) = out;
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0 && !(older && !grow)) *scale_at = scale;
+}
+
+// The same grid; out_k / out_v are token-major [tokens][heads * 64].
+template <bool BF16, bool INT8>
+__global__ void __launch_bounds__(64)
+kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, const int32_t* __restrict__ table,
+               int table_stride, const int32_t* __restrict__ start, const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
+  RT_PDL_LAUNCH_DEPENDENTS();
+  RT_PDL_WAIT();
+  const int head = blockIdx.x % c.heads;
+  const int nth = blockIdx.x / c.heads % spans;
+  const int seq = blockIdx.x / c.heads / spans;
+  const int lane = threadIdx.x & 31;
+  const bool values = threadIdx.x >= 32;
+  const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheRead);
+  if (s.page < 0) return;
+  const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
+  const uint8_t* src = (values ? c.v : c.k) + slot * 4096;
+  const float scale = (values ? c.v_scale : c.k_scale)[slot];
+  uint16_t* out = values ? out_v : out_k;
+  const int sub = lane >> 3, col = (lane & 7) * 8;
+  uint2 w[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t pos = s.base + 4 * i + sub;
+    w[i] = make_uint2(0, 0);
+    if (pos >= s.lo && pos < s.hi) w[i] = *reinterpret_cast<const uint2*>(src + (4 * i + sub) * 64 + col);
+  }
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t pos = s.base + 4 * i + sub;
+    if (pos < s.lo || pos >= s.hi) continue;
+    float f[8];
+    values4<INT8>(w[i].x, scale, f);
+    values4<INT8>(w[i].y, scale, f + 4);
+    uint4 o;
+    o.x = kv::pack16<BF16>(f[0], f[1]);
+    o.y = kv::pack16<BF16>(f[2], f[3]);
+    o.z = kv::pack16<BF16>(f[4], f[5]);
+    o.w = kv::pack16<BF16>(f[6], f[7]);
+    *reinterpret_cast<uint4*>(out + ((s.row0 + pos) * c.heads + head) * 64 + col) = o;
+  }
+}
+
+// Blocks that `max_tokens` new tokens of a sequence touch at most, wherever they start.
+int64_t spans_of(int max_tokens) { return (static_cast<int64_t>(max_tokens) + 62) / 64 + 1; }
+
+rt_status check_ragged(const char* what, const int32_t* table, int table_stride, const int32_t* start, const int32_t* first, int n_seq,
+                       int tokens, int max_tokens, int kv_heads, int dtype, int64_t* grid) {
+  RT_REQUIRE(table && start && first, RT_ERR_INVALID, "%s: null pointer", what);
+  RT_REQUIRE(dtype == RT_F16 || dtype == RT_BF16, RT_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  RT_REQUIRE(n_seq >= 0 && tokens >= 0 && table_stride > 0 && max_tokens >= 0, RT_ERR_INVALID, "%s: bad sizes", what);
+  *grid = static_cast<int64_t>(n_seq) * kv_heads;  // under 2^41
+  if (tokens == 0 || max_tokens == 0) *grid = 0;
+  RT_REQUIRE(*grid < (int64_t{1} << 31) && (*grid *= spans_of(max_tokens)) < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "%s: %d sequences of up to %d tokens are too many for one call", what,
+             n_seq, max_tokens);
+  return RT_OK;
+}
+
+}  // namespace
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k, const void* v, int64_t token_stride,
+                                       int64_t head_stride, const int32_t* table, int table_stride, const int32_t* start,
+                                       const int32_t* first, int n_seq, int tokens, int max_tokens, int dtype, void* stream) {
+  KvView c;
+  int64_t grid = 0;
+  RT_TRY(check_kv_cache("kv_cache_write", cache, &c));
+  RT_TRY(check_ragged("kv_cache_write", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &grid));
+  if (grid == 0) return RT_OK;
+  RT_REQUIRE(k && v, RT_ERR_INVALID, "kv_cache_write: null pointer");
+  RT_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && token_stride % 8 == 0 &&
+                 head_stride % 8 == 0 && token_stride >= 0 && head_stride >= 0,
+             RT_ERR_INVALID, "kv_cache_write: keys and values must be 16-byte aligned, with strides that are multiples of 8 values");
+  int* err = device_error_word();
+  RT_REQUIRE(err != nullptr, RT_ERR_CUDA, "kv_cache_write: cannot allocate the device error word");
+  const bool int8 = cache->format == RT_KV_INT8;
+  auto kern = dtype == RT_BF16 ? (int8 ? kv_write_kernel<true, true> : kv_write_kernel<true, false>)
+                               : (int8 ? kv_write_kernel<false, true> : kv_write_kernel<false, false>);
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(64), 0, static_cast<cudaStream_t>(stream), c,
+                              static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), token_stride, head_stride, table,
+                              table_stride, start, first, tokens, max_tokens, static_cast<int>(spans_of(max_tokens)), err));
+  count_launch();
+  RT_CHECK_CUDA(cudaGetLastError());
+  return RT_OK;
+}
+
+extern "C" rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* out_k, void* out_v, const int32_t* table, int table_stride,
+                                      const int32_t* start, const int32_t* first, int n_seq, int tokens, int max_tokens, int dtype,
+                                      void* stream) {
+  KvView c;
+  int64_t grid = 0;
+  RT_TRY(check_kv_cache("kv_cache_read", cache, &c));
+  RT_TRY(check_ragged("kv_cache_read", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &grid));
+  if (grid == 0) return RT_OK;
+  RT_REQUIRE(out_k && out_v, RT_ERR_INVALID, "kv_cache_read: null pointer");
+  RT_REQUIRE(((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) & 15u) == 0, RT_ERR_INVALID,
+             "kv_cache_read: outputs must be 16-byte aligned");
+  int* err = device_error_word();
+  RT_REQUIRE(err != nullptr, RT_ERR_CUDA, "kv_cache_read: cannot allocate the device error word");
+  const bool int8 = cache->format == RT_KV_INT8;
+  auto kern = dtype == RT_BF16 ? (int8 ? kv_read_kernel<true, true> : kv_read_kernel<true, false>)
+                               : (int8 ? kv_read_kernel<false, true> : kv_read_kernel<false, false>);
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(64), 0, static_cast<cudaStream_t>(stream), c,
+                              static_cast<uint16_t*>(out_k), static_cast<uint16_t*>(out_v), table, table_stride, start, first, tokens,
+                              max_tokens, static_cast<int>(spans_of(max_tokens)), err));
+  count_launch();
+  RT_CHECK_CUDA(cudaGetLastError());
+  return RT_OK;
+}

@@ -1,0 +1,88 @@
+// The 8-bit key/value cache: blocks of 64 tokens x 64 dimensions of one head, one code byte a value, one fp32 scale for each
+// block and head (value = code * scale).  Shared by the kernels that write, read and attend over it.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.h"
+
+namespace rt {
+
+struct KvView {  // rt_kv_cache by value
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int blocks;
+  int heads;
+};
+
+// Checks of a cache argument that every entry point makes.
+rt_status check_kv_cache(const char* what, const rt_kv_cache* cache, KvView* view);
+
+namespace kv {
+
+constexpr float kE4m3Max = 448.f, kInt8Max = 127.f;
+constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: 1 / scale stays a normal number
+
+__device__ __forceinline__ void index_error(int* err, int site) { atomicCAS(err, 0, site); }
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+  uint32_t r;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+  return r;
+}
+
+// Codes as half2, exactly.
+//   int8: the code with its sign bit flipped is an unsigned byte u = code + 128; the half with bits 0x6400 | u is 1024 + u.
+//   e4m3: sign, exponent and mantissa bits moved to where a half has them: the half is the value times 2^-8 (the exponents' biases
+//     differ by 8), subnormal codes included.  kUnit is what brings it back.  The NaN code, which the writer never stores, reads
+//     as 480, so that bytes nobody wrote are finite numbers, too.
+template <bool INT8>
+struct Codes;
+
+template <>
+struct Codes<true> {
+  static constexpr float kUnit = 1.f;
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
+  // bytes `LO` and `LO + 1` of prepared codes
+  template <int LO>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const uint32_t x = prmt(w, 0x64646464u, LO == 0 ? 0x4140u : 0x4342u);
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0xe480)));  // - 1152
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
+};
+
+template <>
+struct Codes<false> {
+  static constexpr float kUnit = 256.f;
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
+  template <int LO>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    const uint32_t x = prmt(w, 0u, LO == 0 ? 0x1404u : 0x3424u);
+    return (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ float2 unpack16(uint32_t w) {
+  if constexpr (BF16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  else return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float a, float b) {
+  if constexpr (BF16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+}  // namespace kv
+}  // namespace rt

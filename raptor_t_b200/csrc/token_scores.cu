@@ -1,0 +1,594 @@
+// Scores of tokens from rows of logits z over a vocabulary, and their gradient.  With m = max z and S = sum e^(z - m):
+//   logp = (z_t - m) - log S,   entropy H = log S - sum e^(z - m) (z - m) / S,   the k best tokens by (value, then lower index);
+//   dz_v = -p_v (g_logp + sum_j g_top_j + g_H (log p_v + H)) + [v = t] g_logp + sum_j [v = id_j] g_top_j.
+// Both read every logit once and are bound by that (the gradient writes as much).
+//
+// Forward: a CTA, or a cluster of CTAs where there are few rows, takes a row.  A thread keeps the running maximum, sum and weighted sum of its
+// share.  The k best come without a second pass over the row: the k-th largest of the maxima of groups of eight threads is a
+// value that at least k logits reach; only threads whose own maximum reaches it look at their share again (a few dozen
+// logits, still in L2) and list what does.  A list that does not fit (thousands of equal logits) is replaced by k
+// searches over the row.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "device_error.h"
+#include "launch.h"
+#include "launch_count.h"
+#include "sm100_ptx.cuh"
+
+namespace rt {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kGroups = kThreads / 8;
+constexpr int kMaxTop = 32;
+constexpr int kListed = 1024;  // candidates that a CTA can list
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int TYPE>
+struct Logits;  // vectors of 16 bytes
+
+template <>
+struct Logits<RT_F32> {
+  using T = float;
+  static constexpr int kVec = 4;
+  static __device__ __forceinline__ float one(const T* p) { return *p; }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+    f[0] = __uint_as_float(v.x);
+    f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z);
+    f[3] = __uint_as_float(v.w);
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+  }
+  static __device__ __forceinline__ T from(float f) { return f; }
+};
+
+template <>
+struct Logits<RT_F16> {
+  using T = __half;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float one(const T* p) { return __half2float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+    const __half2* h = reinterpret_cast<const __half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 t = __half22float2(h[i]);
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    uint4 v;
+    __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    return v;
+  }
+  static __device__ __forceinline__ T from(float f) { return __float2half_rn(f); }
+};
+
+template <>
+struct Logits<RT_BF16> {
+  using T = __nv_bfloat16;
+  static constexpr int kVec = 8;
+  static __device__ __forceinline__ float one(const T* p) { return __bfloat162float(*p); }
+  static __device__ __forceinline__ void unpack(const uint4& v, float* f) {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ uint4 pack(const float* f) {
+    uint4 v;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    return v;
+  }
+  static __device__ __forceinline__ T from(float f) { return __float2bfloat16_rn(f); }
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Running statistics of a share of a row.
+struct Stats {
+  float m = -INFINITY, s = 0.f, w = 0.f;  // maximum, sum e^(z - m), sum e^(z - m) (z - m)
+  // relative to another maximum (at least m)
+  __device__ __forceinline__ void raise(float to) {
+    if (m == -INFINITY) {
+      w = 0.f;  // s is 0, or NaN and stays
+    } else {
+      const float d = m - to, c = ex2(d * kLog2e);
+      w = c > 0.f ? (w + s * d) * c : s * c;  // the product of 0 and an infinite d is left out; a NaN of s stays
+      s *= c;
+    }
+    m = to;
+  }
+  __device__ __forceinline__ void add(float z) {  // z <= m
+    const float x = max_nan(z - m, -1000.f);      // -inf: e^x is 0 and so is its product with x
+    const float e = ex2(x * kLog2e);
+    s += e;
+    w = fmaf(e, x, w);
+  }
+  __device__ __forceinline__ void join(const Stats& o) {
+    Stats b = o;
+    const float to = fmaxf(m, b.m);
+    if (to != m) raise(to);
+    if (to != b.m) b.raise(to);
+    s += b.s;
+    w += b.w;
+  }
+};
+
+// A share of `nv` vectors and the elements before and behind them.  Vectors [lo, hi) belong to this CTA.
+template <int TYPE>
+struct Share {
+  using L = Logits<TYPE>;
+  const typename L::T* row;
+  int head, nv, vocab;  // elements before the first aligned vector; vectors
+  int lo, hi;
+  bool edge;  // this CTA takes the elements outside the vectors
+  __device__ __forceinline__ Share(const typename L::T* p, int v, int rank, int ranks) : row(p), vocab(v) {
+    const int mis = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15u) / static_cast<int>(sizeof(typename L::T));
+    head = min(v, (L::kVec - mis) % L::kVec);
+    nv = (v - head) / L::kVec;
+    const int each = (nv + ranks - 1) / ranks;
+    lo = min(nv, rank * each);
+    hi = min(nv, lo + each);
+    edge = rank == 0;
+  }
+  __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(row + head); }
+  // the index of the `i`-th element outside the vectors, -1 behind the last one
+  __device__ __forceinline__ int outside(int i) const {
+    if (!edge) return -1;
+    if (i < head) return i;
+    const int j = head + nv * L::kVec + (i - head);
+    return j < vocab ? j : -1;
+  }
+  // every element of the calling thread's share
+  template <typename F>
+  __device__ __forceinline__ void each_of_mine(F f) const {
+    for (int i = lo + static_cast<int>(threadIdx.x); i < hi; i += kThreads) {
+      float x[L::kVec];
+      L::unpack(__ldg(vectors() + i), x);
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) f(x[j], head + i * L::kVec + j);
+    }
+    if (threadIdx.x < 2 * L::kVec) {
+      const int i = outside(threadIdx.x);
+      if (i >= 0) f(L::one(row + i), i);
+    }
+  }
+};
+
+// Order of candidates as unsigned numbers: by value (NaN not among them), then lower index first.
+__device__ __forceinline__ unsigned long long key_of(float z, int index) {
+  uint32_t u = __float_as_uint(z == 0.f ? 0.f : z);  // -0 equals 0
+  u = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return static_cast<unsigned long long>(u) << 32 | static_cast<uint32_t>(~index);
+}
+__device__ __forceinline__ float value_of(unsigned long long key) {
+  uint32_t u = static_cast<uint32_t>(key >> 32);
+  u = u & 0x80000000u ? u & 0x7fffffffu : ~u;
+  return __uint_as_float(u);
+}
+__device__ __forceinline__ int index_of(unsigned long long key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
+
+__device__ __forceinline__ unsigned long long max_u64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
+
+struct ScoreArgs {
+  const void* logits;
+  int64_t pitch;
+  const int32_t* targets;
+  int rows, vocab, top, ranks;
+  float* logp;
+  float* entropy;
+  float2* stats;
+  int32_t* top_ids;
+  float* top_logp;
+  int* err;
+};
+
+template <int TYPE>
+__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const ScoreArgs a) {
+  using L = Logits<TYPE>;
+  __shared__ Stats s_warp[kThreads / 32];
+  __shared__ Stats s_cta;                            // of the CTA, then of the row
+  __shared__ float s_group[kGroups];
+  __shared__ float s_bar;                            // what a candidate reaches
+  __shared__ int s_count;
+  __shared__ unsigned long long s_list[kListed];
+  __shared__ unsigned long long s_best[kMaxTop];     // the CTA's best, in order; 0: none
+  __shared__ unsigned long long s_all[8 * kMaxTop];  // those of the cluster
+  RT_PDL_LAUNCH_DEPENDENTS();
+  RT_PDL_WAIT();
+  const int rank = blockIdx.x % a.ranks, row = blockIdx.x / a.ranks;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Share<TYPE> share(static_cast<const typename L::T*>(a.logits) + row * a.pitch, a.vocab, rank, a.ranks);
+
+  Stats mine;
+  auto take = [&](const uint4& v) {
+    float x[L::kVec];
+    L::unpack(v, x);
+    float most = x[0];
+#pragma unroll
+    for (int j = 1; j < L::kVec; ++j) most = fmaxf(most, x[j]);
+    if (most > mine.m) mine.raise(most);
+    if (mine.m == -INFINITY) {  // nothing but -inf (or NaN) so far
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) mine.s += x[j] == x[j] ? 0.f : x[j];
+    } else {
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) mine.add(x[j]);
+    }
+  };
+  {
+    const uint4* p = share.vectors();
+    int i = share.lo + tid;
+    for (; i + 3 * kThreads < share.hi; i += 4 * kThreads) {
+      uint4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = __ldg(p + i + u * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) take(v[u]);
+    }
+    for (; i < share.hi; i += kThreads) take(__ldg(p + i));
+    if (tid < 2 * L::kVec) {
+      const int at = share.outside(tid);
+      if (at >= 0) {
+        const float z = L::one(share.row + at);
+        if (z > mine.m) mine.raise(z);
+        if (mine.m == -INFINITY) mine.s += z == z ? 0.f : z;
+        else mine.add(z);
+      }
+    }
+  }
+  const float my_most = mine.m;
+  {
+    float most = my_most;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if ((lane & 7) == 0) s_group[tid >> 3] = most;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats other;
+    other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
+    other.w = __shfl_xor_sync(0xffffffffu, mine.w, o);
+    mine.join(other);
+  }
+  if (lane == 0) s_warp[warp] = mine;
+  if (tid == 0) s_count = 0;
+  __syncthreads();
+  if (tid == 0) {
+    Stats all = s_warp[0];
+    for (int w = 1; w < kThreads / 32; ++w) all.join(s_warp[w]);
+    s_cta = all;
+  }
+  if (a.top > 0) {
+    if (tid < kGroups) {  // the top-th largest of the groups' maxima: equal ones by place
+      const float x = s_group[tid];
+      int before = 0;
+      for (int i = 0; i < kGroups; ++i) before += s_group[i] > x || (s_group[i] == x && i < tid);
+      if (before == a.top - 1) s_bar = x;
+    }
+    __syncthreads();
+    const float bar = s_bar;
+    if (my_most >= bar)
+      share.each_of_mine([&](float z, int index) {
+        if (z >= bar) {
+          const int at = atomicAdd(&s_count, 1);
+          if (at < kListed) s_list[at] = key_of(z, index);
+        }
+      });
+    if (tid < kMaxTop) s_best[tid] = 0;
+    __syncthreads();
+    const int count = s_count;
+    if (count <= kListed) {
+      for (int c = tid; c < count; c += kThreads) {
+        const unsigned long long key = s_list[c];
+        int before = 0;
+        for (int i = 0; i < count && before < a.top; ++i) before += s_list[i] > key;
+        if (before < a.top) s_best[before] = key;
+      }
+      __syncthreads();
+    } else {  // too many: one search for each place, for the best below the one before
+      unsigned long long last = ~0ull;
+      for (int k = 0; k < a.top; ++k) {
+        unsigned long long best = 0;
+        if (my_most >= bar)
+          share.each_of_mine([&](float z, int index) {
+            if (z >= bar) {
+              const unsigned long long key = key_of(z, index);
+              if (key < last) best = max_u64(best, key);
+            }
+          });
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) best = max_u64(best, __shfl_xor_sync(0xffffffffu, best, o));
+        if (lane == 0) s_list[warp] = best;
+        __syncthreads();
+        best = s_list[0];
+        for (int w = 1; w < kThreads / 32; ++w) best = max_u64(best, s_list[w]);
+        if (tid == 0) s_best[k] = best;
+        last = best;
+        __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
+  const unsigned long long* best = s_best;
+  if (a.ranks > 1) {
+    ptx::cluster_arrive();
+    ptx::cluster_wait();
+    if (rank == 0) {
+      auto peer = [](const void* p, int r) {
+        uint32_t at;
+        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(p)), "r"(r));
+        return at;
+      };
+      const int n = a.ranks * a.top;
+      if (tid < n) {
+        unsigned long long key;
+        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(peer(&s_best[tid % a.top], tid / a.top)) : "memory");
+        s_all[tid] = key;
+      }
+      if (warp == kThreads / 32 - 1) {
+        Stats x;
+        if (lane < a.ranks) {
+          const uint32_t at = peer(&s_cta, lane);
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.m) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.s) : "r"(at + 4) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.w) : "r"(at + 8) : "memory");
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+          Stats other;
+          other.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+          other.s = __shfl_xor_sync(0xffffffffu, x.s, o);
+          other.w = __shfl_xor_sync(0xffffffffu, x.w, o);
+          x.join(other);
+        }
+        if (lane == 0) s_warp[0] = x;
+      }
+      __syncthreads();
+      if (tid == 0) s_cta = s_warp[0];
+      if (tid < kMaxTop) s_best[tid] = 0;
+      __syncthreads();
+      if (tid < n) {
+        const unsigned long long key = s_all[tid];
+        int before = 0;
+        for (int i = 0; i < n; ++i) before += s_all[i] > key;
+        if (key != 0 && before < a.top) s_best[before] = key;
+      }
+      __syncthreads();
+    }
+    ptx::cluster_arrive();  // no CTA leaves while rank 0 reads its shared memory
+    ptx::cluster_wait();
+    if (rank != 0) return;
+  }
+  const Stats all = s_cta;
+  const bool nothing = all.m == -INFINITY && all.s == 0.f;  // a row of -inf
+  const float log_s = nothing ? 0.f : all.m == -INFINITY ? all.s : logf(all.s);
+  if (tid == 0) {
+    a.stats[row] = make_float2(all.m, log_s);
+    if (a.entropy) a.entropy[row] = nothing ? 0.f : log_s - all.w / all.s;
+    if (a.logp) {
+      const int t = a.targets[row];
+      float r = 0.f;
+      if (t >= a.vocab) {
+        atomicCAS(a.err, 0, kSiteToken);
+        r = NAN;
+      } else if (t >= 0) {
+        r = nothing ? -INFINITY : (L::one(share.row + t) - all.m) - log_s;
+      }
+      a.logp[row] = r;
+    }
+  }
+  if (tid < a.top) {
+    const unsigned long long key = best[tid];
+    const bool none = key == 0;  // fewer logits than places that are numbers
+    a.top_ids[static_cast<int64_t>(row) * a.top + tid] = none ? -1 : index_of(key);
+    a.top_logp[static_cast<int64_t>(row) * a.top + tid] =
+        none ? NAN : nothing ? -INFINITY : (value_of(key) - all.m) - log_s;
+  }
+}
+
+struct GradArgs {
+  void* out;
+  int64_t out_pitch;
+  const void* logits;
+  int64_t pitch;
+  const int32_t* targets;
+  const float2* stats;
+  const float* entropy;
+  const float* g_logp;
+  const float* g_entropy;
+  const int32_t* top_ids;
+  const float* g_top;
+  int vocab, top, chunks;
+  int* err;
+};
+
+constexpr int kGradVecs = 4;  // vectors of a thread
+
+template <int TYPE>
+__global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs a) {
+  using L = Logits<TYPE>;
+  using T = typename L::T;
+  RT_PDL_LAUNCH_DEPENDENTS();
+  RT_PDL_WAIT();
+  const int chunk = blockIdx.x % a.chunks, row = blockIdx.x / a.chunks;
+  const int tid = threadIdx.x;
+  const Share<TYPE> share(static_cast<const T*>(a.logits) + row * a.pitch, a.vocab, 0, 1);
+  T* out = static_cast<T*>(a.out) + row * a.out_pitch;
+  const float2 st = a.stats[row];
+  const int target = a.g_logp ? a.targets[row] : -1;
+  const bool given = target >= 0 && target < a.vocab;
+  if (target >= a.vocab && chunk == 0 && tid == 0) atomicCAS(a.err, 0, kSiteToken);
+  const float g_t = given ? a.g_logp[row] : 0.f;
+  float pull = g_t;
+  for (int j = 0; j < a.top; ++j) pull += a.g_top[static_cast<int64_t>(row) * a.top + j];
+  const float g_h = a.g_entropy ? a.g_entropy[row] : 0.f;
+  const float h = a.g_entropy ? a.entropy[row] : 0.f;
+  const bool nothing = st.x == -INFINITY;
+  auto grad = [&](float z) {
+    const float lp = (z - st.x) - st.y;
+    const float p = ex2(lp * kLog2e);
+    // p = 0 leaves nothing, whatever log p is
+    return lp == -INFINITY || nothing ? 0.f : -p * fmaf(g_h, lp + h, pull);
+  };
+  // columns with a term of their own, before anything is overwritten (out may be the logits)
+  int column = -1;
+  float special = 0.f;
+  const int first = share.head + chunk * 256 * kGradVecs * L::kVec;
+  const int behind = min(share.head + share.nv * L::kVec, first + 256 * kGradVecs * L::kVec);
+  if (tid <= a.top) {
+    column = tid == 0 ? (given ? target : -1) : a.top_ids[static_cast<int64_t>(row) * a.top + tid - 1];
+    if (column >= a.vocab) {
+      if (chunk == 0) atomicCAS(a.err, 0, kSiteToken);
+      column = -1;
+    }
+    const bool in_vectors = column >= share.head && column < share.head + share.nv * L::kVec;
+    const bool here = in_vectors ? column >= first && column < behind : chunk == 0;
+    if (!here) column = -1;
+    if (column >= 0) {
+      special = grad(L::one(share.row + column));
+      if (!nothing) {
+        if (given && column == target) special += g_t;
+        for (int j = 0; j < a.top; ++j)
+          if (a.top_ids[static_cast<int64_t>(row) * a.top + j] == column) special += a.g_top[static_cast<int64_t>(row) * a.top + j];
+      }
+    }
+  }
+  __syncthreads();
+  const uint4* src = share.vectors();
+  const bool aligned = (reinterpret_cast<uintptr_t>(out + share.head) & 15u) == 0;
+  const int v0 = chunk * 256 * kGradVecs + tid;
+  uint4 v[kGradVecs];
+#pragma unroll
+  for (int u = 0; u < kGradVecs; ++u)
+    if (v0 + u * 256 < share.nv) v[u] = src[v0 + u * 256];
+#pragma unroll
+  for (int u = 0; u < kGradVecs; ++u) {
+    const int i = v0 + u * 256;
+    if (i >= share.nv) break;
+    float x[L::kVec];
+    L::unpack(v[u], x);
+#pragma unroll
+    for (int j = 0; j < L::kVec; ++j) x[j] = grad(x[j]);
+    T* dst = out + share.head + static_cast<int64_t>(i) * L::kVec;
+    if (aligned) {
+      *reinterpret_cast<uint4*>(dst) = L::pack(x);
+    } else {
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) dst[j] = L::from(x[j]);
+    }
+  }
+  if (chunk == 0 && tid < 2 * L::kVec) {
+    const int at = share.outside(tid);
+    if (at >= 0) out[at] = L::from(grad(L::one(share.row + at)));
+  }
+  __syncthreads();
+  if (column >= 0) out[column] = L::from(special);
+}
+
+int type_size(int dtype) { return dtype == RT_F32 ? 4 : 2; }
+
+rt_status check_logits(const char* what, const void* logits, int64_t pitch, int rows, int vocab, int dtype) {
+  RT_REQUIRE(dtype == RT_F16 || dtype == RT_BF16 || dtype == RT_F32, RT_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
+  RT_REQUIRE(rows >= 0 && vocab > 0 && pitch >= vocab, RT_ERR_INVALID, "%s: need rows >= 0, vocab > 0 and a row pitch of at least that",
+             what);
+  RT_REQUIRE(vocab <= (1 << 30), RT_ERR_UNSUPPORTED, "%s: vocabulary of %d", what, vocab);
+  RT_REQUIRE(rows == 0 || logits, RT_ERR_INVALID, "%s: null pointer", what);
+  RT_REQUIRE(reinterpret_cast<uintptr_t>(logits) % type_size(dtype) == 0, RT_ERR_INVALID, "%s: misaligned logits", what);
+  return RT_OK;
+}
+
+}  // namespace
+}  // namespace rt
+
+using namespace rt;
+
+extern "C" rt_status rt_token_logprobs(const void* logits, int64_t pitch, const int32_t* targets, int rows, int vocab, int top,
+                                       float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp, int dtype,
+                                       void* stream) {
+  RT_TRY(check_logits("token_logprobs", logits, pitch, rows, vocab, dtype));
+  RT_REQUIRE(top >= 0 && top <= kMaxTop && top <= vocab, RT_ERR_UNSUPPORTED,
+             "token_logprobs: %d alternatives (0 to 32, at most the vocabulary)", top);
+  if (rows == 0) return RT_OK;
+  RT_REQUIRE(stats && (!logp || targets) && (top == 0 || (top_ids && top_logp)), RT_ERR_INVALID, "token_logprobs: null pointer");
+  RT_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7u) == 0, RT_ERR_INVALID, "token_logprobs: stats must be 8-byte aligned");
+  ScoreArgs a{logits, pitch, targets, rows, vocab, top, 1, logp, entropy, reinterpret_cast<float2*>(stats), top_ids, top_logp,
+              device_error_word()};
+  RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "token_logprobs: cannot allocate the device error word");
+  // few rows: several CTAs for each, as long as every thread has two vectors
+  const int vectors = vocab / (16 / type_size(dtype));
+  while (a.ranks < 8 && static_cast<int64_t>(rows) * a.ranks < 148 && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
+  RT_REQUIRE(static_cast<int64_t>(rows) * a.ranks < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+  auto kern = dtype == RT_F32 ? token_logprobs_kernel<RT_F32> : dtype == RT_BF16 ? token_logprobs_kernel<RT_BF16> : token_logprobs_kernel<RT_F16>;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * a.ranks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = a.ranks;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = a.ranks > 1 ? 2 : 1;
+  RT_CHECK_CUDA(cudaLaunchKernelEx(&cfg, kern, a));
+  count_launch();
+  RT_CHECK_CUDA(cudaGetLastError());
+  return RT_OK;
+}
+
+extern "C" rt_status rt_token_logprobs_backward(void* dlogits, int64_t out_pitch, const void* logits, int64_t pitch,
+                                                const int32_t* targets, const float* stats, const float* entropy, int rows, int vocab,
+                                                const float* g_logp, const float* g_entropy, int top, const int32_t* top_ids,
+                                                const float* g_top, int dtype, void* stream) {
+  RT_TRY(check_logits("token_logprobs_backward", logits, pitch, rows, vocab, dtype));
+  RT_REQUIRE(top >= 0 && top <= kMaxTop && top <= vocab, RT_ERR_UNSUPPORTED,
+             "token_logprobs_backward: %d alternatives (0 to 32, at most the vocabulary)", top);
+  RT_REQUIRE(out_pitch >= vocab, RT_ERR_INVALID, "token_logprobs_backward: the output's row pitch is below the vocabulary");
+  if (rows == 0) return RT_OK;
+  RT_REQUIRE(dlogits && stats && (!g_logp || targets) && (!g_entropy || entropy) && (top == 0 || (top_ids && g_top)), RT_ERR_INVALID,
+             "token_logprobs_backward: null pointer");
+  RT_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7u) == 0 && reinterpret_cast<uintptr_t>(dlogits) % type_size(dtype) == 0, RT_ERR_INVALID,
+             "token_logprobs_backward: misaligned stats or output");
+  RT_REQUIRE(dlogits != logits || out_pitch == pitch, RT_ERR_INVALID,
+             "token_logprobs_backward: in place, the output has the logits' row pitch");
+  GradArgs a{dlogits, out_pitch, logits, pitch, targets, reinterpret_cast<const float2*>(stats), entropy, g_logp, g_entropy, top_ids,
+             g_top, vocab, top, 1, device_error_word()};
+  RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "token_logprobs_backward: cannot allocate the device error word");
+  const int vec = 16 / type_size(dtype);
+  a.chunks = std::max(1, (vocab / vec + 256 * kGradVecs - 1) / (256 * kGradVecs));
+  RT_REQUIRE(static_cast<int64_t>(rows) * a.chunks < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "token_logprobs_backward: too many rows");
+  auto kern = dtype == RT_F32   ? token_logprobs_grad_kernel<RT_F32>
+              : dtype == RT_BF16 ? token_logprobs_grad_kernel<RT_BF16>
+                                 : token_logprobs_grad_kernel<RT_F16>;
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(rows * a.chunks)), dim3(256), 0, static_cast<cudaStream_t>(stream), a));
+  count_launch();
+  RT_CHECK_CUDA(cudaGetLastError());
+  return RT_OK;
+}

@@ -4,6 +4,7 @@ torch is used for device memory and streams only; every function launches one
 kernel of this library on the current torch stream and returns its output.
 """
 import ctypes as C
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -186,6 +187,188 @@ def sparse_attention_static(q, k, v, cfg, lens_tokens, kv_ptr, kv_idx, scale=1.0
     check(lib.rt_sparse_attention_static(_p(out), _p(q), _p(k), _p(v), C.byref(cfg), lens.ctypes.data_as(i32p),
                                          len(lens), kv_ptr.ctypes.data_as(i32p), kv_idx.ctypes.data_as(i32p),
                                          float(scale), _dt(q), _stream()))
+    return out
+
+
+# ---- answering from encoded documents: 8-bit key/value cache, attention over it, scores of tokens ------------------
+
+_KV_FORMATS = {torch.float8_e4m3fn: capi.RT_KV_E4M3, torch.int8: capi.RT_KV_INT8}
+_LOGIT_TYPES = {torch.float16: capi.RT_F16, torch.bfloat16: capi.RT_BF16, torch.float32: capi.RT_F32}
+
+
+def _need(cond, what):
+    if not cond:
+        raise ValueError(what)
+
+
+def _here(device):
+    """Kernels run on the current device's current stream: the tensors have to be there, too."""
+    if device.type != "cuda":
+        raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
+    if device.index != torch.cuda.current_device():
+        raise RuntimeError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _flat(t, name, dtype, shape, device):
+    """Address of a contiguous tensor of that type and shape on that device."""
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
+    if t.shape != shape or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+class KvCache:
+    """Keys and values in 8 bits: blocks of 64 tokens of one head, one fp32 scale for each block and head (rt_kv_cache).
+    k, v [blocks, kv_heads, 64, 64] float8_e4m3fn or int8; k_scale, v_scale fp32 [blocks, kv_heads]; value = code * scale.
+    Which blocks hold a sequence is the caller's block table, int32 [sequences, width]: entry j = block of tokens
+    64 j .. 64 j + 63.  Sequences may share blocks that none of them writes to."""
+
+    def __init__(self, k, v, k_scale, v_scale):
+        if k.dtype not in _KV_FORMATS:
+            raise TypeError(f"expected float8_e4m3fn or int8, got {k.dtype}")
+        _need(k.dim() == 4 and k.shape[2] == 64 and k.shape[3] == 64, "a cache is [blocks, kv_heads, 64, 64]")
+        if k.device.type != "cuda":
+            raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.blocks, self.kv_heads, self.device = k.shape[0], k.shape[1], k.device
+        two = k.shape[:2]
+        self._c = capi.RtKvCache(_flat(k, "k", k.dtype, k.shape, k.device), _flat(v, "v", k.dtype, k.shape, k.device),
+                                 _flat(k_scale, "k_scale", torch.float32, two, k.device),
+                                 _flat(v_scale, "v_scale", torch.float32, two, k.device), self.blocks, self.kv_heads,
+                                 _KV_FORMATS[k.dtype], 0)
+        self._ref = C.byref(self._c)
+
+    @staticmethod
+    def empty(blocks, kv_heads, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache without tokens.  What its blocks hold before they are written to is never used."""
+        k, v = (torch.empty(blocks, kv_heads, 64, 64, dtype=dtype, device=device) for _ in range(2))
+        return KvCache(k, v, *(torch.empty(blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _table(block_table, lengths, first, device):
+    """The arguments that say which tokens a call is about, as addresses and sizes."""
+    n = lengths.shape[0]
+    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "a block table is [sequences, width]")
+    return (_flat(block_table, "block table", torch.int32, (n, block_table.shape[1]), device), block_table.shape[1],
+            _flat(lengths, "lengths", torch.int32, (n,), device), _flat(first, "first rows", torch.int32, (n + 1,), device), n)
+
+
+def kv_cache_write(cache, k, v, block_table, start, first, max_tokens=None, head_major=False):
+    """Quantises new tokens into the cache (rt_kv_cache_write; the rule for the scales stands there).
+    k, v [tokens, kv_heads, 64] 16-bit, rows may be strided (columns of a projection); head_major: the buffers of
+    gemm_qkv / qkv_bias_transpose instead, [tokens, kv_heads * 64] storage.  Sequence s writes rows first[s] .. first[s + 1] - 1 to
+    its positions from start[s] on (int32 device tensors).  max_tokens: the most new tokens of one sequence (default: all rows)."""
+    _here(cache.device)
+    dt = _dt(k)
+    tokens = k.shape[0]
+    if head_major:
+        shape = (tokens, cache.kv_heads * 64)
+        kp, vp, ts, hs = _flat(k, "k", k.dtype, shape, cache.device), _flat(v, "v", k.dtype, shape, cache.device), 0, 0
+    else:
+        _need(k.dim() == 3 and k.shape[1:] == (cache.kv_heads, 64) and k.shape == v.shape and k.stride() == v.stride() and
+              k.stride(2) == 1 and k.dtype == v.dtype and k.device == v.device == cache.device,
+              "k and v: expected [tokens, kv_heads, 64] of the same type and strides, on the cache's device")
+        kp, vp, ts, hs = k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)
+        if ts == 0:
+            _need(tokens <= 1, "k and v: rows without a stride")
+            ts = 64 * cache.kv_heads
+    tp, width, sp, fp, n = _table(block_table, start, first, cache.device)
+    check(lib.rt_kv_cache_write(cache._ref, kp, vp, ts, hs, tp, width, sp, fp, n, tokens, tokens if max_tokens is None else max_tokens,
+                                dt, _stream()))
+
+
+def kv_cache_read(cache, block_table, start, first, tokens, dtype, max_tokens=None, out=None):
+    """Values of the positions from start[s] on, in 16 bits: (k, v), each [tokens, kv_heads, 64]; sequence s fills rows
+    first[s] .. first[s + 1] - 1 (rt_kv_cache_read)."""
+    _here(cache.device)
+    shape = (tokens, cache.kv_heads, 64)
+    if out is None:
+        out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+    k, v = out
+    tp, width, sp, fp, n = _table(block_table, start, first, cache.device)
+    check(lib.rt_kv_cache_read(cache._ref, _flat(k, "k", dtype, shape, cache.device), _flat(v, "v", dtype, shape, cache.device), tp,
+                               width, sp, fp, n, tokens, tokens if max_tokens is None else max_tokens, _dt(k), _stream()))
+    return k, v
+
+
+def cached_attention(q, cache, block_table, context, first, max_q=None, max_context=0, scale=1.0, causal=False, out=None):
+    """softmax(scale * q k^T) v over the cached tokens (rt_cached_attention): q [tokens, heads, 64], rows may be strided; returns
+    [tokens, heads, 64].  Sequence s has the query rows first[s] .. first[s + 1] - 1 and context[s] cached tokens; causal: its
+    rows are its last tokens, row i of n sees the first context - n + i + 1.  max_q: the most query rows of one sequence (default:
+    all rows); max_context only guides how the work is split."""
+    _here(cache.device)
+    dt = _dt(q)
+    _need(q.dim() == 3 and q.shape[2] == 64 and q.stride(2) == 1 and (q.stride(1) == 64 or q.shape[1] == 1) and q.device == cache.device,
+          "q: expected [tokens, heads, 64] with adjacent heads, on the cache's device")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    tp, width, cp, fp, n = _table(block_table, context, first, cache.device)
+    check(lib.rt_cached_attention(_flat(out, "out", q.dtype, q.shape, q.device), q.data_ptr(), q.stride(0), cache._ref, tp, width, cp,
+                                  fp, n, q.shape[0], q.shape[0] if max_q is None else max_q, max_context, q.shape[1], scale, causal, dt,
+                                  _stream()))
+    return out
+
+
+class TokenScores(NamedTuple):
+    """What token_logprobs returns, fp32 (top_ids int32): logp and entropy [rows], stats [rows, 2], top_ids and top_logp
+    [rows, top_k]; None what was not asked for."""
+    logp: Optional[torch.Tensor]
+    entropy: torch.Tensor
+    stats: torch.Tensor
+    top_ids: Optional[torch.Tensor]
+    top_logp: Optional[torch.Tensor]
+
+
+def _logits(z, name="logits"):
+    if z.dtype not in _LOGIT_TYPES:
+        raise TypeError(f"{name}: expected float16, bfloat16 or float32, got {z.dtype}")
+    _here(z.device)
+    rows, vocab = z.shape
+    _need(vocab == 1 or z.stride(1) == 1, f"{name}: expected rows of adjacent values")
+    pitch = z.stride(0) if rows > 1 else max(z.stride(0), vocab)
+    return rows, vocab, pitch, _LOGIT_TYPES[z.dtype]
+
+
+def token_logprobs(logits, targets=None, top_k=0):
+    """Log probabilities of given tokens, entropy and the top_k (0 to 32) best alternatives of each row of logits [rows, vocab]
+    (rt_token_logprobs).  targets int32 [rows], negative: no token given, its logp is 0; None: no logp."""
+    rows, vocab, pitch, dt = _logits(logits)
+    dev = logits.device
+    tp = None if targets is None else _flat(targets, "targets", torch.int32, (rows,), dev)
+    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
+    logp, entropy, stats = None if tp is None else new(rows), new(rows), new(rows, 2)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
+    best = new(rows, top_k) if top_k > 0 else None
+    check(lib.rt_token_logprobs(logits.data_ptr(), pitch, tp, rows, vocab, top_k, None if logp is None else logp.data_ptr(),
+                                entropy.data_ptr(), stats.data_ptr(), None if ids is None else ids.data_ptr(),
+                                None if best is None else best.data_ptr(), dt, _stream()))
+    return TokenScores(logp, entropy, stats, ids, best)
+
+
+def token_logprobs_backward(logits, targets, stats, entropy=None, grad_logp=None, grad_entropy=None, top_ids=None, grad_top=None,
+                            out=None):
+    """Gradient of token_logprobs' logp, entropy and top_logp with respect to the logits (rt_token_logprobs_backward), in their type.
+    grad_logp, grad_entropy fp32 [rows], grad_top fp32 [rows, k] for top_ids; None: no such term.  out may be the logits."""
+    rows, vocab, pitch, dt = _logits(logits)
+    dev = logits.device
+    if out is None:
+        # the logits' own row pitch: rows then have the same alignment
+        out = torch.empty((rows, pitch), dtype=logits.dtype, device=dev)[:, :vocab]
+    _need(out.shape == logits.shape and out.device == dev, "out: expected the logits' shape and device")
+    if out.dtype != logits.dtype:
+        raise TypeError(f"out: expected {logits.dtype}, got {out.dtype}")
+    out_pitch = _logits(out, "out")[2]
+    f = lambda t, name, *shape: None if t is None else _flat(t, name, torch.float32, shape, dev)  # noqa: E731
+    top = 0 if grad_top is None else grad_top.shape[1]
+    _need(grad_logp is None or targets is not None, "grad_logp needs the targets")
+    _need(grad_entropy is None or entropy is not None, "grad_entropy needs the entropy")
+    _need(top == 0 or top_ids is not None, "grad_top needs top_ids")
+    check(lib.rt_token_logprobs_backward(
+        out.data_ptr(), out_pitch, logits.data_ptr(), pitch,
+        None if targets is None else _flat(targets, "targets", torch.int32, (rows,), dev), f(stats, "stats", rows, 2),
+        f(entropy, "entropy", rows), rows, vocab, f(grad_logp, "grad_logp", rows), f(grad_entropy, "grad_entropy", rows), top,
+        None if top == 0 else _flat(top_ids, "top_ids", torch.int32, (rows, top), dev), f(grad_top, "grad_top", rows, top), dt, _stream()))
     return out
 
 
