@@ -15,7 +15,7 @@
 // bf16 queries are turned into halves scaled by a power of two per row (largest entry in [2^14, 2^15)): exact but for
 // entries 2^-28 below the row's largest.  Probabilities are rounded to halves (2^-11 relative) for the second product; their
 // sum is taken in fp32 before.
-#include "kv_cache.cuh"
+#include "cached_attention.h"
 
 #include <algorithm>
 
@@ -28,21 +28,9 @@ namespace rt {
 namespace {
 
 constexpr int kWarps = 8;
+constexpr int kFewRows = 64;  // rows of a sequence and key head up to which this kernel is taken
 
-struct Args {
-  uint16_t* out;
-  const uint16_t* q;
-  int64_t q_stride;
-  KvView cache;
-  const int32_t* table;
-  int table_stride;
-  const int32_t* context;
-  const int32_t* first;
-  int tokens, max_q, heads, group, tiles, splits;
-  float scale_log2;
-  int causal;
-  int* err;
-};
+using Args = CachedAttentionArgs;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -55,22 +43,6 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint32_t peer_address(uint32_t addr, int rank) {
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
-  return r;
 }
 
 // 16 dimensions [16 t, 16 t + 16) of one query row as eight half2, and the power of two that they were multiplied with.
@@ -92,15 +64,14 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int t, uint32_t
     for (int i = 0; i < 8; ++i) most = max(most, max((p[i] << 16) & 0x7fffffffu, p[i] & 0x7fff0000u));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = static_cast<int>(most >> 23);                              // biased exponent
-    const int up = e == 255 ? 0 : max(-126, min(126, 127 + 14 - e));         // infinities and NaN pass as they are
-    const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);  // 2^up
+    const int up = kv::query_shift(most);
+    const float f = kv::pow2(up);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float2 x = kv::unpack16<true>(p[i]);
       h[i] = kv::pack16<false>(x.x * f, x.y * f);
     }
-    return __uint_as_float(static_cast<uint32_t>(127 - up) << 23);
+    return kv::pow2(-up);
   }
 }
 
@@ -120,24 +91,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
   const int head = rest % a.cache.heads, seq = rest / a.cache.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-  const int f0 = a.first[seq], f1 = a.first[seq + 1];
-  const int n = f1 - f0;
-  int ctx = a.context[seq];
-  if (n <= 0) return;
-  if (f0 < 0 || f1 > a.tokens || n > a.max_q || ctx < 0 || ctx > static_cast<int64_t>(a.table_stride) * 64) {
-    if (threadIdx.x == 0) kv::index_error(a.err, kSiteCachedAttention);
-    return;
-  }
-  const int rows = n * a.group, row0 = tile * 16;
+  const CachedRows seq_rows(a, seq);
+  if (!seq_rows.ok) return;
+  const int rows = seq_rows.rows, row0 = tile * 16;
   if (row0 >= rows) return;
-  // keys that a row sees
-  auto limit_of = [&](int row) {
-    if (row >= rows) return 0;
-    return a.causal ? max(0, ctx - n + row / a.group + 1) : ctx;
-  };
-  auto q_row = [&](int row) {
-    return a.q + (f0 + row / a.group) * a.q_stride + (head * a.group + row % a.group) * 64;
-  };
+  auto limit_of = [&](int row) { return row < rows ? seq_rows.limit(a, row) : 0; };  // keys that a row sees
   const int least = limit_of(row0), most = limit_of(min(row0 + 16, rows) - 1);
   const int lim0 = limit_of(row0 + g), lim1 = limit_of(row0 + g + 8);
   const bool two = row0 + 8 < rows;  // the tile's upper eight rows are in use
@@ -146,8 +104,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
   float unit0, unit1;
   {
     uint32_t lo[8], hi[8];
-    unit0 = load_query<BF16>(row0 + g < rows ? q_row(row0 + g) : nullptr, t, lo);
-    unit1 = load_query<BF16>(row0 + g + 8 < rows ? q_row(row0 + g + 8) : nullptr, t, hi);
+    unit0 = load_query<BF16>(row0 + g < rows ? seq_rows.query(a, head, row0 + g) : nullptr, t, lo);
+    unit1 = load_query<BF16>(row0 + g + 8 < rows ? seq_rows.query(a, head, row0 + g + 8) : nullptr, t, hi);
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       q[s][0] = lo[2 * s];
@@ -303,11 +261,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
   __syncthreads();
   auto store = [&](int r, int d, float4 v, float l) {
     const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // NaN stays
-    const int row = row0 + r;
     uint2 w;
     w.x = kv::pack16<BF16>(v.x * inv, v.y * inv);
     w.y = kv::pack16<BF16>(v.z * inv, v.w * inv);
-    *reinterpret_cast<uint2*>(a.out + static_cast<int64_t>(f0 + row / a.group) * a.heads * 64 + (head * a.group + row % a.group) * 64 + d) = w;
+    *reinterpret_cast<uint2*>(seq_rows.output(a, head, row0 + r) + d) = w;
   };
   const int valid = min(16, rows - row0);
   const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
@@ -345,11 +302,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
     const uint32_t ml_at = ptx::smem_u32(&s_sum_ml[rr]), o_at = ptx::smem_u32(&s_sum[rr][dd]);
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
-    for (int w = 0; w < a.splits; ++w) M = fmaxf(M, ld_cluster_f2(peer_address(ml_at, w)).x);
+    for (int w = 0; w < a.splits; ++w) M = fmaxf(M, kv::ld_cluster_f2(kv::peer_address(ml_at, w)).x);
     const float ref = M == -INFINITY ? 0.f : M;
     for (int w = 0; w < a.splits; ++w) {
-      const float2 ml = ld_cluster_f2(peer_address(ml_at, w));
-      const float4 x = ld_cluster_f4(peer_address(o_at, w));
+      const float2 ml = kv::ld_cluster_f2(kv::peer_address(ml_at, w));
+      const float4 x = kv::ld_cluster_f4(kv::peer_address(o_at, w));
       const float f = ex2(ml.x - ref);
       L = fmaf(ml.y, f, L);
       v.x = fmaf(x.x, f, v.x);
@@ -363,10 +320,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
   ptx::cluster_wait();
 }
 
-rt_status launch_few_rows(const Args& a, int n_seq, bool bf16, bool int8, cudaStream_t st) {
+rt_status launch_few_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) {
   auto kern = bf16 ? (int8 ? few_rows_kernel<true, true> : few_rows_kernel<true, false>)
                    : (int8 ? few_rows_kernel<false, true> : few_rows_kernel<false, false>);
-  const int64_t grid = static_cast<int64_t>(n_seq) * a.cache.heads * a.tiles * a.splits;
+  const int64_t grid = static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kWarps * 32);
@@ -414,12 +371,15 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   a.table_stride = table_stride;
   a.context = context;
   a.first = first;
+  a.n_seq = n_seq;
   a.tokens = tokens;
   a.max_q = max_q;
   a.heads = heads;
   a.group = heads / a.cache.heads;
   RT_REQUIRE(static_cast<int64_t>(max_q) * a.group < (int64_t{1} << 30), RT_ERR_UNSUPPORTED, "cached_attention: too many query rows");
-  a.tiles = (max_q * a.group + 15) / 16;
+  const int rows = max_q * a.group;
+  const bool many = rows > kFewRows;
+  a.tiles = many ? (rows + 255) / 256 : (rows + 15) / 16;
   const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
   RT_REQUIRE(heads_of_all < (int64_t{1} << 28) && heads_of_all * a.tiles < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
              "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
@@ -429,9 +389,11 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "cached_attention: cannot allocate the device error word");
   const int64_t widest = static_cast<int64_t>(table_stride) * 64;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
-  // as many CTAs per tile as fill the chip, with a block for every warp
-  int splits = 1;
-  while (splits < 8 && static_cast<int64_t>(n_seq) * a.cache.heads * a.tiles * splits < 148 * 2 && keys > 64 * kWarps * splits) splits *= 2;
-  a.splits = splits;
-  return launch_few_rows(a, n_seq, dtype == RT_BF16, cache->format == RT_KV_INT8, static_cast<cudaStream_t>(stream));
+  // as many CTAs per tile as fill the chip, with work for every warp
+  const int64_t full = many ? 148 : 2 * 148, least = many ? 512 : 64 * kWarps;
+  a.splits = 1;
+  while (a.splits < 8 && heads_of_all * a.tiles * a.splits < full && keys > least * a.splits) a.splits *= 2;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool bf16 = dtype == RT_BF16, int8 = cache->format == RT_KV_INT8;
+  return many ? launch_cached_attention_many_rows(a, bf16, int8, st) : launch_few_rows(a, bf16, int8, st);
 }

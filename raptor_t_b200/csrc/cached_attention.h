@@ -1,0 +1,86 @@
+// Arguments of the kernels behind rt_cached_attention (cached_attention.cu: few query rows, cached_attention_sm100.cu: many).
+#pragma once
+#include "device_error.h"
+#include "kv_cache.cuh"
+
+namespace rt {
+
+struct CachedAttentionArgs {
+  uint16_t* out;
+  const uint16_t* q;
+  int64_t q_stride;
+  KvView cache;
+  const int32_t* table;
+  int table_stride;
+  const int32_t* context;
+  const int32_t* first;
+  int n_seq, tokens, max_q, heads, group;  // group: query heads of a key head
+  int tiles;                               // row tiles of the longest sequence
+  int splits;                              // CTAs of a cluster that share a tile's keys
+  float scale_log2;
+  int causal;
+  int* err;
+};
+
+// What one sequence of a call is: its query rows and how many keys each of them sees.
+struct CachedRows {
+  int f0, n, ctx, rows;
+  bool ok;
+  __device__ __forceinline__ CachedRows(const CachedAttentionArgs& a, int seq) {
+    f0 = a.first[seq];
+    const int f1 = a.first[seq + 1];
+    ctx = a.context[seq];
+    ok = f1 > f0;
+    n = rows = 0;
+    if (!ok) return;
+    if (f0 < 0 || f1 > a.tokens || f1 - f0 > a.max_q || ctx < 0 || ctx > static_cast<int64_t>(a.table_stride) * 64) {
+      if (threadIdx.x == 0) kv::index_error(a.err, kSiteCachedAttention);
+      ok = false;
+      return;
+    }
+    n = f1 - f0;
+    rows = n * a.group;
+  }
+  __device__ __forceinline__ int limit(const CachedAttentionArgs& a, int row) const {
+    return a.causal ? max(0, ctx - n + row / a.group + 1) : ctx;
+  }
+  __device__ __forceinline__ const uint16_t* query(const CachedAttentionArgs& a, int head, int row) const {
+    return a.q + (f0 + row / a.group) * a.q_stride + (head * a.group + row % a.group) * 64;
+  }
+  __device__ __forceinline__ uint16_t* output(const CachedAttentionArgs& a, int head, int row) const {
+    return a.out + (static_cast<int64_t>(f0 + row / a.group) * a.heads + head * a.group + row % a.group) * 64;
+  }
+};
+
+namespace kv {
+
+// 2^up that brings a row's largest magnitude (its bf16 or fp32 bits, sign removed) into [2^14, 2^15), so that the row can be
+// held in halves; infinities and NaN pass as they are.
+__device__ __forceinline__ int query_shift(uint32_t most) {
+  const int e = static_cast<int>(most >> 23);  // biased exponent
+  return e == 255 ? 0 : max(-126, min(126, 127 + 14 - e));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float(static_cast<uint32_t>(127 + e) << 23); }
+
+__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+// The address of the same variable in CTA `rank` of the cluster.
+__device__ __forceinline__ uint32_t peer_address(uint32_t addr, int rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+
+}  // namespace kv
+
+rt_status launch_cached_attention_many_rows(const CachedAttentionArgs& a, bool bf16, bool int8, cudaStream_t st);
+
+}  // namespace rt

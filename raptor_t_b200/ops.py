@@ -31,7 +31,8 @@ def _p(t):
 
 
 def _stream():
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the handle alone: an object of class Stream for it costs 3 us a call
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 def bias_residual_layernorm(x, bias, residual, gamma, beta, eps, out=None):
@@ -201,21 +202,23 @@ def _need(cond, what):
         raise ValueError(what)
 
 
-def _here(device):
-    """Kernels run on the current device's current stream: the tensors have to be there, too."""
-    if device.type != "cuda":
+def _here(index):
+    """Kernels run on the current device's current stream: the tensors have to be there, too.  Returns the stream."""
+    if index < 0:
         raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
-    if device.index != torch.cuda.current_device():
-        raise RuntimeError(f"tensors on {device}, but the current device is cuda:{torch.cuda.current_device()}")
+    if index != torch._C._cuda_getDevice():
+        raise RuntimeError(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
-def _flat(t, name, dtype, shape, device):
+def _flat(t, name, dtype, shape, index):
     """Address of a contiguous tensor of that type and shape on that device."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+        return t.data_ptr()
     if t.dtype != dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    if t.shape != shape or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)} on {device}, got {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)} on cuda:{index}, got {tuple(t.shape)} "
+                     f"with strides {t.stride()} on {t.device}")
 
 
 class KvCache:
@@ -232,12 +235,12 @@ class KvCache:
             raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.blocks, self.kv_heads, self.device = k.shape[0], k.shape[1], k.device
-        two = k.shape[:2]
-        self._c = capi.RtKvCache(_flat(k, "k", k.dtype, k.shape, k.device), _flat(v, "v", k.dtype, k.shape, k.device),
-                                 _flat(k_scale, "k_scale", torch.float32, two, k.device),
-                                 _flat(v_scale, "v_scale", torch.float32, two, k.device), self.blocks, self.kv_heads,
+        two, at = k.shape[:2], k.get_device()
+        self._c = capi.RtKvCache(_flat(k, "k", k.dtype, k.shape, at), _flat(v, "v", k.dtype, k.shape, at),
+                                 _flat(k_scale, "k_scale", torch.float32, two, at),
+                                 _flat(v_scale, "v_scale", torch.float32, two, at), self.blocks, self.kv_heads,
                                  _KV_FORMATS[k.dtype], 0)
-        self._ref = C.byref(self._c)
+        self._ref, self._at, self._row = C.byref(self._c), at, (self.kv_heads, 64)
 
     @staticmethod
     def empty(blocks, kv_heads, dtype=torch.float8_e4m3fn, device="cuda"):
@@ -246,12 +249,11 @@ class KvCache:
         return KvCache(k, v, *(torch.empty(blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _table(block_table, lengths, first, device):
+def _table(block_table, lengths, first, index):
     """The arguments that say which tokens a call is about, as addresses and sizes."""
-    n = lengths.shape[0]
-    _need(block_table.dim() == 2 and block_table.shape[1] > 0, "a block table is [sequences, width]")
-    return (_flat(block_table, "block table", torch.int32, (n, block_table.shape[1]), device), block_table.shape[1],
-            _flat(lengths, "lengths", torch.int32, (n,), device), _flat(first, "first rows", torch.int32, (n + 1,), device), n)
+    n, width = lengths.shape[0], block_table.shape[-1]
+    return (_flat(block_table, "block table", torch.int32, (n, width), index), width,
+            _flat(lengths, "lengths", torch.int32, (n,), index), _flat(first, "first rows", torch.int32, (n + 1,), index), n)
 
 
 def kv_cache_write(cache, k, v, block_table, start, first, max_tokens=None, head_major=False):
@@ -259,37 +261,40 @@ def kv_cache_write(cache, k, v, block_table, start, first, max_tokens=None, head
     k, v [tokens, kv_heads, 64] 16-bit, rows may be strided (columns of a projection); head_major: the buffers of
     gemm_qkv / qkv_bias_transpose instead, [tokens, kv_heads * 64] storage.  Sequence s writes rows first[s] .. first[s + 1] - 1 to
     its positions from start[s] on (int32 device tensors).  max_tokens: the most new tokens of one sequence (default: all rows)."""
-    _here(cache.device)
-    dt = _dt(k)
-    tokens = k.shape[0]
+    at = cache._at
+    st = _here(at)
+    dt, tokens = _dt(k), k.shape[0]
     if head_major:
         shape = (tokens, cache.kv_heads * 64)
-        kp, vp, ts, hs = _flat(k, "k", k.dtype, shape, cache.device), _flat(v, "v", k.dtype, shape, cache.device), 0, 0
+        kp, vp, ts, hs = _flat(k, "k", k.dtype, shape, at), _flat(v, "v", k.dtype, shape, at), 0, 0
     else:
-        _need(k.dim() == 3 and k.shape[1:] == (cache.kv_heads, 64) and k.shape == v.shape and k.stride() == v.stride() and
-              k.stride(2) == 1 and k.dtype == v.dtype and k.device == v.device == cache.device,
-              "k and v: expected [tokens, kv_heads, 64] of the same type and strides, on the cache's device")
-        kp, vp, ts, hs = k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1)
+        strides = k.stride()
+        if not (len(strides) == 3 and strides[2] == 1 and v.stride() == strides and k.shape == v.shape == (tokens, *cache._row) and
+                v.dtype is k.dtype and k.get_device() == v.get_device() == at):
+            raise ValueError("k and v: expected [tokens, kv_heads, 64] of the same type and strides, on the cache's device")
+        kp, vp, ts, hs = k.data_ptr(), v.data_ptr(), strides[0], strides[1]
         if ts == 0:
             _need(tokens <= 1, "k and v: rows without a stride")
             ts = 64 * cache.kv_heads
-    tp, width, sp, fp, n = _table(block_table, start, first, cache.device)
+    tp, width, sp, fp, n = _table(block_table, start, first, at)
     check(lib.rt_kv_cache_write(cache._ref, kp, vp, ts, hs, tp, width, sp, fp, n, tokens, tokens if max_tokens is None else max_tokens,
-                                dt, _stream()))
+                                dt, st))
 
 
 def kv_cache_read(cache, block_table, start, first, tokens, dtype, max_tokens=None, out=None):
     """Values of the positions from start[s] on, in 16 bits: (k, v), each [tokens, kv_heads, 64]; sequence s fills rows
     first[s] .. first[s + 1] - 1 (rt_kv_cache_read)."""
-    _here(cache.device)
-    shape = (tokens, cache.kv_heads, 64)
+    at = cache._at
+    st = _here(at)
+    shape = (tokens, *cache._row)
     if out is None:
-        out = tuple(torch.empty(shape, dtype=dtype, device=cache.device) for _ in range(2))
+        k = torch.empty(shape, dtype=dtype, device=cache.device)
+        out = (k, torch.empty_like(k))
     k, v = out
-    tp, width, sp, fp, n = _table(block_table, start, first, cache.device)
-    check(lib.rt_kv_cache_read(cache._ref, _flat(k, "k", dtype, shape, cache.device), _flat(v, "v", dtype, shape, cache.device), tp,
-                               width, sp, fp, n, tokens, tokens if max_tokens is None else max_tokens, _dt(k), _stream()))
-    return k, v
+    tp, width, sp, fp, n = _table(block_table, start, first, at)
+    check(lib.rt_kv_cache_read(cache._ref, _flat(k, "k", dtype, shape, at), _flat(v, "v", dtype, shape, at), tp, width, sp, fp, n,
+                               tokens, tokens if max_tokens is None else max_tokens, _dt(k), st))
+    return out
 
 
 def cached_attention(q, cache, block_table, context, first, max_q=None, max_context=0, scale=1.0, causal=False, out=None):
@@ -297,16 +302,18 @@ def cached_attention(q, cache, block_table, context, first, max_q=None, max_cont
     [tokens, heads, 64].  Sequence s has the query rows first[s] .. first[s + 1] - 1 and context[s] cached tokens; causal: its
     rows are its last tokens, row i of n sees the first context - n + i + 1.  max_q: the most query rows of one sequence (default:
     all rows); max_context only guides how the work is split."""
-    _here(cache.device)
+    at = cache._at
+    st = _here(at)
     dt = _dt(q)
-    _need(q.dim() == 3 and q.shape[2] == 64 and q.stride(2) == 1 and (q.stride(1) == 64 or q.shape[1] == 1) and q.device == cache.device,
-          "q: expected [tokens, heads, 64] with adjacent heads, on the cache's device")
+    tokens, heads, dim = q.shape
+    qs, hs, ds = q.stride()
+    if not (dim == 64 and ds == 1 and (hs == 64 or heads == 1) and q.get_device() == at):
+        raise ValueError("q: expected [tokens, heads, 64] with adjacent heads, on the cache's device")
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    tp, width, cp, fp, n = _table(block_table, context, first, cache.device)
-    check(lib.rt_cached_attention(_flat(out, "out", q.dtype, q.shape, q.device), q.data_ptr(), q.stride(0), cache._ref, tp, width, cp,
-                                  fp, n, q.shape[0], q.shape[0] if max_q is None else max_q, max_context, q.shape[1], scale, causal, dt,
-                                  _stream()))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    tp, width, cp, fp, n = _table(block_table, context, first, at)
+    check(lib.rt_cached_attention(_flat(out, "out", q.dtype, q.shape, at), q.data_ptr(), qs, cache._ref, tp, width, cp, fp, n, tokens,
+                                  tokens if max_q is None else max_q, max_context, heads, scale, causal, dt, st))
     return out
 
 
@@ -321,28 +328,33 @@ class TokenScores(NamedTuple):
 
 
 def _logits(z, name="logits"):
-    if z.dtype not in _LOGIT_TYPES:
+    dt = _LOGIT_TYPES.get(z.dtype)
+    if dt is None:
         raise TypeError(f"{name}: expected float16, bfloat16 or float32, got {z.dtype}")
-    _here(z.device)
     rows, vocab = z.shape
-    _need(vocab == 1 or z.stride(1) == 1, f"{name}: expected rows of adjacent values")
-    pitch = z.stride(0) if rows > 1 else max(z.stride(0), vocab)
-    return rows, vocab, pitch, _LOGIT_TYPES[z.dtype]
+    pitch, step = z.stride()
+    _need(step == 1 or vocab == 1, f"{name}: expected rows of adjacent values")
+    return rows, vocab, pitch if rows > 1 else max(pitch, vocab), dt
 
 
 def token_logprobs(logits, targets=None, top_k=0):
     """Log probabilities of given tokens, entropy and the top_k (0 to 32) best alternatives of each row of logits [rows, vocab]
     (rt_token_logprobs).  targets int32 [rows], negative: no token given, its logp is 0; None: no logp."""
     rows, vocab, pitch, dt = _logits(logits)
-    dev = logits.device
-    tp = None if targets is None else _flat(targets, "targets", torch.int32, (rows,), dev)
-    new = lambda *shape: torch.empty(shape, dtype=torch.float32, device=dev)  # noqa: E731
-    logp, entropy, stats = None if tp is None else new(rows), new(rows), new(rows, 2)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev) if top_k > 0 else None
-    best = new(rows, top_k) if top_k > 0 else None
-    check(lib.rt_token_logprobs(logits.data_ptr(), pitch, tp, rows, vocab, top_k, None if logp is None else logp.data_ptr(),
-                                entropy.data_ptr(), stats.data_ptr(), None if ids is None else ids.data_ptr(),
-                                None if best is None else best.data_ptr(), dt, _stream()))
+    at = logits.get_device()
+    st = _here(at)
+    # empty_like and new_empty cost the host 1.3 and 1.8 us a tensor, torch.empty 2.2
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
+    entropy = stats.new_empty(rows)
+    tp = logp = ids = best = lp = ip = bp = None
+    if targets is not None:
+        tp, logp = _flat(targets, "targets", torch.int32, (rows,), at), torch.empty_like(entropy)
+        lp = logp.data_ptr()
+    if top_k > 0:
+        best = stats.new_empty((rows, top_k))
+        ids = torch.empty_like(best, dtype=torch.int32)
+        ip, bp = ids.data_ptr(), best.data_ptr()
+    check(lib.rt_token_logprobs(logits.data_ptr(), pitch, tp, rows, vocab, top_k, lp, entropy.data_ptr(), stats.data_ptr(), ip, bp, dt, st))
     return TokenScores(logp, entropy, stats, ids, best)
 
 
@@ -351,24 +363,31 @@ def token_logprobs_backward(logits, targets, stats, entropy=None, grad_logp=None
     """Gradient of token_logprobs' logp, entropy and top_logp with respect to the logits (rt_token_logprobs_backward), in their type.
     grad_logp, grad_entropy fp32 [rows], grad_top fp32 [rows, k] for top_ids; None: no such term.  out may be the logits."""
     rows, vocab, pitch, dt = _logits(logits)
-    dev = logits.device
+    at = logits.get_device()
+    st = _here(at)
     if out is None:
         # the logits' own row pitch: rows then have the same alignment
-        out = torch.empty((rows, pitch), dtype=logits.dtype, device=dev)[:, :vocab]
-    _need(out.shape == logits.shape and out.device == dev, "out: expected the logits' shape and device")
+        out = torch.empty((rows, pitch), dtype=logits.dtype, device=logits.device)
+        if pitch != vocab:
+            out = out[:, :vocab]
+    if out.shape != logits.shape or out.get_device() != at:
+        raise ValueError("out: expected the logits' shape and device")
     if out.dtype != logits.dtype:
         raise TypeError(f"out: expected {logits.dtype}, got {out.dtype}")
     out_pitch = _logits(out, "out")[2]
-    f = lambda t, name, *shape: None if t is None else _flat(t, name, torch.float32, shape, dev)  # noqa: E731
-    top = 0 if grad_top is None else grad_top.shape[1]
+    f = lambda t, name, shape: None if t is None else _flat(t, name, torch.float32, shape, at)  # noqa: E731
+    top, ip = 0, None
+    if grad_top is not None and grad_top.shape[1] > 0:
+        top = grad_top.shape[1]
+        _need(top_ids is not None, "grad_top needs top_ids")
+        ip = _flat(top_ids, "top_ids", torch.int32, (rows, top), at)
     _need(grad_logp is None or targets is not None, "grad_logp needs the targets")
     _need(grad_entropy is None or entropy is not None, "grad_entropy needs the entropy")
-    _need(top == 0 or top_ids is not None, "grad_top needs top_ids")
+    row = (rows,)
     check(lib.rt_token_logprobs_backward(
-        out.data_ptr(), out_pitch, logits.data_ptr(), pitch,
-        None if targets is None else _flat(targets, "targets", torch.int32, (rows,), dev), f(stats, "stats", rows, 2),
-        f(entropy, "entropy", rows), rows, vocab, f(grad_logp, "grad_logp", rows), f(grad_entropy, "grad_entropy", rows), top,
-        None if top == 0 else _flat(top_ids, "top_ids", torch.int32, (rows, top), dev), f(grad_top, "grad_top", rows, top), dt, _stream()))
+        out.data_ptr(), out_pitch, logits.data_ptr(), pitch, None if targets is None else _flat(targets, "targets", torch.int32, row, at),
+        f(stats, "stats", (rows, 2)), f(entropy, "entropy", row), rows, vocab, f(grad_logp, "grad_logp", row),
+        f(grad_entropy, "grad_entropy", row), top, ip, f(grad_top, "grad_top", (rows, top)), dt, st))
     return out
 
 
