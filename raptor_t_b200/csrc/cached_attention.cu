@@ -27,7 +27,8 @@
 namespace rt {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kWarps = 4;
+constexpr int kMaxSplits = 16;
 constexpr int kFewRows = 64;  // rows of a sequence and key head up to which this kernel is taken
 
 using Args = CachedAttentionArgs;
@@ -76,7 +77,7 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int t, uint32_t
 }
 
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) {
   using C = kv::Codes<INT8>;
   __shared__ float s_o[kWarps][16][64];
   __shared__ float2 s_ml[kWarps][16];
@@ -267,8 +268,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
     *reinterpret_cast<uint2*>(seq_rows.output(a, head, row0 + r) + d) = w;
   };
   const int valid = min(16, rows - row0);
-  const int r = threadIdx.x >> 4, d = (threadIdx.x & 15) * 4;
-  {
+  for (int i = threadIdx.x; i < valid * 16; i += kWarps * 32) {
+    const int r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
@@ -286,24 +287,24 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
       v.w = fmaf(x.w, f, v.w);
     }
     if (a.splits == 1) {
-      if (r < valid) store(r, d, v, L);
-      return;
+      store(r, d, v, L);
+    } else {
+      *reinterpret_cast<float4*>(&s_sum[r][d]) = v;
+      if (d == 0) s_sum_ml[r] = make_float2(M, L);
     }
-    *reinterpret_cast<float4*>(&s_sum[r][d]) = v;
-    if (d == 0) s_sum_ml[r] = make_float2(M, L);
   }
+  if (a.splits == 1) return;
   // ---- the CTAs of the cluster: each finishes its share of the tile's quads of dimensions
   ptx::cluster_arrive();
   ptx::cluster_wait();
-  const int share = kWarps * 32 / a.splits;
-  const int item = rank * share + static_cast<int>(threadIdx.x);
-  if (static_cast<int>(threadIdx.x) < share && (item >> 4) < valid) {
-    const int rr = item >> 4, dd = (item & 15) * 4;
-    const uint32_t ml_at = ptx::smem_u32(&s_sum_ml[rr]), o_at = ptx::smem_u32(&s_sum[rr][dd]);
+  for (int i = rank + a.splits * static_cast<int>(threadIdx.x); i < valid * 16; i += a.splits * kWarps * 32) {
+    const int r = i >> 4, d = (i & 15) * 4;
+    const uint32_t ml_at = ptx::smem_u32(&s_sum_ml[r]), o_at = ptx::smem_u32(&s_sum[r][d]);
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
     for (int w = 0; w < a.splits; ++w) M = fmaxf(M, kv::ld_cluster_f2(kv::peer_address(ml_at, w)).x);
     const float ref = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
     for (int w = 0; w < a.splits; ++w) {
       const float2 ml = kv::ld_cluster_f2(kv::peer_address(ml_at, w));
       const float4 x = kv::ld_cluster_f4(kv::peer_address(o_at, w));
@@ -314,7 +315,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2) few_rows_kernel(const Args a) 
       v.z = fmaf(x.z, f, v.z);
       v.w = fmaf(x.w, f, v.w);
     }
-    store(rr, dd, v, L);
+    store(r, d, v, L);
   }
   ptx::cluster_arrive();  // no CTA leaves while another one reads its shared memory
   ptx::cluster_wait();
@@ -324,6 +325,7 @@ rt_status launch_few_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) 
   auto kern = bf16 ? (int8 ? few_rows_kernel<true, true> : few_rows_kernel<true, false>)
                    : (int8 ? few_rows_kernel<false, true> : few_rows_kernel<false, false>);
   const int64_t grid = static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits;
+  if (a.splits > 8) RT_TRY(ensure_large_clusters(reinterpret_cast<const void*>(kern)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kWarps * 32);
@@ -389,10 +391,15 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "cached_attention: cannot allocate the device error word");
   const int64_t widest = static_cast<int64_t>(table_stride) * 64;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
-  // as many CTAs per tile as fill the chip, with work for every warp
-  const int64_t full = many ? 148 : 2 * 148, least = many ? 512 : 64 * kWarps;
   a.splits = 1;
-  while (a.splits < 8 && heads_of_all * a.tiles * a.splits < full && keys > least * a.splits) a.splits *= 2;
+  if (many) {
+    // tiles of up to 256 rows see very different numbers of keys under the causal rule: four CTAs per SM over the call balance them
+    while (a.splits < 8 && heads_of_all * a.tiles * a.splits < 4 * 148 && keys > 512 * a.splits) a.splits *= 2;
+  } else {
+    // 16 blocks a CTA, four a warp; fewer, down to one a warp, until the chip is full
+    while (a.splits < kMaxSplits && (keys > 1024 * a.splits || (heads_of_all * a.tiles * a.splits < 4 * 148 && keys > 256 * a.splits)))
+      a.splits *= 2;
+  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == RT_BF16, int8 = cache->format == RT_KV_INT8;
   return many ? launch_cached_attention_many_rows(a, bf16, int8, st) : launch_few_rows(a, bf16, int8, st);

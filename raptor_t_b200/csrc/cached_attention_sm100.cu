@@ -8,8 +8,9 @@
 //   warps 0-3, 4-7   softmax of stream 0, 1: thread r owns row r (TMEM lane r), as in attention_sm100.cu: score row from TMEM, running
 //                    maximum and sum in fp32, 16-bit probabilities back to TMEM, output rescaled only when the maximum has grown by
 //                    more than 2^8.
-//   warps 8-11       bring the codes: 16-byte loads, exact conversion to halves, stores into the 128-byte-swizzled operand tiles
-//                    (keys K-major, values MN-major).  The tile that 256 rows share is converted once.
+//   warps 8-11       bring the codes: bulk copies of whole blocks (4 KB) a few steps ahead into a ring, from there exact conversion to
+//                    halves and stores into the 128-byte-swizzled operand tiles (keys K-major, values MN-major).  The tile that 256
+//                    rows share is converted once.
 //   warps 12-15      issue the MMAs: scores and outputs of stream 0, scores and outputs of stream 1.
 // A block's key scale multiplies its scores.  Its value scale goes into the probabilities, relative to the largest one of the keys that the CTA
 // visits: p' = p * scale / largest * 2^7 (2^7: halves keep all their bits down to p = 2^-21 of the row's maximum; p' <= 2^15).
@@ -34,7 +35,9 @@ using namespace softmax;
 using Args = CachedAttentionArgs;
 
 constexpr int kThreads = 512;
-constexpr int kStages = 4;               // of keys, and of values
+constexpr int kStages = 3;               // of keys, and of values
+constexpr int kRaw = 4;                  // steps of codes on their way
+constexpr int kBlock = 4096;             // codes of a block
 constexpr int kRing = 16;                // scales of a step, read up to two steps after its keys' slot is free
 constexpr int kHalfTile = 64 * 128;      // 64 rows of 64 halves
 constexpr int kTile = 2 * kHalfTile;
@@ -47,8 +50,10 @@ constexpr int kRegsSoftmax = 200, kRegsBring = 72, kRegsIssue = 40;
 
 struct Smem {
   uint8_t q[2][kTile];
-  uint8_t k[kStages][kTile];  // afterwards: partial results, [2][128 rows][64] fp32
+  uint8_t k[kStages][kTile];
   uint8_t v[kStages][kTile];
+  uint8_t raw[kRaw][4 * kBlock];  // keys of block 0, 1, values of block 0, 1; afterwards: partial results, [2][128 rows][64] fp32
+  uint64_t raw_full[kRaw], raw_empty[kRaw];
   uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2];
   float4 scales[kRing];  // {key scale of block 0, 1, value scale of block 0, 1}
@@ -57,7 +62,7 @@ struct Smem {
   uint32_t tmem_slot;
   int abort_flag;
 };
-static_assert(kStages * kTile >= 2 * 128 * 64 * 4, "partial results fit the key slots");
+static_assert(kRaw * 4 * kBlock >= 2 * 128 * 64 * 4, "partial results fit the ring of codes");
 static_assert(sizeof(Smem) <= 227 * 1024, "one CTA per SM");
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
@@ -67,6 +72,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
 }
 
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+// Contiguous copy global -> shared (16-byte aligned), completion on an mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
 
 // 16 bytes of codes (16 dimensions of row `row`, chunk `c` of four) as 32 bytes of halves into a swizzled tile.
 template <bool INT8>
@@ -129,6 +141,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       mbar_init(&sm.p_full[x][1], 4);
       mbar_init(&sm.pv_done[x], 1);
     }
+    for (int s = 0; s < kRaw; ++s) {
+      mbar_init(&sm.raw_full[s], 1);
+      mbar_init(&sm.raw_empty[s], 4);
+    }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sm.k_full[s], 4);
       mbar_init(&sm.k_empty[s], 2);  // both streams, whether they use the step or not
@@ -147,6 +163,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   tc_fence_after_sync();
   const uint32_t tmem = sm.tmem_slot;
   AbortCtx ab{&sm.abort_flag, a.err};
+  // bounded, and the same answer for the whole warp
+  auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, site)) != 0;
+  };
   const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
   const int64_t slots = static_cast<int64_t>(a.cache.heads);
 
@@ -160,12 +180,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       constexpr uint32_t idesc128 = make_idesc_f16(128, 128, 0, false), idesc64 = make_idesc_f16(128, 64, 0, false);
       const uint64_t dq = make_smem_desc_sw128(smem_u32(sm.q[x]));
       const uint32_t d = tmem + kColS + x * 128;
-      if (steps_of(x) > 0 && mbar_wait(&sm.q_full[x], 0, ab, 310)) {
+      if (steps_of(x) > 0 && wait(&sm.q_full[x], 0, 310)) {
         for (int j = 0; j < n_steps; ++j) {
           const int s = j % kStages;
           const bool mine = uses(x, j);
-          if (mine && c > 0 && !mbar_wait(&sm.s_free[x], (c - 1) & 1, ab, 311)) break;
-          if (!mbar_wait(&sm.k_full[s], (j / kStages) & 1, ab, 312)) break;
+          if (mine && c > 0 && !wait(&sm.s_free[x], (c - 1) & 1, 311)) break;
+          if (!wait(&sm.k_full[s], (j / kStages) & 1, 312)) break;
           if (mine) {
             tc_fence_after_sync();
             const uint64_t dk = make_smem_desc_sw128(smem_u32(sm.k[s]));
@@ -184,7 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         }
       } else if (steps_of(x) == 0) {
         for (int j = 0; j < n_steps; ++j) {
-          if (!mbar_wait(&sm.k_full[j % kStages], (j / kStages) & 1, ab, 313)) break;
+          if (!wait(&sm.k_full[j % kStages], (j / kStages) & 1, 313)) break;
           if (leader) mbar_arrive(&sm.k_empty[j % kStages]);
           __syncwarp();
         }
@@ -194,16 +214,16 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       const uint32_t d = tmem + kColO + x * 64, p = tmem + kColP + x * 64;
       for (int j = 0; j < n_steps; ++j) {
         const int s = j % kStages;
-        if (!mbar_wait(&sm.v_full[s], (j / kStages) & 1, ab, 314)) break;
+        if (!wait(&sm.v_full[s], (j / kStages) & 1, 314)) break;
         if (uses(x, j)) {
           const uint64_t dv = make_smem_desc_sw128(smem_u32(sm.v[s]));
-          if (!mbar_wait(&sm.p_full[x][0], c & 1, ab, 315)) break;
+          if (!wait(&sm.p_full[x][0], c & 1, 315)) break;
           tc_fence_after_sync();
           if (leader) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, dv + (k * 2048 >> 4), idesc, c > 0 || k ? 1u : 0u);
           }
-          if (!mbar_wait(&sm.p_full[x][1], c & 1, ab, 316)) break;
+          if (!wait(&sm.p_full[x][1], c & 1, 316)) break;
           tc_fence_after_sync();
           if (leader) {
             if (2 * (j0 + j) + 1 < n_blocks) {
@@ -240,53 +260,73 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       }
       return page;
     };
-    uint4 wk[4], wv[4];
+    // thread 0 requests step j: pages and scales were read a step earlier
+    int pa = 0, pb = 0;
     float4 sc = make_float4(0, 0, 0, 0);
-    int pa = page_of(2 * j0), pb = page_of(2 * j0 + 1);
-    // chunks p and p + 128 of either block; a step's second block may be missing, then the first is taken twice
-    auto load = [&](const uint8_t* base, uint4* w) {
-      const uint4* x = reinterpret_cast<const uint4*>(base + (pa * slots + head) * 4096) + p;
-      const uint4* y = reinterpret_cast<const uint4*>(base + (pb * slots + head) * 4096) + p;
-      w[0] = __ldg(x);
-      w[1] = __ldg(x + 128);
-      w[2] = __ldg(y);
-      w[3] = __ldg(y + 128);
+    auto look = [&](int j) {
+      pa = page_of(2 * (j0 + j));
+      pb = page_of(2 * (j0 + j) + 1);
     };
-    auto store = [&](uint8_t* dst, const uint4* w) {
-      put_codes<INT8>(dst, p >> 2, p & 3, w[0]);
-      put_codes<INT8>(dst, (p >> 2) + 32, p & 3, w[1]);
-      put_codes<INT8>(dst + kHalfTile, p >> 2, p & 3, w[2]);
-      put_codes<INT8>(dst + kHalfTile, (p >> 2) + 32, p & 3, w[3]);
+    auto request = [&](int j) {
+      const int s = j % kRaw;
+      const bool pair = 2 * (j0 + j) + 1 < n_blocks;
+      const int64_t oa = (pa * slots + head) * kBlock, ob = (pb * slots + head) * kBlock;
+      mbar_arrive_expect_tx(&sm.raw_full[s], pair ? 4 * kBlock : 2 * kBlock);
+      bulk_load(sm.raw[s], a.cache.k + oa, kBlock, &sm.raw_full[s]);
+      if (pair) bulk_load(sm.raw[s] + kBlock, a.cache.k + ob, kBlock, &sm.raw_full[s]);
+      bulk_load(sm.raw[s] + 2 * kBlock, a.cache.v + oa, kBlock, &sm.raw_full[s]);
+      if (pair) bulk_load(sm.raw[s] + 3 * kBlock, a.cache.v + ob, kBlock, &sm.raw_full[s]);
+      sc = make_float4(a.cache.k_scale[pa * slots + head], a.cache.k_scale[pb * slots + head], a.cache.v_scale[pa * slots + head],
+                       a.cache.v_scale[pb * slots + head]);
+      sm.scales[j % kRing] = sc;
     };
-    if (n_steps > 0) {
-      load(a.cache.k, wk);
-      load(a.cache.v, wv);
+    // two of a block's 256 chunks of 16 codes a thread, of both blocks; a second block that a step does not have is what was there before
+    auto convert = [&](uint8_t* dst, const uint8_t* src) {
+      const uint4* w = reinterpret_cast<const uint4*>(src) + p;
+      const uint4 w0 = w[0], w1 = w[128], w2 = w[256], w3 = w[384];
+      put_codes<INT8>(dst, p >> 2, p & 3, w0);
+      put_codes<INT8>(dst, (p >> 2) + 32, p & 3, w1);
+      put_codes<INT8>(dst + kHalfTile, p >> 2, p & 3, w2);
+      put_codes<INT8>(dst + kHalfTile, (p >> 2) + 32, p & 3, w3);
+    };
+    int asked = 0;
+    if (p == 0) {
+      for (; asked < min(kRaw, n_steps); ++asked) {
+        look(asked);
+        request(asked);
+      }
+      if (asked < n_steps) look(asked);
     }
     for (int j = 0; j < n_steps; ++j) {
-      const int s = j % kStages;
-      if (p == 0) {
-        sc.x = a.cache.k_scale[pa * slots + head];
-        sc.y = a.cache.k_scale[pb * slots + head];
-        sc.z = a.cache.v_scale[pa * slots + head];
-        sc.w = a.cache.v_scale[pb * slots + head];
-      }
-      if (j + 1 < n_steps) {  // pages of the next step, on their way during the wait
-        pa = page_of(2 * (j0 + j) + 2);
-        pb = page_of(2 * (j0 + j) + 3);
-      }
-      if (!mbar_wait(&sm.k_empty[s], ((j / kStages) & 1) ^ 1, ab, 317)) break;
-      if (p == 0) sm.scales[j % kRing] = sc;
-      store(sm.k[s], wk);
+      const int s = j % kStages, rs = j % kRaw;
+      if (!wait(&sm.raw_full[rs], (j / kRaw) & 1, 322)) break;
+      if (!wait(&sm.k_empty[s], ((j / kStages) & 1) ^ 1, 317)) break;
+      convert(sm.k[s], sm.raw[rs]);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.k_full[s]);
-      if (j + 1 < n_steps) load(a.cache.k, wk);
-      if (!mbar_wait(&sm.v_empty[s], ((j / kStages) & 1) ^ 1, ab, 318)) break;
-      store(sm.v[s], wv);
+      if (!wait(&sm.v_empty[s], ((j / kStages) & 1) ^ 1, 318)) break;
+      convert(sm.v[s], sm.raw[rs] + 2 * kBlock);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.v_full[s]);
-      if (j + 1 < n_steps) load(a.cache.v, wv);
+      if (lane == 0) {
+        mbar_arrive(&sm.v_full[s]);
+        mbar_arrive(&sm.raw_empty[rs]);
+      }
+      if (j + kRaw < n_steps && warp == 8) {  // into the slot that this step has just left
+        if (!wait(&sm.raw_empty[rs], (j / kRaw) & 1, 323)) break;
+        if (p == 0) {
+          request(asked++);
+          if (asked < n_steps) look(asked);
+        }
+        __syncwarp();
+      }
+    }
+    if (p == 0 && *ab.cta_flag) {  // gave up: copies in flight land before the CTA ends
+      const long long t0 = clock64();
+      for (int j = max(0, asked - kRaw); j < asked; ++j)
+        while (!mbar_try_wait(&sm.raw_full[j % kRaw], (j / kRaw) & 1) && clock64() - t0 < kWaitCycles) {
+        }
     }
     __syncwarp();
     if (a.splits > 1) {
@@ -367,7 +407,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       const int key0 = (j0 + j) * 128;
       const bool pair = 2 * (j0 + j) + 1 < n_blocks;
       const bool act0 = live && key0 < wmax, act1 = live && pair && key0 + 64 < wmax;
-      if (!mbar_wait(&sm.s_full[x], c & 1, ab, 319)) { ok = false; break; }
+      if (!wait(&sm.s_full[x], c & 1, 319)) { ok = false; break; }
       tc_fence_after_sync();
       const float4 sc = sm.scales[j % kRing];
       uint32_t s[128];
@@ -407,7 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       l *= alpha;
       if (act0) l = fmaf(exp64<false>(s, p, c0, ref - e0), ex2(-e0), l);
       if (c > 0) {
-        if (!mbar_wait(&sm.pv_done[x], (c - 1) & 1, ab, 320)) { ok = false; break; }
+        if (!wait(&sm.pv_done[x], (c - 1) & 1, 320)) { ok = false; break; }
         tc_fence_after_sync();
       }
       if (__any_sync(0xffffffffu, fix) && c > 0) {
@@ -453,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     }
     ok = __all_sync(0xffffffffu, ok);
     if (ok && steps > 0) {
-      ok = mbar_wait(&sm.pv_done[x], (steps - 1) & 1, ab, 321);
+      ok = wait(&sm.pv_done[x], (steps - 1) & 1, 321);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after_sync();
     }
@@ -486,8 +526,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(sr.output(a, head, row) + 8 * q) = make_uint4(0, 0, 0, 0);
       }
     } else {
-      softmax_barrier();  // both streams' MMAs have read the last operands: the key slots are free
-      float* part = reinterpret_cast<float*>(sm.k) + x * 128 * 64 + r * 64;
+      softmax_barrier();  // both streams have seen the last step: its codes have been converted, the ring is free
+      float* part = reinterpret_cast<float*>(sm.raw) + x * 128 * 64 + r * 64;
       sm.ml[x][r] = make_float2(any && lim > 0 ? m_ref : -INFINITY, any && m_ref != -INFINITY ? l : 0.f);
       const bool keep = any;
 #pragma unroll
@@ -518,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       for (int i = rank * 256 + tid; i < here * 4; i += a.splits * 256) {
         const int rr = i >> 2, quarter = i & 3;
         const int x0 = two ? rr >> 7 : 0, xs = two ? 1 : 2, pr = rr & 127;
-        const uint32_t ml_at = smem_u32(&sm.ml[x0][pr]), o_at = smem_u32(reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64);
+        const uint32_t ml_at = smem_u32(&sm.ml[x0][pr]), o_at = smem_u32(reinterpret_cast<float*>(sm.raw) + (x0 * 128 + pr) * 64);
         float M = -INFINITY, L = 0.f;
         for (int w = 0; w < a.splits; ++w)
           for (int y = 0; y < xs; ++y) M = max_nan(M, kv::ld_cluster_f2(kv::peer_address(ml_at + y * 1024, w)).x);

@@ -87,28 +87,68 @@ __device__ __forceinline__ float scale_for(float most) {
   return fmaxf(__uint_as_float((bits + low) & ~low), kv::kMinScale);
 }
 
-// four codes of x / scale
-template <bool INT8>
-__device__ __forceinline__ uint32_t codes4(const float* x, float scale) {
-  if constexpr (INT8) {
-    uint32_t r = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float q = x[i] / scale;
-      const int c = __float2int_rn(q == q ? fminf(fmaxf(q, -kv::kInt8Max), kv::kInt8Max) : 0.f);
-      r |= static_cast<uint32_t>(c & 0xff) << (8 * i);
-    }
-    return r;
-  } else {
-    const float inv = 1.0f / scale;  // exact: a power of two
-    float q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = x[i] == x[i] ? x[i] * inv : 0.f;
-    const uint32_t a = __nv_cvt_float2_to_fp8x2(make_float2(q[0], q[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t b = __nv_cvt_float2_to_fp8x2(make_float2(q[2], q[3]), __NV_SATFINITE, __NV_E4M3);
-    return a | (b << 16);
-  }
+__device__ __forceinline__ unsigned long long f2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
 }
+__device__ __forceinline__ float2 f2_split(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// Codes of x / scale.  int8: the quotient from the correctly rounded reciprocal y by Markstein's correction, q = x y,
+// q + (x - q s) y, which is the correctly rounded one (P. Markstein, IBM J. Res. Dev. 34, 1990); then rounded to a whole number by adding 1.5 * 2^23,
+// whose last byte is the code.  e4m3: the scale is a power of two, the product with its reciprocal exact.
+template <bool INT8>
+struct Coder {
+  unsigned long long inv, neg;
+  float most;
+  __device__ __forceinline__ explicit Coder(float scale) {
+    const float y = __frcp_rn(scale);
+    inv = f2(y, y);
+    neg = f2(-scale, -scale);
+    most = INT8 ? kv::kInt8Max * scale : 0.f;  // what infinities become
+  }
+  // x where it may be no number
+  __device__ __forceinline__ float number(float x) const {
+    if (x != x) return 0.f;
+    return INT8 ? fminf(fmaxf(x, -most), most) : x;
+  }
+  __device__ __forceinline__ uint32_t four(const float* x) const {
+    const unsigned long long a = f2(x[0], x[1]), b = f2(x[2], x[3]);
+    unsigned long long p = f2_mul(a, inv), q = f2_mul(b, inv);
+    if constexpr (INT8) {
+      p = f2_fma(f2_fma(p, neg, a), inv, p);
+      q = f2_fma(f2_fma(q, neg, b), inv, q);
+      const unsigned long long magic = f2(12582912.f, 12582912.f);
+      const float2 u = f2_split(f2_add(p, magic)), v = f2_split(f2_add(q, magic));
+      const uint32_t lo = kv::prmt(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040u);
+      return kv::prmt(lo, kv::prmt(__float_as_uint(v.x), __float_as_uint(v.y), 0x0040u), 0x5410u);
+    } else {
+      const float2 u = f2_split(p), v = f2_split(q);
+      const uint32_t lo = __nv_cvt_float2_to_fp8x2(u, __NV_SATFINITE, __NV_E4M3);
+      const uint32_t hi = __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
+      return lo | (hi << 16);
+    }
+  }
+};
 
 // values of four codes, times `scale`
 template <bool INT8>
@@ -123,57 +163,79 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
   x[3] = b.y * s;
 }
 
-// grid: (block of the sequence, head) pairs of every sequence; warp 0 takes the keys, warp 1 the values.
+// grid: (block of the sequence, head) pairs of every sequence; warps 0 and 1 take the keys, 2 and 3 the values, 32 tokens each.
+// Two warps for a tile keep 32 warps a SM in registers: 8 sequences of 1024 to 4096 tokens, 12 heads, f16 to int8 (95 MB) with one
+// warp a tile, quotients by division and maxima in fp32 took 67.7 us.
+constexpr int kWriteThreads = 128;
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kWriteThreads, 8)
 kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t token_stride, int64_t head_stride,
                 const int32_t* __restrict__ table, int table_stride, const int32_t* __restrict__ start,
                 const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
+  __shared__ uint32_t s_most[kWriteThreads / 32];
   RT_PDL_LAUNCH_DEPENDENTS();
   RT_PDL_WAIT();
   const int head = blockIdx.x % c.heads;
   const int nth = blockIdx.x / c.heads % spans;
   const int seq = blockIdx.x / c.heads / spans;
-  const int lane = threadIdx.x & 31;
-  const bool values = threadIdx.x >= 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool values = warp >= 2;
   const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheWrite);
   if (s.page < 0) return;
-  const uint16_t* x = values ? v : k;
   const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
   uint8_t* dst = (values ? c.v : c.k) + slot * 4096;
   float* scale_at = (values ? c.v_scale : c.k_scale) + slot;
-
-  // eight lanes a row, four rows an instruction
-  uint4 w[16];
-  const int sub = lane >> 3, col = (lane & 7) * 8;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t pos = s.base + 4 * i + sub;
-    w[i] = make_uint4(0, 0, 0, 0);
-    if (pos >= s.lo && pos < s.hi)
-      w[i] = __ldg(reinterpret_cast<const uint4*>(x + value_offset(s, s.row0 + pos, head, c.heads, token_stride, head_stride) + col));
-  }
   const bool older = s.lo > s.base;
   const float was = older ? *scale_at : 0.f;
-  float most = 0.f;
+
+  // eight lanes a row, four rows an instruction
+  const int row0 = (warp & 1) * 32 + (lane >> 3), col = (lane & 7) * 8;
+  const int lo = static_cast<int>(s.lo - s.base), hi = static_cast<int>(s.hi - s.base);
+  uint4 w[8];
+  {
+    const int64_t t = s.row0 + s.base + row0;
+    const uint16_t* x = (values ? v : k) + value_offset(s, t, head, c.heads, token_stride, head_stride) + col;
+    const int64_t step = 4 * (token_stride == 0 ? 64 : token_stride);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 f = kv::unpack16<BF16>(p[j]);
-      const float a = fabsf(f.x), b = fabsf(f.y);
-      if (a < INFINITY) most = fmaxf(most, a);
-      if (b < INFINITY) most = fmaxf(most, b);
+    for (int i = 0; i < 8; ++i) {
+      w[i] = make_uint4(0, 0, 0, 0);
+      if (row0 + 4 * i >= lo && row0 + 4 * i < hi) w[i] = __ldg(reinterpret_cast<const uint4*>(x + i * step));
     }
   }
+  // the largest magnitude: without their signs the bits order as the numbers do, infinity and NaN on top
+  constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
+  uint32_t top = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-  const float need = scale_for<INT8>(most);
-  const bool grow = older && !(need <= was);
-  const float scale = older && !grow ? was : need;
-  if (grow) {  // the earlier tokens' codes, four lanes a row
-    for (int r = lane >> 2; r < s.lo - s.base; r += 8) {
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = __vmaxu2(top, p[j] & 0x7fff7fffu);
+  }
+  top = max(top & 0xffffu, top >> 16);
+  top = __reduce_max_sync(0xffffffffu, top);
+  const bool strange = top >= kInf;  // of the whole warp
+  if (strange) {                     // the largest finite one then
+    top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a = p[j] & 0x7fffu, b = (p[j] >> 16) & 0x7fffu;
+        top = max(top, max(a < kInf ? a : 0u, b < kInf ? b : 0u));
+      }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+  }
+  if (lane == 0) s_most[warp] = top;
+  __syncthreads();  // also: both warps of the tile have read the old scale
+  top = max(top, s_most[warp ^ 1]);
+  const float need = scale_for<INT8>(kv::unpack16<BF16>(top).x);
+  const bool keep = older && need <= was;
+  const float scale = keep ? was : need;
+  const Coder<INT8> code(scale);
+  if (older && !keep) {  // the earlier tokens' codes, four lanes a row
+    for (int r = (warp & 1) * 8 + (lane >> 2); r < lo; r += 16) {
       uint4* at = reinterpret_cast<uint4*>(dst + r * 64 + (lane & 3) * 16);
       uint4 old = *at;
       uint32_t* p = reinterpret_cast<uint32_t*>(&old);
@@ -181,17 +243,16 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
       for (int j = 0; j < 4; ++j) {
         float f[4];
         values4<INT8>(p[j], was, f);
-        p[j] = codes4<INT8>(f, scale);
+        p[j] = code.four(f);
       }
       *at = old;
     }
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t pos = s.base + 4 * i + sub;
-    if (pos < s.lo || pos >= s.hi) continue;
+  for (int i = 0; i < 8; ++i) {
+    const int r = row0 + 4 * i;
+    if (r < lo || r >= hi) continue;
     const uint32_t* p = reinterpret_cast<const uint32_t*>(&w[i]);
-    uint2 out;
     float f[8];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -199,12 +260,13 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
       f[2 * j] = t.x;
       f[2 * j + 1] = t.y;
     }
-    out.x = codes4<INT8>(f, scale);
-    out.y = codes4<INT8>(f + 4, scale);
-    *reinterpret_cast<uint2*>(dst + (4 * i + sub) * 64 + col) = out;
+    if (strange) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = code.number(f[j]);
+    }
+    *reinterpret_cast<uint2*>(dst + r * 64 + col) = make_uint2(code.four(f), code.four(f + 4));
   }
-  __syncwarp();  // every lane has read the old scale
-  if (lane == 0 && !(older && !grow)) *scale_at = scale;
+  if ((warp & 1) == 0 && lane == 0 && !keep) *scale_at = scale;
 }
 
 // The same grid; out_k / out_v are token-major [tokens][heads * 64].
@@ -286,7 +348,7 @@ extern "C" rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k, 
   const bool int8 = cache->format == RT_KV_INT8;
   auto kern = dtype == RT_BF16 ? (int8 ? kv_write_kernel<true, true> : kv_write_kernel<true, false>)
                                : (int8 ? kv_write_kernel<false, true> : kv_write_kernel<false, false>);
-  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(64), 0, static_cast<cudaStream_t>(stream), c,
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
                               static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), token_stride, head_stride, table,
                               table_stride, start, first, tokens, max_tokens, static_cast<int>(spans_of(max_tokens)), err));
   count_launch();

@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "device_error.h"
@@ -27,7 +28,45 @@ constexpr int kThreads = 512;
 constexpr int kGroups = kThreads / 8;
 constexpr int kMaxTop = 32;
 constexpr int kListed = 1024;  // candidates that a CTA can list
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kSlack = 5.5f;  // the reference follows a share's maximum when e^z has grown by more than 2^8
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+__device__ __forceinline__ unsigned long long f2(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 f2_split(unsigned long long v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 template <int TYPE>
 struct Logits;  // vectors of 16 bytes
@@ -47,6 +86,26 @@ struct Logits<RT_F32> {
     return make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
   }
   static __device__ __forceinline__ T from(float f) { return f; }
+  // the largest number of some vectors (NaN left out), and -inf replaced by a number far below every reference
+  static constexpr float kFloor = -1e30f;
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4* v) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float x[4];
+      unpack(v[i], x);
+      m = fmaxf(m, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+    }
+    return m;
+  }
+  static __device__ __forceinline__ uint4 floored(const uint4& v) {
+    float x[4];
+    unpack(v, x);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = max_nan(x[j], kFloor);
+    return pack(x);
+  }
 };
 
 template <>
@@ -71,6 +130,24 @@ struct Logits<RT_F16> {
     return v;
   }
   static __device__ __forceinline__ T from(float f) { return __float2half_rn(f); }
+  static constexpr float kFloor = -65504.f;
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(v);
+    __half2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; ++i) m = __hmax2(m, h[i]);
+    const float a = __low2float(m), b = __high2float(m);
+    return fmaxf(fmaxf(a, b), -INFINITY);
+  }
+  static __device__ __forceinline__ uint4 floored(const uint4& v) {
+    uint4 r;
+    const __half2 low = __float2half2_rn(kFloor);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<__half2*>(&r)[i] = __hmax2_nan(reinterpret_cast<const __half2*>(&v)[i], low);
+    return r;
+  }
 };
 
 template <>
@@ -94,44 +171,52 @@ struct Logits<RT_BF16> {
     return v;
   }
   static __device__ __forceinline__ T from(float f) { return __float2bfloat16_rn(f); }
+  static constexpr float kFloor = -1e30f;
+  template <int N>
+  static __device__ __forceinline__ float largest(const uint4* v) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(v);
+    __nv_bfloat162 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * N; ++i) m = __hmax2(m, h[i]);
+    const float a = __low2float(m), b = __high2float(m);
+    return fmaxf(fmaxf(a, b), -INFINITY);
+  }
+  static __device__ __forceinline__ uint4 floored(const uint4& v) {
+    uint4 r;
+    const __nv_bfloat162 low = __float2bfloat162_rn(kFloor);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      reinterpret_cast<__nv_bfloat162*>(&r)[i] = __hmax2_nan(reinterpret_cast<const __nv_bfloat162*>(&v)[i], low);
+    return r;
+  }
 };
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
-// Running statistics of a share of a row.
+// Running statistics of a share of a row relative to a reference r near the share's maximum: with t = (z - r) log2 e,
+// s = sum 2^t and w = sum 2^t t.
 struct Stats {
-  float m = -INFINITY, s = 0.f, w = 0.f;  // maximum, sum e^(z - m), sum e^(z - m) (z - m)
-  // relative to another maximum (at least m)
+  float r = -INFINITY, s = 0.f, w = 0.f;
+  // relative to another reference (at least r)
   __device__ __forceinline__ void raise(float to) {
-    if (m == -INFINITY) {
+    if (r == -INFINITY) {
       w = 0.f;  // s is 0, or NaN and stays
     } else {
-      const float d = m - to, c = ex2(d * kLog2e);
-      w = c > 0.f ? (w + s * d) * c : s * c;  // the product of 0 and an infinite d is left out; a NaN of s stays
-      s *= c;
+      const float d = (r - to) * kLog2e, f = ex2(d);
+      w = f > 0.f ? (w + s * d) * f : s * f;  // the product of 0 and an infinite d is left out; a NaN of s stays
+      s *= f;
     }
-    m = to;
+    r = to;
   }
-  __device__ __forceinline__ void add(float z) {  // z <= m
-    const float x = max_nan(z - m, -1000.f);      // -inf: e^x is 0 and so is its product with x
-    const float e = ex2(x * kLog2e);
+  __device__ __forceinline__ void add(float z) {
+    const float t = max_nan((z - r) * kLog2e, -2000.f);  // -inf: 2^t is 0 and so is its product with t
+    const float e = ex2(t);
     s += e;
-    w = fmaf(e, x, w);
+    w = fmaf(e, t, w);
   }
   __device__ __forceinline__ void join(const Stats& o) {
     Stats b = o;
-    const float to = fmaxf(m, b.m);
-    if (to != m) raise(to);
-    if (to != b.m) b.raise(to);
+    const float to = fmaxf(r, b.r);
+    if (to != r) raise(to);
+    if (to != b.r) b.raise(to);
     s += b.s;
     w += b.w;
   }
@@ -212,6 +297,8 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
   __shared__ Stats s_warp[kThreads / 32];
   __shared__ Stats s_cta;                            // of the CTA, then of the row
   __shared__ float s_group[kGroups];
+  __shared__ float s_max;                            // of the CTA
+  __shared__ int s_flagged[kThreads], s_flags;       // threads whose share holds candidates
   __shared__ float s_bar;                            // what a candidate reaches
   __shared__ int s_count;
   __shared__ unsigned long long s_list[kListed];
@@ -224,20 +311,51 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
   const Share<TYPE> share(static_cast<const typename L::T*>(a.logits) + row * a.pitch, a.vocab, rank, a.ranks);
 
   Stats mine;
-  auto take = [&](const uint4& v) {
-    float x[L::kVec];
-    L::unpack(v, x);
-    float most = x[0];
+  float my_most = -INFINITY;
+  // N vectors: one look at their maximum, then five instructions a value in packed fp32
+  auto take = [&](auto count, const uint4* v) {
+    constexpr int N = decltype(count)::value;
+    const float most = L::template largest<N>(v);
+    my_most = fmaxf(my_most, most);
+    if (most == -INFINITY) {  // nothing but -inf or NaN
 #pragma unroll
-    for (int j = 1; j < L::kVec; ++j) most = fmaxf(most, x[j]);
-    if (most > mine.m) mine.raise(most);
-    if (mine.m == -INFINITY) {  // nothing but -inf (or NaN) so far
+      for (int u = 0; u < N; ++u) {
+        float x[L::kVec];
+        L::unpack(v[u], x);
 #pragma unroll
-      for (int j = 0; j < L::kVec; ++j) mine.s += x[j] == x[j] ? 0.f : x[j];
-    } else {
-#pragma unroll
-      for (int j = 0; j < L::kVec; ++j) mine.add(x[j]);
+        for (int j = 0; j < L::kVec; ++j) mine.s += x[j] == x[j] ? 0.f : x[j];
+      }
+      return;
     }
+    if (!(most <= mine.r + kSlack)) mine.raise(most);
+    if (!(mine.r > 0.5f * L::kFloor && mine.r < 1e30f)) {  // logits near the value that stands for -inf, or near overflow
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        float x[L::kVec];
+        L::unpack(v[u], x);
+#pragma unroll
+        for (int j = 0; j < L::kVec; ++j) mine.add(x[j]);
+      }
+      return;
+    }
+    const unsigned long long k = f2(kLog2e, kLog2e), r = f2(-mine.r, -mine.r);
+    unsigned long long s2 = 0ull, w2 = 0ull;
+#pragma unroll
+    for (int u = 0; u < N; ++u) {
+      float x[L::kVec];
+      L::unpack(L::floored(v[u]), x);
+#pragma unroll
+      for (int j = 0; j < L::kVec; j += 2) {
+        const unsigned long long t = f2_mul(f2_add(f2(x[j], x[j + 1]), r), k);
+        const float2 q = f2_split(t);
+        const unsigned long long e = f2(ex2(q.x), ex2(q.y));
+        s2 = f2_add(s2, e);
+        w2 = f2_fma(e, t, w2);
+      }
+    }
+    const float2 s = f2_split(s2), w = f2_split(w2);
+    mine.s += s.x + s.y;
+    mine.w += w.x + w.y;
   };
   {
     const uint4* p = share.vectors();
@@ -246,21 +364,23 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
       uint4 v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = __ldg(p + i + u * kThreads);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) take(v[u]);
+      take(std::integral_constant<int, 4>(), v);
     }
-    for (; i < share.hi; i += kThreads) take(__ldg(p + i));
+    for (; i < share.hi; i += kThreads) {
+      const uint4 v = __ldg(p + i);
+      take(std::integral_constant<int, 1>(), &v);
+    }
     if (tid < 2 * L::kVec) {
       const int at = share.outside(tid);
       if (at >= 0) {
         const float z = L::one(share.row + at);
-        if (z > mine.m) mine.raise(z);
-        if (mine.m == -INFINITY) mine.s += z == z ? 0.f : z;
+        my_most = fmaxf(my_most, z);
+        if (z > mine.r) mine.raise(z);
+        if (mine.r == -INFINITY) mine.s += z == z ? 0.f : z;
         else mine.add(z);
       }
     }
   }
-  const float my_most = mine.m;
   {
     float most = my_most;
 #pragma unroll
@@ -270,18 +390,32 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     Stats other;
-    other.m = __shfl_xor_sync(0xffffffffu, mine.m, o);
+    other.r = __shfl_xor_sync(0xffffffffu, mine.r, o);
     other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
     other.w = __shfl_xor_sync(0xffffffffu, mine.w, o);
     mine.join(other);
   }
   if (lane == 0) s_warp[warp] = mine;
-  if (tid == 0) s_count = 0;
+  if (tid == 0) s_count = s_flags = 0;
   __syncthreads();
-  if (tid == 0) {
-    Stats all = s_warp[0];
-    for (int w = 1; w < kThreads / 32; ++w) all.join(s_warp[w]);
-    s_cta = all;
+  if (warp == kThreads / 32 - 1) {
+    Stats all;
+    if (lane < kThreads / 32) all = s_warp[lane];
+#pragma unroll
+    for (int o = kThreads / 64; o > 0; o >>= 1) {
+      Stats other;
+      other.r = __shfl_xor_sync(0xffffffffu, all.r, o);
+      other.s = __shfl_xor_sync(0xffffffffu, all.s, o);
+      other.w = __shfl_xor_sync(0xffffffffu, all.w, o);
+      all.join(other);
+    }
+    float most = fmaxf(s_group[lane], s_group[lane + 32]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) {
+      s_cta = all;
+      s_max = most;
+    }
   }
   if (a.top > 0) {
     if (tid < kGroups) {  // the top-th largest of the groups' maxima: equal ones by place
@@ -292,13 +426,29 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
     }
     __syncthreads();
     const float bar = s_bar;
-    if (my_most >= bar)
-      share.each_of_mine([&](float z, int index) {
-        if (z >= bar) {
-          const int at = atomicAdd(&s_count, 1);
-          if (at < kListed) s_list[at] = key_of(z, index);
-        }
-      });
+    auto list = [&](float z, int index) {
+      if (z >= bar) {
+        const int at = atomicAdd(&s_count, 1);
+        if (at < kListed) s_list[at] = key_of(z, index);
+      }
+    };
+    if (my_most >= bar) s_flagged[atomicAdd(&s_flags, 1)] = tid;
+    if (tid < 2 * L::kVec) {
+      const int at = share.outside(tid);
+      if (at >= 0) list(L::one(share.row + at), at);
+    }
+    __syncthreads();
+    {  // the vectors of those threads, one a thread and turn
+      const int per = (share.hi - share.lo + kThreads - 1) / kThreads, n = s_flags * per;
+      for (int q = tid; q < n; q += kThreads) {
+        const int i = share.lo + s_flagged[q / per] + q % per * kThreads;
+        if (i >= share.hi) continue;
+        float x[L::kVec];
+        L::unpack(__ldg(share.vectors() + i), x);
+#pragma unroll
+        for (int j = 0; j < L::kVec; ++j) list(x[j], share.head + i * L::kVec + j);
+      }
+    }
     if (tid < kMaxTop) s_best[tid] = 0;
     __syncthreads();
     const int count = s_count;
@@ -352,24 +502,33 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
       }
       if (warp == kThreads / 32 - 1) {
         Stats x;
+        float most = -INFINITY;
         if (lane < a.ranks) {
           const uint32_t at = peer(&s_cta, lane);
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.m) : "r"(at) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.r) : "r"(at) : "memory");
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.s) : "r"(at + 4) : "memory");
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.w) : "r"(at + 8) : "memory");
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(most) : "r"(peer(&s_max, lane)) : "memory");
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) {
           Stats other;
-          other.m = __shfl_xor_sync(0xffffffffu, x.m, o);
+          other.r = __shfl_xor_sync(0xffffffffu, x.r, o);
           other.s = __shfl_xor_sync(0xffffffffu, x.s, o);
           other.w = __shfl_xor_sync(0xffffffffu, x.w, o);
           x.join(other);
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
         }
-        if (lane == 0) s_warp[0] = x;
+        if (lane == 0) {
+          s_warp[0] = x;
+          s_group[0] = most;
+        }
       }
       __syncthreads();
-      if (tid == 0) s_cta = s_warp[0];
+      if (tid == 0) {
+        s_cta = s_warp[0];
+        s_max = s_group[0];
+      }
       if (tid < kMaxTop) s_best[tid] = 0;
       __syncthreads();
       if (tid < n) {
@@ -385,11 +544,13 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
     if (rank != 0) return;
   }
   const Stats all = s_cta;
-  const bool nothing = all.m == -INFINITY && all.s == 0.f;  // a row of -inf
-  const float log_s = nothing ? 0.f : all.m == -INFINITY ? all.s : logf(all.s);
+  const float m = s_max;
+  const bool nothing = m == -INFINITY && all.s == 0.f;  // a row of -inf
+  const float log2_s = log2f(all.s);
+  const float log_s = nothing ? 0.f : m == -INFINITY ? all.s : fmaf(kLn2, log2_s, all.r - m);
   if (tid == 0) {
-    a.stats[row] = make_float2(all.m, log_s);
-    if (a.entropy) a.entropy[row] = nothing ? 0.f : log_s - all.w / all.s;
+    a.stats[row] = make_float2(m, log_s);
+    if (a.entropy) a.entropy[row] = nothing ? 0.f : kLn2 * (log2_s - all.w / all.s);
     if (a.logp) {
       const int t = a.targets[row];
       float r = 0.f;
@@ -397,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
         atomicCAS(a.err, 0, kSiteToken);
         r = NAN;
       } else if (t >= 0) {
-        r = nothing ? -INFINITY : (L::one(share.row + t) - all.m) - log_s;
+        r = nothing ? -INFINITY : (L::one(share.row + t) - m) - log_s;
       }
       a.logp[row] = r;
     }
@@ -407,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
     const bool none = key == 0;  // fewer logits than places that are numbers
     a.top_ids[static_cast<int64_t>(row) * a.top + tid] = none ? -1 : index_of(key);
     a.top_logp[static_cast<int64_t>(row) * a.top + tid] =
-        none ? NAN : nothing ? -INFINITY : (value_of(key) - all.m) - log_s;
+        none ? NAN : nothing ? -INFINITY : (value_of(key) - m) - log_s;
   }
 }
 
@@ -439,6 +600,15 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
   const int tid = threadIdx.x;
   const Share<TYPE> share(static_cast<const T*>(a.logits) + row * a.pitch, a.vocab, 0, 1);
   T* out = static_cast<T*>(a.out) + row * a.out_pitch;
+  // the logits are on their way while the row's terms are read
+  const uint4* src = share.vectors();
+  const int v0 = chunk * 256 * kGradVecs + tid;
+  uint4 v[kGradVecs];
+#pragma unroll
+  for (int u = 0; u < kGradVecs; ++u) {
+    v[u] = make_uint4(0, 0, 0, 0);
+    if (v0 + u * 256 < share.nv) v[u] = src[v0 + u * 256];
+  }
   const float2 st = a.stats[row];
   const int target = a.g_logp ? a.targets[row] : -1;
   const bool given = target >= 0 && target < a.vocab;
@@ -479,13 +649,7 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
     }
   }
   __syncthreads();
-  const uint4* src = share.vectors();
   const bool aligned = (reinterpret_cast<uintptr_t>(out + share.head) & 15u) == 0;
-  const int v0 = chunk * 256 * kGradVecs + tid;
-  uint4 v[kGradVecs];
-#pragma unroll
-  for (int u = 0; u < kGradVecs; ++u)
-    if (v0 + u * 256 < share.nv) v[u] = src[v0 + u * 256];
 #pragma unroll
   for (int u = 0; u < kGradVecs; ++u) {
     const int i = v0 + u * 256;

@@ -106,6 +106,37 @@ def test_masked_vocabulary(ops, dtype, rows):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [5, 160])
+def test_rows_at_the_ends_of_the_type(ops, dtype, rows):
+    """Rows of nothing but the lowest value, with -inf among them, with the largest value, with both; and a large common offset."""
+    vocab, low, big = 6000, torch.finfo(dtype).min, torch.finfo(dtype).max
+    z, t = _rows(rows, vocab, dtype)
+    z = z.clone()
+    z[0] = low
+    z[1] = low
+    z[1, 1::2] = -float("inf")
+    t[1] = 2
+    z[2] = 0
+    z[2, 17] = big
+    t[2] = 17
+    z[3] = low
+    z[3, 100] = low / 2
+    z[3, 4000] = big
+    t[3] = 4000
+    z[4] = z[4] + (1000 if dtype != torch.float32 else 100000)
+    got = ops.token_logprobs(z, t, top_k=3)
+    lp = torch.log_softmax(z.double(), 1)
+    want = lp[torch.arange(rows, device="cuda"), t.long()]
+    assert ((got.logp.double() - want).abs() <= 2.0 ** -16 + 2.0 ** -22 * want.abs()).all()
+    h = -(lp.exp() * torch.where(lp.exp() == 0, 0.0, lp)).sum(1)
+    assert ((got.entropy.double() - h).abs() <= 2.0 ** -12).all()
+    assert torch.equal(got.top_ids.long(), torch.sort(z.float(), dim=1, descending=True, stable=True).indices[:, :3])
+    assert got.top_ids[1].tolist() == [0, 2, 4] and got.logp[2] == 0
+    d = ops.token_logprobs_backward(z, t, got.stats, got.entropy, grad_logp=torch.ones(rows, device="cuda"))
+    assert not d.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_rows_with_nan_and_infinity(ops, dtype):
     z, t = _rows(6, 5000, dtype)
     z = z.clone()
