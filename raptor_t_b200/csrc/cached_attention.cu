@@ -7,9 +7,10 @@
 //   out = sum_w O_w 2^(m_w - M) / sum_w l_w 2^(m_w - M),  M = max_w m_w.
 // Splitting the keys and not the rows is what fills the chip with a handful of rows, and one launch does it.
 //
-// The products run on mma.sync (m16n8k16, 16-bit operands, fp32 sums): the work is the bytes of the cache, and a 16-row tile costs
+// A warp's blocks come by bulk copies of 4 KB into a ring of its own, two blocks ahead, so that HBM sees 192 KB of requests per SM
+// and no register waits for them.  The products run on mma.sync (m16n8k16, 16-bit operands, fp32 sums): the work is the bytes of the cache, and a 16-row tile costs
 // about a fifth of the tensor pipe at the rate HBM delivers codes.  Codes become halves exactly (kv_cache.cuh), a block's
-// scale multiplies its scores and its output in fp32.  Codes go from global memory straight into the operand registers:
+// scale multiplies its scores and its output in fp32.  Codes go from shared memory straight into the operand registers:
 // the order of the 64 dimensions inside Q K^T and of the keys and dimensions inside P V is free, so it is chosen such that a thread's
 // operands are 16 consecutive bytes of a key and 8 of a value.
 // bf16 queries are turned into halves scaled by a power of two per row (largest entry in [2^14, 2^15)): exact but for
@@ -40,7 +41,7 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -76,13 +77,29 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int t, uint32_t
   }
 }
 
+constexpr int kStages = 2;
+struct Smem {
+  uint8_t ring[kWarps][kStages][2][4096];  // keys, values; afterwards the first 4 KB of a warp's ring are its output, fp32 [16][64]
+  float sum[16][64];                       // of the CTA
+  float2 sum_ml[16];
+  float2 ml[kWarps][16];
+  uint64_t full[kWarps][kStages];
+  int abort_flag;
+};
+static_assert(3 * (sizeof(Smem) + 1024) <= 228 * 1024, "three CTAs share an SM");
+
+// Contiguous copy global -> shared (16-byte aligned), completion on an mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ptx::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(ptx::smem_u32(bar))
+               : "memory");
+}
+
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) {
+__global__ void __launch_bounds__(kWarps * 32, 3) few_rows_kernel(const Args a) {
   using C = kv::Codes<INT8>;
-  __shared__ float s_o[kWarps][16][64];
-  __shared__ float2 s_ml[kWarps][16];
-  __shared__ float s_sum[16][64];
-  __shared__ float2 s_sum_ml[16];
+  extern __shared__ __align__(128) uint8_t smem_raw[];
+  Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   RT_PDL_LAUNCH_DEPENDENTS();
   RT_PDL_WAIT();
   const int rank = blockIdx.x % a.splits;
@@ -125,119 +142,175 @@ __global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) 
 
   const int n_blocks = (most + 63) / 64, step = a.splits * kWarps;
   const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
-  int b = rank * kWarps + warp;
-  int page = b < n_blocks ? table[b] : 0;
-  for (; b < n_blocks; b += step) {
-    const int at = page;
-    if (b + step < n_blocks) page = table[b + step];
-    if (at < 0 || at >= a.cache.blocks) {
-      if (lane == 0) kv::index_error(a.err, kSiteCachedAttention);
-      continue;
+  const int b0 = rank * kWarps + warp;
+  if (threadIdx.x == 0) {
+    for (int w = 0; w < kWarps; ++w)
+      for (int s = 0; s < kStages; ++s) ptx::mbar_init(&sm.full[w][s], 1);
+    sm.abort_flag = 0;
+    ptx::fence_barrier_init();
+  }
+  __syncthreads();
+  ptx::AbortCtx ab{&sm.abort_flag, a.err};
+  // A block on its way: its scales, negative where the table has no such block.
+  float ks[kStages], vs[kStages];
+  int page[kStages];  // of the blocks to be requested next
+  auto look = [&](int s, int b) { page[s] = b < n_blocks ? __ldg(table + b) : -1; };
+  auto request = [&](int s, int b) {
+    if (b >= n_blocks) return;
+    const bool bad = page[s] < 0 || page[s] >= a.cache.blocks;
+    if (bad && lane == 0) kv::index_error(a.err, kSiteCachedAttention);
+    const int64_t slot = static_cast<int64_t>(bad ? 0 : page[s]) * a.cache.heads + head;
+    if (lane == 0) {
+      ptx::mbar_arrive_expect_tx(&sm.full[warp][s], 8192);
+      bulk_load(sm.ring[warp][s][0], a.cache.k + slot * 4096, 4096, &sm.full[warp][s]);
+      bulk_load(sm.ring[warp][s][1], a.cache.v + slot * 4096, 4096, &sm.full[warp][s]);
     }
-    const int64_t slot = static_cast<int64_t>(at) * a.cache.heads + head;
-    const uint8_t* kp = a.cache.k + slot * 4096;
-    const uint8_t* vp = a.cache.v + slot * 4096;
-    uint4 kw[8];
+    ks[s] = bad ? -1.f : __ldg(a.cache.k_scale + slot);
+    vs[s] = __ldg(a.cache.v_scale + slot);
+  };
 #pragma unroll
-    for (int j = 0; j < 8; ++j) kw[j] = __ldg(reinterpret_cast<const uint4*>(kp + (8 * j + g) * 64 + 16 * t));
-    uint2 vw[16];  // keys 16 s + 2 t, + 1, + 8, + 9 of every step s of 16 keys, dimensions 8 g .. 8 g + 7
+  for (int s = 0; s < kStages; ++s) look(s, b0 + s * step);
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+  for (int s = 0; s < kStages; ++s) request(s, b0 + s * step);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        vw[4 * s + i] = __ldg(reinterpret_cast<const uint2*>(vp + (16 * s + 2 * t + (i & 1) + 4 * (i & 2)) * 64 + 8 * g));
-    const float ks = a.cache.k_scale[slot], vs = a.cache.v_scale[slot] * C::kUnit;
+  for (int s = 0; s < kStages; ++s) look(s, b0 + (kStages + s) * step);
 
-    // scores; step s of the product covers dimensions 16 t + 4 s .. + 3 of every thread's share
-    float sc[8][4];
+  // Thread (g, t) takes key row g ^ (t's lowest bit) of every eight, so that the rows that four threads read at once are even and odd:
+  // rows are 64 bytes, banks repeat after 128.
+  const int kg = g ^ ((g >> 1) & 1), odd = t & 1;
+  bool ok = true;
+  uint32_t phase = 0;
+  for (int bb = b0; bb < n_blocks && ok; bb += kStages * step, phase ^= 1) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-      const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
+    for (int st = 0; st < kStages; ++st) {
+      const int b = bb + st * step;
+      if (b >= n_blocks) break;
+      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&sm.full[warp][st], phase, ab, 330))) {
+        // gives up: copies in flight land before the ring is used again
+        const long long t0 = clock64();
+        for (int s = 0; lane == 0 && s < kStages; ++s) {
+          const bool next = s < st;  // the slot has been requested again
+          if (bb + (next ? kStages + s : s) * step >= n_blocks) continue;
+          while (!ptx::mbar_try_wait(&sm.full[warp][s], next ? phase ^ 1 : phase) && clock64() - t0 < ptx::kWaitCycles) {
+          }
+        }
+        __syncwarp();
+        ok = false;
+        break;
+      }
+      const uint8_t* kp = sm.ring[warp][st][0];
+      const uint8_t* vp = sm.ring[warp][st][1];
+      const float k_scale = ks[st], v_scale = vs[st] * C::kUnit;
+      uint4 kw[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kw[j] = *reinterpret_cast<const uint4*>(kp + (8 * j + kg) * 64 + 16 * t);
+
+      // scores; step s of the product covers dimensions 16 t + 4 s .. + 3 of every thread's share
+      float sc[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
+        const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const uint32_t p = C::prepare(w[s]);
+          mma16816(sc[j], q[s], C::template pair<0>(p), C::template pair<2>(p));
+        }
+      }
+      const float u0 = unit0 * k_scale, u1 = unit1 * k_scale;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sc[j][0] *= u0;
+        sc[j][1] *= u0;
+        sc[j][2] *= u1;
+        sc[j][3] *= u1;
+      }
+      if (b * 64 + 64 > least || k_scale < 0.f) {  // keys that some row of the tile does not see
+        const int l0 = k_scale < 0.f ? 0 : lim0, l1 = k_scale < 0.f ? 0 : lim1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = b * 64 + 8 * j + 2 * t;
+          if (key + odd >= l0) sc[j][0] = -INFINITY;
+          if (key + 1 - odd >= l0) sc[j][1] = -INFINITY;
+          if (key + odd >= l1) sc[j][2] = -INFINITY;
+          if (key + 1 - odd >= l1) sc[j][3] = -INFINITY;
+        }
+      }
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        x0 = fmaxf(x0, fmaxf(sc[j][0], sc[j][1]));
+        x1 = fmaxf(x1, fmaxf(sc[j][2], sc[j][3]));
+      }
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
+      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
+      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
+      x0 = fmaxf(x0, m0);
+      x1 = fmaxf(x1, m1);
+      // a row that has seen nothing yet: every exponential below is 2^(-inf)
+      const float r0 = x0 == -INFINITY ? 0.f : x0, r1 = x1 == -INFINITY ? 0.f : x1;
+      const float c0 = ex2(m0 - r0), c1 = ex2(m1 - r1);
+      m0 = x0;
+      m1 = x1;
+      l0 *= c0;
+      l1 *= c1;
+      uint32_t p[4][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float e0 = ex2(sc[j][0] - r0), e1 = ex2(sc[j][1] - r0);
+        l0 += e0 + e1;
+        p[j >> 1][(j & 1) * 2] = kv::pack16<false>(e0, e1);
+        p[j >> 1][(j & 1) * 2 + 1] = 0u;
+      }
+      if (two) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float e0 = ex2(sc[j][2] - r1), e1 = ex2(sc[j][3] - r1);
+          l1 += e0 + e1;
+          p[j >> 1][(j & 1) * 2 + 1] = kv::pack16<false>(e0, e1);
+        }
+      }
+      uint2 vw[16];  // keys 16 s + 2 t, + 1, + 8, + 9 of every step s of 16 keys, dimensions 8 g .. 8 g + 7
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          vw[4 * s + i] = *reinterpret_cast<const uint2*>(vp + (16 * s + 2 * t + ((i & 1) ^ odd) + 4 * (i & 2)) * 64 + 8 * g);
+      __syncwarp();  // the slot has been read
+      request(st, b + kStages * step);
+      look(st, b + 2 * kStages * step);
+      // output: column c of 8-column tile j is dimension 8 c + j
+      float acc[8][4];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const uint32_t p = C::prepare(w[s]);
-        mma16816(sc[j], q[s], C::template pair<0>(p), C::template pair<2>(p));
-      }
-    }
-    const float u0 = unit0 * ks, u1 = unit1 * ks;
+        const uint2* w = vw + 4 * s;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      sc[j][0] *= u0;
-      sc[j][1] *= u0;
-      sc[j][2] *= u1;
-      sc[j][3] *= u1;
-    }
-    if (b * 64 + 64 > least) {  // keys that some row of the tile does not see
+        for (int half = 0; half < 2; ++half) {  // dimensions 8 g + 4 half .. + 3
+          const uint32_t ka = half ? w[0].y : w[0].x, kb = half ? w[1].y : w[1].x;
+          const uint32_t kc = half ? w[2].y : w[2].x, kd = half ? w[3].y : w[3].x;
+          const uint32_t ab0 = C::prepare(kv::prmt(ka, kb, 0x5140u)), ab1 = C::prepare(kv::prmt(ka, kb, 0x7362u));
+          const uint32_t cd0 = C::prepare(kv::prmt(kc, kd, 0x5140u)), cd1 = C::prepare(kv::prmt(kc, kd, 0x7362u));
+          mma16816(acc[4 * half], p[s], C::template pair<0>(ab0), C::template pair<0>(cd0));
+          mma16816(acc[4 * half + 1], p[s], C::template pair<2>(ab0), C::template pair<2>(cd0));
+          mma16816(acc[4 * half + 2], p[s], C::template pair<0>(ab1), C::template pair<0>(cd1));
+          mma16816(acc[4 * half + 3], p[s], C::template pair<2>(ab1), C::template pair<2>(cd1));
+        }
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = b * 64 + 8 * j + 2 * t;
-        if (key >= lim0) sc[j][0] = -INFINITY;
-        if (key + 1 >= lim0) sc[j][1] = -INFINITY;
-        if (key >= lim1) sc[j][2] = -INFINITY;
-        if (key + 1 >= lim1) sc[j][3] = -INFINITY;
+        o[j][0] = fmaf(acc[j][0], v_scale, o[j][0] * c0);
+        o[j][1] = fmaf(acc[j][1], v_scale, o[j][1] * c0);
       }
-    }
-    float x0 = -INFINITY, x1 = -INFINITY;
+      if (two) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      x0 = fmaxf(x0, fmaxf(sc[j][0], sc[j][1]));
-      x1 = fmaxf(x1, fmaxf(sc[j][2], sc[j][3]));
-    }
-    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-    x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-    x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-    x0 = fmaxf(x0, m0);
-    x1 = fmaxf(x1, m1);
-    // a row that has seen nothing yet: every exponential below is 2^(-inf)
-    const float r0 = x0 == -INFINITY ? 0.f : x0, r1 = x1 == -INFINITY ? 0.f : x1;
-    const float c0 = ex2(m0 - r0), c1 = ex2(m1 - r1);
-    m0 = x0;
-    m1 = x1;
-    l0 *= c0;
-    l1 *= c1;
-    uint32_t p[4][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float e0 = ex2(sc[j][0] - r0), e1 = ex2(sc[j][1] - r0);
-      l0 += e0 + e1;
-      p[j >> 1][(j & 1) * 2] = kv::pack16<false>(e0, e1);
-      p[j >> 1][(j & 1) * 2 + 1] = 0u;
-    }
-    if (two) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e0 = ex2(sc[j][2] - r1), e1 = ex2(sc[j][3] - r1);
-        l1 += e0 + e1;
-        p[j >> 1][(j & 1) * 2 + 1] = kv::pack16<false>(e0, e1);
+        for (int j = 0; j < 8; ++j) {
+          o[j][2] = fmaf(acc[j][2], v_scale, o[j][2] * c1);
+          o[j][3] = fmaf(acc[j][3], v_scale, o[j][3] * c1);
+        }
       }
-    }
-    // output: column c of 8-column tile j is dimension 8 c + j
-    float acc[8][4];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      const uint2* w = vw + 4 * s;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {  // dimensions 8 g + 4 half .. + 3
-        const uint32_t ka = half ? w[0].y : w[0].x, kb = half ? w[1].y : w[1].x;
-        const uint32_t kc = half ? w[2].y : w[2].x, kd = half ? w[3].y : w[3].x;
-        const uint32_t ab0 = C::prepare(kv::prmt(ka, kb, 0x5140u)), ab1 = C::prepare(kv::prmt(ka, kb, 0x7362u));
-        const uint32_t cd0 = C::prepare(kv::prmt(kc, kd, 0x5140u)), cd1 = C::prepare(kv::prmt(kc, kd, 0x7362u));
-        mma16816(acc[4 * half], p[s], C::template pair<0>(ab0), C::template pair<0>(cd0));
-        mma16816(acc[4 * half + 1], p[s], C::template pair<2>(ab0), C::template pair<2>(cd0));
-        mma16816(acc[4 * half + 2], p[s], C::template pair<0>(ab1), C::template pair<0>(cd1));
-        mma16816(acc[4 * half + 3], p[s], C::template pair<2>(ab1), C::template pair<2>(cd1));
-      }
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      o[j][0] = fmaf(acc[j][0], vs, o[j][0] * c0);
-      o[j][1] = fmaf(acc[j][1], vs, o[j][1] * c0);
-      o[j][2] = fmaf(acc[j][2], vs, o[j][2] * c1);
-      o[j][3] = fmaf(acc[j][3], vs, o[j][3] * c1);
     }
   }
   l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
@@ -246,18 +319,19 @@ __global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) 
   l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
   // ---- the warps of the CTA.  Thread (g, t) holds dimensions 16 t .. 16 t + 15 of rows g and g + 8.
+  auto out_of = [&](int w) { return reinterpret_cast<float(*)[64]>(sm.ring[w][0][0]); };
   if (t == 0) {
-    s_ml[warp][g] = make_float2(m0, l0);
-    s_ml[warp][g + 8] = make_float2(m1, l1);
+    sm.ml[warp][g] = make_float2(m0, l0);
+    sm.ml[warp][g + 8] = make_float2(m1, l1);
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int j = 0; j < 8; j += 4) {
-      *reinterpret_cast<float4*>(&s_o[warp][g][16 * t + 8 * c + j]) =
-          make_float4(o[j][c], o[j + 1][c], o[j + 2][c], o[j + 3][c]);
-      *reinterpret_cast<float4*>(&s_o[warp][g + 8][16 * t + 8 * c + j]) =
-          make_float4(o[j][2 + c], o[j + 1][2 + c], o[j + 2][2 + c], o[j + 3][2 + c]);
+      *reinterpret_cast<float4*>(&out_of(warp)[g][16 * t + 8 * c + j]) = make_float4(o[j][c], o[j + 1][c], o[j + 2][c], o[j + 3][c]);
+      if (two)
+        *reinterpret_cast<float4*>(&out_of(warp)[g + 8][16 * t + 8 * c + j]) =
+            make_float4(o[j][2 + c], o[j + 1][2 + c], o[j + 2][2 + c], o[j + 3][2 + c]);
     }
   __syncthreads();
   auto store = [&](int r, int d, float4 v, float l) {
@@ -273,13 +347,13 @@ __global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) 
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, s_ml[w][r].x);
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.ml[w][r].x);
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float2 ml = s_ml[w][r];
+      const float2 ml = sm.ml[w][r];
       const float f = ex2(ml.x - ref);
-      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][r][d]);
+      const float4 x = *reinterpret_cast<const float4*>(&out_of(w)[r][d]);
       L = fmaf(ml.y, f, L);
       v.x = fmaf(x.x, f, v.x);
       v.y = fmaf(x.y, f, v.y);
@@ -289,8 +363,8 @@ __global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) 
     if (a.splits == 1) {
       store(r, d, v, L);
     } else {
-      *reinterpret_cast<float4*>(&s_sum[r][d]) = v;
-      if (d == 0) s_sum_ml[r] = make_float2(M, L);
+      *reinterpret_cast<float4*>(&sm.sum[r][d]) = v;
+      if (d == 0) sm.sum_ml[r] = make_float2(M, L);
     }
   }
   if (a.splits == 1) return;
@@ -299,7 +373,7 @@ __global__ void __launch_bounds__(kWarps * 32, 4) few_rows_kernel(const Args a) 
   ptx::cluster_wait();
   for (int i = rank + a.splits * static_cast<int>(threadIdx.x); i < valid * 16; i += a.splits * kWarps * 32) {
     const int r = i >> 4, d = (i & 15) * 4;
-    const uint32_t ml_at = ptx::smem_u32(&s_sum_ml[r]), o_at = ptx::smem_u32(&s_sum[r][d]);
+    const uint32_t ml_at = ptx::smem_u32(&sm.sum_ml[r]), o_at = ptx::smem_u32(&sm.sum[r][d]);
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
     for (int w = 0; w < a.splits; ++w) M = fmaxf(M, kv::ld_cluster_f2(kv::peer_address(ml_at, w)).x);
@@ -325,10 +399,12 @@ rt_status launch_few_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) 
   auto kern = bf16 ? (int8 ? few_rows_kernel<true, true> : few_rows_kernel<true, false>)
                    : (int8 ? few_rows_kernel<false, true> : few_rows_kernel<false, false>);
   const int64_t grid = static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits;
+  RT_TRY(ensure_kernel_smem(reinterpret_cast<const void*>(kern), sizeof(Smem), true));
   if (a.splits > 8) RT_TRY(ensure_large_clusters(reinterpret_cast<const void*>(kern)));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
   cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -251,18 +251,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     // ---------------------------------------------------------------- codes to operand tiles
     reg_dealloc<kRegsBring>();
     const int p = tid - 256;
-    auto page_of = [&](int b) {
-      if (b >= n_blocks) return 0;  // no such block: whatever is there is not used
-      int page = table[b];
-      if (page < 0 || page >= a.cache.blocks) {
-        if (p == 0) kv::index_error(a.err, kSiteCachedAttention);
-        page = 0;
-      }
-      return page;
+    auto page_of = [&](int b) { return b < n_blocks ? __ldg(table + b) : 0; };
+    // the first code of a block, and its key scale: negative where the table has no such block, whose keys nobody sees then
+    auto place_of = [&](int page, float* scale) {
+      const bool bad = page < 0 || page >= a.cache.blocks;
+      if (bad) kv::index_error(a.err, kSiteCachedAttention);
+      const int64_t slot = (bad ? 0 : page) * slots + head;
+      *scale = bad ? -1.f : a.cache.k_scale[slot];
+      return slot;
     };
     // thread 0 requests step j: pages and scales were read a step earlier
     int pa = 0, pb = 0;
-    float4 sc = make_float4(0, 0, 0, 0);
     auto look = [&](int j) {
       pa = page_of(2 * (j0 + j));
       pb = page_of(2 * (j0 + j) + 1);
@@ -270,15 +269,15 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     auto request = [&](int j) {
       const int s = j % kRaw;
       const bool pair = 2 * (j0 + j) + 1 < n_blocks;
-      const int64_t oa = (pa * slots + head) * kBlock, ob = (pb * slots + head) * kBlock;
+      float ka, kb;
+      const int64_t sa = place_of(pa, &ka), sb = place_of(pb, &kb);
+      const int64_t oa = sa * kBlock, ob = sb * kBlock;
       mbar_arrive_expect_tx(&sm.raw_full[s], pair ? 4 * kBlock : 2 * kBlock);
       bulk_load(sm.raw[s], a.cache.k + oa, kBlock, &sm.raw_full[s]);
       if (pair) bulk_load(sm.raw[s] + kBlock, a.cache.k + ob, kBlock, &sm.raw_full[s]);
       bulk_load(sm.raw[s] + 2 * kBlock, a.cache.v + oa, kBlock, &sm.raw_full[s]);
       if (pair) bulk_load(sm.raw[s] + 3 * kBlock, a.cache.v + ob, kBlock, &sm.raw_full[s]);
-      sc = make_float4(a.cache.k_scale[pa * slots + head], a.cache.k_scale[pb * slots + head], a.cache.v_scale[pa * slots + head],
-                       a.cache.v_scale[pb * slots + head]);
-      sm.scales[j % kRing] = sc;
+      sm.scales[j % kRing] = make_float4(ka, kb, a.cache.v_scale[sa], a.cache.v_scale[sb]);
     };
     // two of a block's 256 chunks of 16 codes a thread, of both blocks; a second block that a step does not have is what was there before
     auto convert = [&](uint8_t* dst, const uint8_t* src) {
@@ -406,10 +405,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       const int j = two ? c : 2 * c + x;
       const int key0 = (j0 + j) * 128;
       const bool pair = 2 * (j0 + j) + 1 < n_blocks;
-      const bool act0 = live && key0 < wmax, act1 = live && pair && key0 + 64 < wmax;
       if (!wait(&sm.s_full[x], c & 1, 319)) { ok = false; break; }
       tc_fence_after_sync();
       const float4 sc = sm.scales[j % kRing];
+      const bool act0 = live && key0 < wmax && sc.x >= 0.f, act1 = live && pair && key0 + 64 < wmax && sc.y >= 0.f;
       uint32_t s[128];
       tmem_ld32(ts, s);
       tmem_ld32(ts + 32, s + 32);

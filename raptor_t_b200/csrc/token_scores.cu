@@ -4,7 +4,7 @@
 // Both read every logit once and are bound by that (the gradient writes as much).
 //
 // Forward: a CTA, or a cluster of CTAs where there are few rows, takes a row.  A thread keeps the running maximum, sum and weighted sum of its
-// share.  The k best come without a second pass over the row: the k-th largest of the maxima of groups of eight threads is a
+// share.  The k best come without a second pass over the row: the k-th largest of the maxima of groups of four threads is a
 // value that at least k logits reach; only threads whose own maximum reaches it look at their share again (a few dozen
 // logits, still in L2) and list what does.  A list that does not fit (thousands of equal logits) is replaced by k
 // searches over the row.
@@ -24,8 +24,9 @@
 namespace rt {
 namespace {
 
-constexpr int kThreads = 512;
-constexpr int kGroups = kThreads / 8;
+constexpr int kThreads = 256;
+constexpr int kGroup = 4;  // threads of a group
+constexpr int kGroups = kThreads / kGroup;
 constexpr int kMaxTop = 32;
 constexpr int kListed = 1024;  // candidates that a CTA can list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -212,15 +213,25 @@ struct Stats {
     s += e;
     w = fmaf(e, t, w);
   }
-  __device__ __forceinline__ void join(const Stats& o) {
-    Stats b = o;
-    const float to = fmaxf(r, b.r);
-    if (to != r) raise(to);
-    if (to != b.r) b.raise(to);
-    s += b.s;
-    w += b.w;
-  }
 };
+
+__device__ __forceinline__ float warp_max(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+// The statistics of a warp's shares, in every lane: one change of reference each, then plain sums.
+__device__ __forceinline__ void join_warp(Stats& x) {
+  const float to = warp_max(x.r);
+  if (to != x.r) x.raise(to);
+  x.s = warp_sum(x.s);
+  x.w = warp_sum(x.w);
+}
 
 // A share of `nv` vectors and the elements before and behind them.  Vectors [lo, hi) belong to this CTA.
 template <int TYPE>
@@ -292,11 +303,12 @@ struct ScoreArgs {
 };
 
 template <int TYPE>
-__global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const ScoreArgs a) {
   using L = Logits<TYPE>;
   __shared__ Stats s_warp[kThreads / 32];
   __shared__ Stats s_cta;                            // of the CTA, then of the row
-  __shared__ float s_group[kGroups];
+  __shared__ __align__(16) float s_group[kGroups];
+  __shared__ float s_warp_max[kThreads / 32];
   __shared__ float s_max;                            // of the CTA
   __shared__ int s_flagged[kThreads], s_flags;       // threads whose share holds candidates
   __shared__ float s_bar;                            // what a candidate reaches
@@ -381,37 +393,29 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
       }
     }
   }
-  {
+  if (a.top > 0) {
     float most = my_most;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-    if ((lane & 7) == 0) s_group[tid >> 3] = most;
+    for (int o = kGroup / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane % kGroup == 0) s_group[tid / kGroup] = most;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats other;
-    other.r = __shfl_xor_sync(0xffffffffu, mine.r, o);
-    other.s = __shfl_xor_sync(0xffffffffu, mine.s, o);
-    other.w = __shfl_xor_sync(0xffffffffu, mine.w, o);
-    mine.join(other);
+  join_warp(mine);
+  const float warp_most = warp_max(my_most);
+  if (lane == 0) {
+    s_warp[warp] = mine;
+    s_warp_max[warp] = warp_most;
   }
-  if (lane == 0) s_warp[warp] = mine;
   if (tid == 0) s_count = s_flags = 0;
   __syncthreads();
   if (warp == kThreads / 32 - 1) {
     Stats all;
-    if (lane < kThreads / 32) all = s_warp[lane];
-#pragma unroll
-    for (int o = kThreads / 64; o > 0; o >>= 1) {
-      Stats other;
-      other.r = __shfl_xor_sync(0xffffffffu, all.r, o);
-      other.s = __shfl_xor_sync(0xffffffffu, all.s, o);
-      other.w = __shfl_xor_sync(0xffffffffu, all.w, o);
-      all.join(other);
+    float most = -INFINITY;
+    if (lane < kThreads / 32) {
+      all = s_warp[lane];
+      most = s_warp_max[lane];
     }
-    float most = fmaxf(s_group[lane], s_group[lane + 32]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+    join_warp(all);
+    most = warp_max(most);
     if (lane == 0) {
       s_cta = all;
       s_max = most;
@@ -421,7 +425,14 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
     if (tid < kGroups) {  // the top-th largest of the groups' maxima: equal ones by place
       const float x = s_group[tid];
       int before = 0;
-      for (int i = 0; i < kGroups; ++i) before += s_group[i] > x || (s_group[i] == x && i < tid);
+#pragma unroll
+      for (int i = 0; i < kGroups; i += 4) {
+        const float4 y = *reinterpret_cast<const float4*>(&s_group[i]);
+        before += y.x > x || (y.x == x && i < tid);
+        before += y.y > x || (y.y == x && i + 1 < tid);
+        before += y.z > x || (y.z == x && i + 2 < tid);
+        before += y.w > x || (y.w == x && i + 3 < tid);
+      }
       if (before == a.top - 1) s_bar = x;
     }
     __syncthreads();
@@ -510,24 +521,17 @@ __global__ void __launch_bounds__(kThreads, 2) token_logprobs_kernel(const Score
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.w) : "r"(at + 8) : "memory");
           asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(most) : "r"(peer(&s_max, lane)) : "memory");
         }
-#pragma unroll
-        for (int o = 4; o > 0; o >>= 1) {
-          Stats other;
-          other.r = __shfl_xor_sync(0xffffffffu, x.r, o);
-          other.s = __shfl_xor_sync(0xffffffffu, x.s, o);
-          other.w = __shfl_xor_sync(0xffffffffu, x.w, o);
-          x.join(other);
-          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-        }
+        join_warp(x);
+        most = warp_max(most);
         if (lane == 0) {
           s_warp[0] = x;
-          s_group[0] = most;
+          s_warp_max[0] = most;
         }
       }
       __syncthreads();
       if (tid == 0) {
         s_cta = s_warp[0];
-        s_max = s_group[0];
+        s_max = s_warp_max[0];
       }
       if (tid < kMaxTop) s_best[tid] = 0;
       __syncthreads();
@@ -614,8 +618,12 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
   const bool given = target >= 0 && target < a.vocab;
   if (target >= a.vocab && chunk == 0 && tid == 0) atomicCAS(a.err, 0, kSiteToken);
   const float g_t = given ? a.g_logp[row] : 0.f;
-  float pull = g_t;
-  for (int j = 0; j < a.top; ++j) pull += a.g_top[static_cast<int64_t>(row) * a.top + j];
+  // every warp reads the alternatives, one a lane
+  const int lane = tid & 31, warp = tid >> 5;
+  const int64_t alt = static_cast<int64_t>(row) * a.top + lane;
+  const float g_alt = lane < a.top ? a.g_top[alt] : 0.f;
+  const int id = lane < a.top ? a.top_ids[alt] : -1;
+  const float pull = g_t + (a.top > 0 ? warp_sum(g_alt) : 0.f);
   const float g_h = a.g_entropy ? a.g_entropy[row] : 0.f;
   const float h = a.g_entropy ? a.entropy[row] : 0.f;
   const bool nothing = st.x == -INFINITY;
@@ -630,22 +638,21 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
   float special = 0.f;
   const int first = share.head + chunk * 256 * kGradVecs * L::kVec;
   const int behind = min(share.head + share.nv * L::kVec, first + 256 * kGradVecs * L::kVec);
-  if (tid <= a.top) {
-    column = tid == 0 ? (given ? target : -1) : a.top_ids[static_cast<int64_t>(row) * a.top + tid - 1];
+  if (warp < 2) {  // warp 0: the alternatives, lane 0 of warp 1: the target
+    column = warp == 0 ? id : lane == 0 && given ? target : -1;
     if (column >= a.vocab) {
       if (chunk == 0) atomicCAS(a.err, 0, kSiteToken);
       column = -1;
     }
     const bool in_vectors = column >= share.head && column < share.head + share.nv * L::kVec;
-    const bool here = in_vectors ? column >= first && column < behind : chunk == 0;
-    if (!here) column = -1;
-    if (column >= 0) {
-      special = grad(L::one(share.row + column));
-      if (!nothing) {
-        if (given && column == target) special += g_t;
-        for (int j = 0; j < a.top; ++j)
-          if (a.top_ids[static_cast<int64_t>(row) * a.top + j] == column) special += a.g_top[static_cast<int64_t>(row) * a.top + j];
+    if (!(in_vectors ? column >= first && column < behind : chunk == 0)) column = -1;
+    if (__any_sync(0xffffffffu, column >= 0)) {
+      float own = given && column == target ? g_t : 0.f;
+      for (int j = 0; j < a.top; ++j) {
+        const float g = __shfl_sync(0xffffffffu, g_alt, j);
+        if (__shfl_sync(0xffffffffu, id, j) == column) own += g;
       }
+      if (column >= 0) special = grad(L::one(share.row + column)) + (nothing ? 0.f : own);
     }
   }
   __syncthreads();
@@ -703,7 +710,7 @@ extern "C" rt_status rt_token_logprobs(const void* logits, int64_t pitch, const 
   ScoreArgs a{logits, pitch, targets, rows, vocab, top, 1, logp, entropy, reinterpret_cast<float2*>(stats), top_ids, top_logp,
               device_error_word()};
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "token_logprobs: cannot allocate the device error word");
-  // few rows: several CTAs for each, as long as every thread has two vectors
+  // few rows: several CTAs for each, as long as every thread has four vectors
   const int vectors = vocab / (16 / type_size(dtype));
   while (a.ranks < 8 && static_cast<int64_t>(rows) * a.ranks < 148 && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
   RT_REQUIRE(static_cast<int64_t>(rows) * a.ranks < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
