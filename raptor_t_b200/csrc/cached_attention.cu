@@ -1,21 +1,20 @@
 // Attention of few query rows over the 8-bit key/value cache (layout: kv_cache.cuh): single tokens of running answers, short
 // questions.
 //
-// The rows of one sequence that share a key head (token x query heads of the group) form tiles of 16.  A warp takes every n-th
-// 64-token block of the tile's sequence and keeps the tile's running maximum, sum and output for its blocks alone; the
-// warps of a CTA, and the CTAs of a cluster through distributed shared memory, are joined at the end:
+// The rows of one sequence that share a key head (token x query heads of the group) form tiles of 8 or 16.  A warp works on one
+// 64-token block of one tile at a time and keeps a running maximum, sum and output for the blocks it has seen; partial results are joined by
 //   out = sum_w O_w 2^(m_w - M) / sum_w l_w 2^(m_w - M),  M = max_w m_w.
-// Splitting the keys and not the rows is what fills the chip with a handful of rows, and one launch does it.
+// Splitting the keys and not the rows is what fills the chip with a handful of rows: the warps of a CTA take every n-th block of a tile, and
+// the CTAs of a cluster share it, too; results meet in (distributed) shared memory.  One launch.
 //
-// A warp's blocks come by bulk copies of 4 KB into a ring of its own, two blocks ahead, so that HBM sees 192 KB of requests per SM
-// and no register waits for them.  The products run on mma.sync (m16n8k16, 16-bit operands, fp32 sums): the work is the bytes of the cache, and a 16-row tile costs
-// about a fifth of the tensor pipe at the rate HBM delivers codes.  Codes become halves exactly (kv_cache.cuh), a block's
-// scale multiplies its scores and its output in fp32.  Codes go from shared memory straight into the operand registers:
-// the order of the 64 dimensions inside Q K^T and of the keys and dimensions inside P V is free, so it is chosen such that a thread's
-// operands are 16 consecutive bytes of a key and 8 of a value.
+// A warp's blocks come by bulk copies of 4 KB into a ring of its own, 12 KB ahead, so that HBM sees 192 KB of requests per SM
+// and no register waits for them.  The products run on mma.sync (m16n8k16, 16-bit operands, fp32 sums): the work is the bytes of the cache.
+// Codes become halves exactly, a block's scale multiplies its scores and its output in fp32.  Codes go from shared memory
+// straight into the operand registers: the order of the 64 dimensions inside Q K^T and of the keys and dimensions inside P V is free, so it is chosen
+// such that a thread's operands are 16 consecutive bytes of a key and 8 of a value.
 // bf16 queries are turned into halves scaled by a power of two per row (largest entry in [2^14, 2^15)): exact but for
 // entries 2^-28 below the row's largest.  Probabilities are rounded to halves (2^-11 relative) for the second product; their
-// sum is taken in fp32 before.
+// sum is that of the rounded ones, in fp32.
 #include "cached_attention.h"
 
 #include <algorithm>
@@ -28,11 +27,15 @@
 namespace rt {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kMaxSplits = 16;
-constexpr int kFewRows = 64;  // rows of a sequence and key head up to which this kernel is taken
-
 using Args = CachedAttentionArgs;
+
+constexpr int kWarps = 4;       // of a CTA
+constexpr int ctas_per_sm(int nt) { return nt == 1 ? 4 : 3; }  // as the registers allow
+constexpr int kSlots = 3;       // pieces of 4 KB of a warp on their way
+constexpr int kMaxSplits = 8;   // CTAs of a cluster
+constexpr int kFewRows = 64;    // rows of a sequence and key head up to which these kernels are taken
+constexpr int kBlock = 4096;    // bytes of a block's keys, or values
+constexpr float kSlack = 8.f, kShift = 7.f;  // probabilities are at most 2^15
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -41,52 +44,10 @@ __device__ __forceinline__ float ex2(float x) {
 }
 
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-
-// 16 dimensions [16 t, 16 t + 16) of one query row as eight half2, and the power of two that they were multiplied with.
-template <bool BF16>
-__device__ __forceinline__ float load_query(const uint16_t* row, int t, uint32_t* h) {
-  uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-  if (row) {
-    w[0] = __ldg(reinterpret_cast<const uint4*>(row + 16 * t));
-    w[1] = __ldg(reinterpret_cast<const uint4*>(row + 16 * t + 8));
-  }
-  const uint32_t* p = reinterpret_cast<const uint32_t*>(w);
-  if constexpr (!BF16) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) h[i] = p[i];
-    return 1.f;
-  } else {
-    uint32_t most = 0;  // bits of the largest magnitude: integers order as the magnitudes do
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, max((p[i] << 16) & 0x7fffffffu, p[i] & 0x7fff0000u));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int up = kv::query_shift(most);
-    const float f = kv::pow2(up);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float2 x = kv::unpack16<true>(p[i]);
-      h[i] = kv::pack16<false>(x.x * f, x.y * f);
-    }
-    return kv::pow2(-up);
-  }
-}
-
-constexpr int kStages = 2;
-struct Smem {
-  uint8_t ring[kWarps][kStages][2][4096];  // keys, values; afterwards the first 4 KB of a warp's ring are its output, fp32 [16][64]
-  float sum[16][64];                       // of the CTA
-  float2 sum_ml[16];
-  float2 ml[kWarps][16];
-  uint64_t full[kWarps][kStages];
-  int abort_flag;
-};
-static_assert(3 * (sizeof(Smem) + 1024) <= 228 * 1024, "three CTAs share an SM");
 
 // Contiguous copy global -> shared (16-byte aligned), completion on an mbarrier.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -95,9 +56,410 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(kWarps * 32, 3) few_rows_kernel(const Args a) {
-  using C = kv::Codes<INT8>;
+// Codes as operands of the products, two codes a register, to be multiplied with kUnit after kBias has been taken off.
+//   int8: the code with its sign bit flipped is an unsigned byte u = code + 128; the half with the bits u is the subnormal number
+//     u 2^-24, so a byte move does it.  128 of each code is taken off the sums: 128 sum q is the same for every key, and 128 sum p
+//     comes from the product that sums the probabilities anyway.  fp32 sums keep 2^-17 of a code that way.
+//   e4m3: the hardware's conversion.  A code that is NaN, which the writer never stores, stays NaN; the caller keeps those of places that hold no
+//     token out of P V.
+template <bool INT8>
+struct Operand;
+template <>
+struct Operand<true> {
+  static constexpr float kUnit = 16777216.f, kBias = 128.f;
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
+  template <int LO>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) { return kv::prmt(w, 0u, LO == 0 ? 0x4140u : 0x4342u); }
+};
+template <>
+struct Operand<false> {
+  static constexpr float kUnit = 1.f, kBias = 0.f;
+  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
+  template <int LO>
+  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
+    uint32_t r;
+    if constexpr (LO == 0) asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}" : "=r"(r) : "r"(w));
+    else asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, hi;}" : "=r"(r) : "r"(w));
+    return r;
+  }
+};
+
+// 8 x 8 halves: thread (g, t) gives row g, columns 2 t and 2 t + 1, and gets them of the transposed matrix.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+
+// 16 dimensions [16 t, 16 t + 16) of one query row, times `sign`, as eight half2, and the power of two that they were multiplied with.
+template <bool BF16>
+__device__ __forceinline__ float load_query(const uint16_t* row, int t, float sign, uint32_t* h) {
+  uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
+  if (row) {
+    w[0] = __ldg(reinterpret_cast<const uint4*>(row + 16 * t));
+    w[1] = __ldg(reinterpret_cast<const uint4*>(row + 16 * t + 8));
+  }
+  const uint32_t* p = reinterpret_cast<const uint32_t*>(w);
+  int up = 0;
+  if constexpr (BF16) {
+    uint32_t most = 0;  // bits of the largest magnitude: integers order as the magnitudes do
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, max((p[i] << 16) & 0x7fffffffu, p[i] & 0x7fff0000u));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    up = kv::query_shift(most);
+  }
+  const float f = kv::pow2(up) * sign;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 x = kv::unpack16<BF16>(p[i]);
+    h[i] = kv::pack16<false>(x.x * f, x.y * f);
+  }
+  return kv::pow2(-up);
+}
+
+// One warp's state for a tile of 8 NT rows.  The products are taken transposed, S^T = K Q^T and O^T = V^T P^T: keys and dimensions fill the
+// 16-row side of m16n8k16, query rows the 8-column side, so a conversion serves all rows and nothing is computed for rows that a tile does
+// not have.  Thread (g, t) = (lane / 4, lane % 4) has columns (rows of the tile) 8 n + 2 t, + 1.
+template <bool BF16, bool INT8, int NT>
+struct RowTile {
+  using C = Operand<INT8>;
+  static constexpr int kRows = 8 * NT;
+  int g, t;
+  int ctx, least;         // keys of the sequence, and of those what the tile's first row sees
+  int lim[NT][2];         // and what this thread's rows see
+  uint32_t q[NT][4][2];
+  float unit[NT][2], bias[NT][2];  // a score in base 2 is (product * unit - bias) * key scale
+  float m[NT][2], l[NT][2];        // reference of the exponentials, sum of the rounded probabilities
+  float o[NT][4][4];               // dimensions 8 g + 2 j (first two), 8 g + 2 j + 1 (last two)
+
+  __device__ __forceinline__ void begin(const Args& a, const CachedRows& sr, int head, int row0) {
+    ctx = sr.ctx;
+    least = sr.limit(a, row0);
+    // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
+    const float sign = a.scale_log2 > 0.f ? 1.f : a.scale_log2 < 0.f ? -1.f : 0.f;
+    const float size = (sign == 0.f ? 1.f : fabsf(a.scale_log2));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int mine = row0 + 8 * n + g;
+      uint32_t h[8];
+      const float back = load_query<BF16>(mine < sr.rows ? sr.query(a, head, mine) : nullptr, t, sign, h) * size;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        q[n][s][0] = h[2 * s];
+        q[n][s][1] = h[2 * s + 1];
+        if constexpr (INT8) mma16816(sum, kOnes, h[2 * s], h[2 * s + 1]);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = row0 + 8 * n + 2 * t + e;
+        lim[n][e] = row < sr.rows ? sr.limit(a, row) : 0;
+        const float u = __shfl_sync(0xffffffffu, back, (2 * t + e) * 4);  // of the thread that loaded the row
+        unit[n][e] = u * C::kUnit;
+        bias[n][e] = C::kBias * sum[e] * u;
+        m[n][e] = -INFINITY;
+        l[n][e] = 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[n][j][0] = o[n][j][1] = o[n][j][2] = o[n][j][3] = 0.f;
+    }
+  }
+
+  // Block b of the sequence; k_scale < 0: no such block, nobody sees its keys.  keys_read(): the keys' codes are in registers;
+  // values(): where the values' codes are, once they are there; values_read(): they are in registers.
+  // Key kk of every 16 is row kk with its lowest bit turned where bit 1 is set, so that the value rows that four threads read at once are
+  // even and odd: rows are 64 bytes, banks repeat after 128.
+  template <typename KeysRead, typename Values, typename ValuesRead>
+  __device__ __forceinline__ bool block(const uint8_t* kp, float k_scale, float v_scale, int b, KeysRead keys_read, Values values,
+                                        ValuesRead values_read) {
+    const int kg = g ^ ((g >> 1) & 1), odd = t & 1;
+    float sc[NT][4][4];  // of key tile i: keys g (first two), g + 8, of rows 2 t, 2 t + 1
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 lo = *reinterpret_cast<const uint4*>(kp + (16 * i + kg) * 64 + 16 * t);
+      const uint4 hi = *reinterpret_cast<const uint4*>(kp + (16 * i + 8 + kg) * 64 + 16 * t);
+      const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n][i][0] = sc[n][i][1] = sc[n][i][2] = sc[n][i][3] = 0.f;
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {  // dimensions 16 t + 4 s .. + 3 of every thread's share
+        const uint32_t x = C::prepare(wl[s]), y = C::prepare(wh[s]);
+        const uint32_t k[4] = {C::template pair<0>(x), C::template pair<0>(y), C::template pair<2>(x), C::template pair<2>(y)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) mma16816(sc[n][i], k, q[n][s][0], q[n][s][1]);
+      }
+    }
+    __syncwarp();
+    keys_read();
+    const bool edge = b * 64 + 64 > least || k_scale < 0.f;  // keys that some row of the tile does not see
+    if (edge) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int e0 = k_scale < 0.f ? 0 : lim[n][0], e1 = k_scale < 0.f ? 0 : lim[n][1];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = b * 64 + 16 * i + kg;
+          if (key >= e0) sc[n][i][0] = -INFINITY;
+          if (key >= e1) sc[n][i][1] = -INFINITY;
+          if (key + 8 >= e0) sc[n][i][2] = -INFINITY;
+          if (key + 8 >= e1) sc[n][i][3] = -INFINITY;
+        }
+      }
+    }
+    // The reference of a row follows its maximum when that has grown by more than 2^8.
+    float u[NT][2], c[NT][2];
+    bool grown = false;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        u[n][e] = fmaxf(unit[n][e] * k_scale, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
+        c[n][e] = -bias[n][e] * k_scale;
+        float x = fmaxf(fmaxf(sc[n][0][e], sc[n][0][e + 2]), fmaxf(sc[n][1][e], sc[n][1][e + 2]));
+        x = fmaxf(x, fmaxf(fmaxf(sc[n][2][e], sc[n][2][e + 2]), fmaxf(sc[n][3][e], sc[n][3][e + 2])));
+        grown |= fmaf(x, u[n][e], c[n][e]) > m[n][e] + kSlack;
+      }
+    float alpha[NT][2];
+    const bool change = __any_sync(0xffffffffu, grown);
+    if (change) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float x = fmaxf(fmaxf(sc[n][0][e], sc[n][0][e + 2]), fmaxf(sc[n][1][e], sc[n][1][e + 2]));
+          x = fmaxf(x, fmaxf(fmaxf(sc[n][2][e], sc[n][2][e + 2]), fmaxf(sc[n][3][e], sc[n][3][e + 2])));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+          x = fmaxf(m[n][e], fmaf(x, u[n][e], c[n][e]));
+          alpha[n][e] = x == -INFINITY ? 1.f : ex2(m[n][e] - x);
+          m[n][e] = x;
+          l[n][e] *= alpha[n][e];
+        }
+    }
+    // probabilities as halves, 2^7 times larger (halves keep all their bits down to 2^-21 of the reference), and turned into the operand P^T
+    uint32_t p[NT][4][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      // a row that has seen nothing yet: every exponential is 2^(-inf)
+      const float c0 = c[n][0] - (m[n][0] == -INFINITY ? 0.f : m[n][0]) + kShift, c1 = c[n][1] - (m[n][1] == -INFINITY ? 0.f : m[n][1]) + kShift;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e0 = ex2(fmaf(sc[n][i][0], u[n][0], c0)), e1 = ex2(fmaf(sc[n][i][1], u[n][1], c1));
+        const float e2 = ex2(fmaf(sc[n][i][2], u[n][0], c0)), e3 = ex2(fmaf(sc[n][i][3], u[n][1], c1));
+        p[n][i][0] = transpose8(kv::pack16<false>(e0, e1));
+        p[n][i][1] = transpose8(kv::pack16<false>(e2, e3));
+      }
+    }
+    // keys 2 t, + 1, + 8, + 9 of key tile i, dimensions 8 g .. 8 g + 7.  With 16 rows a tile they are read as they are needed: all at once
+    // would not fit the registers.
+    uint2 vw[NT == 1 ? 16 : 4];
+    const uint8_t* vp = values();
+    if (!vp) return false;
+    auto load = [&](int i, uint2* w) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int row = 16 * i + 2 * t + ((e & 1) ^ odd) + 4 * (e & 2);
+        w[e] = *reinterpret_cast<const uint2*>(vp + row * 64 + 8 * g);
+        if (!INT8 && b * 64 + row >= ctx) w[e] = make_uint2(0, 0);  // places that hold no token may hold the code NaN
+      }
+    };
+    if constexpr (NT == 1) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) load(i, vw + 4 * i);
+      __syncwarp();
+      values_read();
+    }
+    float acc[NT][4][4], sum[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[n][j][0] = acc[n][j][1] = acc[n][j][2] = acc[n][j][3] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) mma16816(sum[n], kOnes, p[n][i][0], p[n][i][1]);
+      if constexpr (NT > 1) load(i, vw);
+      const uint2* w = NT == 1 ? vw + 4 * i : vw;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // dimensions 8 g + 4 half .. + 3
+        const uint32_t ka = half ? w[0].y : w[0].x, kb = half ? w[1].y : w[1].x;
+        const uint32_t kc = half ? w[2].y : w[2].x, kd = half ? w[3].y : w[3].x;
+        const uint32_t xa = C::prepare(ka), xb = C::prepare(kb), xc = C::prepare(kc), xd = C::prepare(kd);
+        const uint32_t ab0 = kv::prmt(xa, xb, 0x5140u), ab1 = kv::prmt(xa, xb, 0x7362u);
+        const uint32_t cd0 = kv::prmt(xc, xd, 0x5140u), cd1 = kv::prmt(xc, xd, 0x7362u);
+        const uint32_t v0[4] = {C::template pair<0>(ab0), C::template pair<2>(ab0), C::template pair<0>(cd0), C::template pair<2>(cd0)};
+        const uint32_t v1[4] = {C::template pair<0>(ab1), C::template pair<2>(ab1), C::template pair<0>(cd1), C::template pair<2>(cd1)};
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mma16816(acc[n][2 * half], v0, p[n][i][0], p[n][i][1]);
+          mma16816(acc[n][2 * half + 1], v1, p[n][i][0], p[n][i][1]);
+        }
+      }
+    }
+    if constexpr (NT > 1) {
+      __syncwarp();
+      values_read();
+    }
+    const float vs = v_scale * C::kUnit;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const float off0 = -C::kBias * v_scale * sum[n][0], off1 = -C::kBias * v_scale * sum[n][1];
+      l[n][0] += sum[n][0];
+      l[n][1] += sum[n][1];
+      if (change) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[n][j][0] *= alpha[n][0];
+          o[n][j][1] *= alpha[n][1];
+          o[n][j][2] *= alpha[n][0];
+          o[n][j][3] *= alpha[n][1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        o[n][j][0] += fmaf(acc[n][j][0], vs, off0);
+        o[n][j][1] += fmaf(acc[n][j][1], vs, off1);
+        o[n][j][2] += fmaf(acc[n][j][2], vs, off0);
+        o[n][j][3] += fmaf(acc[n][j][3], vs, off1);
+      }
+    }
+    return true;
+  }
+
+  // un-normalised outputs and {m, l} of the tile's rows
+  __device__ __forceinline__ void put(float (*out)[64], float2* ml, int valid) const {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * n + 2 * t + e;
+        if (r >= valid) continue;
+        if (g == 0) ml[r] = make_float2(m[n][e], l[n][e]);
+        float4* at = reinterpret_cast<float4*>(&out[r][8 * g]);
+        at[0] = make_float4(o[n][0][e], o[n][0][e + 2], o[n][1][e], o[n][1][e + 2]);
+        at[1] = make_float4(o[n][2][e], o[n][2][e + 2], o[n][3][e], o[n][3][e + 2]);
+      }
+  }
+};
+
+// 1 / l for a row that saw something, 0 for one that saw nothing; NaN stays.
+__device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.0f / l; }
+
+template <bool BF16>
+__device__ __forceinline__ void store4(uint16_t* at, const float4& v, float l) {
+  const float inv = inverse(l);
+  *reinterpret_cast<uint2*>(at) = make_uint2(kv::pack16<BF16>(v.x * inv, v.y * inv), kv::pack16<BF16>(v.z * inv, v.w * inv));
+}
+
+// What a warp has on its way: keys and values of its blocks in turn, kSlots pieces of 4 KB ahead.  look(i): entry of the block table for the
+// i-th block of the warp's list.
+struct Ring {
+  uint8_t codes[kSlots][kBlock];
+};
+
+template <typename Look>
+struct Feed {
+  const Args& a;
+  Ring* ring;
+  uint64_t* full;
+  int head, count;         // key head, blocks of the list
+  Look look;
+  int slot = 0, done = 0;  // of the piece that is waited for next, pieces so far
+  uint32_t phase = 0;
+  float ks[2], vs[2];      // scales of the present block and the next; a negative key scale: there is no such block
+  int64_t next = 0;        // the next block's place in the cache
+  int later = 0;           // table entry of the block after that
+
+  __device__ __forceinline__ Feed(const Args& args, Ring* r, uint64_t* f, int h, int n, Look l)
+      : a(args), ring(r), full(f), head(h), count(n), look(l) {}
+
+  __device__ __forceinline__ int64_t resolve(int page, float* k, float* v) {
+    const bool bad = page < 0 || page >= a.cache.blocks;
+    if (bad) kv::index_error(a.err, kSiteCachedAttention);
+    const int64_t at = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
+    *k = bad ? -1.f : __ldg(a.cache.k_scale + at);
+    *v = bad ? 0.f : __ldg(a.cache.v_scale + at);
+    return at;
+  }
+  __device__ __forceinline__ void request(int s, const uint8_t* base, int64_t at) {
+    if ((threadIdx.x & 31) == 0) {
+      ptx::mbar_arrive_expect_tx(&full[s], kBlock);
+      bulk_load(ring->codes[s], base + at * kBlock, kBlock, &full[s]);
+    }
+  }
+  __device__ __forceinline__ void begin() {
+    static_assert(kSlots == 3, "keys and values of the first block, keys of the second");
+    const int p0 = look(0), p1 = count > 1 ? look(1) : 0;
+    const int64_t at = resolve(p0, &ks[0], &vs[0]);
+    request(0, a.cache.k, at);
+    request(1, a.cache.v, at);
+    if (count > 1) {
+      next = resolve(p1, &ks[1], &vs[1]);
+      request(2, a.cache.k, next);
+    }
+    if (count > 2) later = look(2);
+  }
+  // The next piece, once it is there; nullptr: gave up, with the pieces on their way landed.
+  __device__ __forceinline__ const uint8_t* wait(const ptx::AbortCtx& ab) {
+    if (__all_sync(0xffffffffu, ptx::mbar_wait(&full[slot], phase, ab, 330))) return ring->codes[slot];
+    const long long t0 = clock64();
+    int s = slot;
+    uint32_t ph = phase;
+    for (int k = 0; (threadIdx.x & 31) == 0 && k < kSlots && done + k < 2 * count; ++k) {
+      while (!ptx::mbar_try_wait(&full[s], ph) && clock64() - t0 < ptx::kWaitCycles) {
+      }
+      if (++s == kSlots) {
+        s = 0;
+        ph ^= 1;
+      }
+    }
+    __syncwarp();
+    return nullptr;
+  }
+  __device__ __forceinline__ void advance() {
+    ++done;
+    if (++slot == kSlots) {
+      slot = 0;
+      phase ^= 1;
+    }
+  }
+  // block i's keys have been read: its slot takes the values of block i + 1
+  __device__ __forceinline__ void keys_read(int i) {
+    if (i + 1 < count) request(slot, a.cache.v, next);
+    advance();
+  }
+  // its values: the slot takes the keys of block i + 2
+  __device__ __forceinline__ void values_read(int i) {
+    ks[0] = ks[1];
+    vs[0] = vs[1];
+    if (i + 2 < count) {
+      next = resolve(later, &ks[1], &vs[1]);
+      request(slot, a.cache.k, next);
+    }
+    if (i + 3 < count) later = look(i + 3);
+    advance();
+  }
+};
+
+struct Smem {
+  Ring ring[kWarps];  // afterwards the first 4 KB of a warp's ring are its output, fp32 [16][64]
+  float sum[16][64];  // of the CTA
+  float2 sum_ml[16];
+  float2 ml[kWarps][16];
+  uint64_t full[kWarps][kSlots];
+  int cost[kWarps * 32 + 1];
+  int abort_flag;
+};
+static_assert(4 * (sizeof(Smem) + 1024) <= 228 * 1024, "four CTAs share an SM");
+
+template <bool BF16, bool INT8, int NT>
+__global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   RT_PDL_LAUNCH_DEPENDENTS();
@@ -106,242 +468,54 @@ __global__ void __launch_bounds__(kWarps * 32, 3) few_rows_kernel(const Args a) 
   int rest = blockIdx.x / a.splits;
   const int tile = rest % a.tiles;
   rest /= a.tiles;
-  const int head = rest % a.cache.heads, seq = rest / a.cache.heads;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-
-  const CachedRows seq_rows(a, seq);
-  if (!seq_rows.ok) return;
-  const int rows = seq_rows.rows, row0 = tile * 16;
-  if (row0 >= rows) return;
-  auto limit_of = [&](int row) { return row < rows ? seq_rows.limit(a, row) : 0; };  // keys that a row sees
-  const int least = limit_of(row0), most = limit_of(min(row0 + 16, rows) - 1);
-  const int lim0 = limit_of(row0 + g), lim1 = limit_of(row0 + g + 8);
-  const bool two = row0 + 8 < rows;  // the tile's upper eight rows are in use
-
-  uint32_t q[4][4];
-  float unit0, unit1;
-  {
-    uint32_t lo[8], hi[8];
-    unit0 = load_query<BF16>(row0 + g < rows ? seq_rows.query(a, head, row0 + g) : nullptr, t, lo);
-    unit1 = load_query<BF16>(row0 + g + 8 < rows ? seq_rows.query(a, head, row0 + g + 8) : nullptr, t, hi);
-#pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      q[s][0] = lo[2 * s];
-      q[s][1] = hi[2 * s];
-      q[s][2] = lo[2 * s + 1];
-      q[s][3] = hi[2 * s + 1];
-    }
+  const int head = rest % a.cache.heads;
+  int seq = rest / a.cache.heads;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (a.sorted) {
+    const int tid = threadIdx.x;
+    seq = index_by_cost(sm.cost, a.n_seq, tid < a.n_seq ? a.context[tid] : 0, seq);
   }
-  unit0 *= a.scale_log2 * C::kUnit;
-  unit1 *= a.scale_log2 * C::kUnit;
 
-  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-  float o[8][4];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-
-  const int n_blocks = (most + 63) / 64, step = a.splits * kWarps;
+  const CachedRows sr(a, seq);
+  if (!sr.ok) return;
+  using Tile = RowTile<BF16, INT8, NT>;
+  const int row0 = tile * Tile::kRows;
+  if (row0 >= sr.rows) return;
+  const int valid = min(Tile::kRows, sr.rows - row0);
+  const int n_blocks = (sr.limit(a, row0 + valid - 1) + 63) / 64, step = a.splits * kWarps;
   const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
-  const int b0 = rank * kWarps + warp;
+  const int b0 = rank * kWarps + warp;  // this warp's blocks: every step-th one
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
-      for (int s = 0; s < kStages; ++s) ptx::mbar_init(&sm.full[w][s], 1);
+      for (int s = 0; s < kSlots; ++s) ptx::mbar_init(&sm.full[w][s], 1);
     sm.abort_flag = 0;
     ptx::fence_barrier_init();
   }
   __syncthreads();
   ptx::AbortCtx ab{&sm.abort_flag, a.err};
-  // A block on its way: its scales, negative where the table has no such block.
-  float ks[kStages], vs[kStages];
-  int page[kStages];  // of the blocks to be requested next
-  auto look = [&](int s, int b) { page[s] = b < n_blocks ? __ldg(table + b) : -1; };
-  auto request = [&](int s, int b) {
-    if (b >= n_blocks) return;
-    const bool bad = page[s] < 0 || page[s] >= a.cache.blocks;
-    if (bad && lane == 0) kv::index_error(a.err, kSiteCachedAttention);
-    const int64_t slot = static_cast<int64_t>(bad ? 0 : page[s]) * a.cache.heads + head;
-    if (lane == 0) {
-      ptx::mbar_arrive_expect_tx(&sm.full[warp][s], 8192);
-      bulk_load(sm.ring[warp][s][0], a.cache.k + slot * 4096, 4096, &sm.full[warp][s]);
-      bulk_load(sm.ring[warp][s][1], a.cache.v + slot * 4096, 4096, &sm.full[warp][s]);
-    }
-    ks[s] = bad ? -1.f : __ldg(a.cache.k_scale + slot);
-    vs[s] = __ldg(a.cache.v_scale + slot);
-  };
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) look(s, b0 + s * step);
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) request(s, b0 + s * step);
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) look(s, b0 + (kStages + s) * step);
+  const int count = b0 < n_blocks ? (n_blocks - b0 + step - 1) / step : 0;
+  auto look = [&](int i) { return __ldg(table + b0 + i * step); };
+  Feed<decltype(look)> feed(a, &sm.ring[warp], sm.full[warp], head, count, look);
+  if (count > 0) feed.begin();
 
-  // Thread (g, t) takes key row g ^ (t's lowest bit) of every eight, so that the rows that four threads read at once are even and odd:
-  // rows are 64 bytes, banks repeat after 128.
-  const int kg = g ^ ((g >> 1) & 1), odd = t & 1;
-  bool ok = true;
-  uint32_t phase = 0;
-  for (int bb = b0; bb < n_blocks && ok; bb += kStages * step, phase ^= 1) {
-#pragma unroll
-    for (int st = 0; st < kStages; ++st) {
-      const int b = bb + st * step;
-      if (b >= n_blocks) break;
-      if (!__all_sync(0xffffffffu, ptx::mbar_wait(&sm.full[warp][st], phase, ab, 330))) {
-        // gives up: copies in flight land before the ring is used again
-        const long long t0 = clock64();
-        for (int s = 0; lane == 0 && s < kStages; ++s) {
-          const bool next = s < st;  // the slot has been requested again
-          if (bb + (next ? kStages + s : s) * step >= n_blocks) continue;
-          while (!ptx::mbar_try_wait(&sm.full[warp][s], next ? phase ^ 1 : phase) && clock64() - t0 < ptx::kWaitCycles) {
-          }
-        }
-        __syncwarp();
-        ok = false;
-        break;
-      }
-      const uint8_t* kp = sm.ring[warp][st][0];
-      const uint8_t* vp = sm.ring[warp][st][1];
-      const float k_scale = ks[st], v_scale = vs[st] * C::kUnit;
-      uint4 kw[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) kw[j] = *reinterpret_cast<const uint4*>(kp + (8 * j + kg) * 64 + 16 * t);
-
-      // scores; step s of the product covers dimensions 16 t + 4 s .. + 3 of every thread's share
-      float sc[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-        const uint32_t w[4] = {kw[j].x, kw[j].y, kw[j].z, kw[j].w};
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const uint32_t p = C::prepare(w[s]);
-          mma16816(sc[j], q[s], C::template pair<0>(p), C::template pair<2>(p));
-        }
-      }
-      const float u0 = unit0 * k_scale, u1 = unit1 * k_scale;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sc[j][0] *= u0;
-        sc[j][1] *= u0;
-        sc[j][2] *= u1;
-        sc[j][3] *= u1;
-      }
-      if (b * 64 + 64 > least || k_scale < 0.f) {  // keys that some row of the tile does not see
-        const int l0 = k_scale < 0.f ? 0 : lim0, l1 = k_scale < 0.f ? 0 : lim1;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int key = b * 64 + 8 * j + 2 * t;
-          if (key + odd >= l0) sc[j][0] = -INFINITY;
-          if (key + 1 - odd >= l0) sc[j][1] = -INFINITY;
-          if (key + odd >= l1) sc[j][2] = -INFINITY;
-          if (key + 1 - odd >= l1) sc[j][3] = -INFINITY;
-        }
-      }
-      float x0 = -INFINITY, x1 = -INFINITY;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        x0 = fmaxf(x0, fmaxf(sc[j][0], sc[j][1]));
-        x1 = fmaxf(x1, fmaxf(sc[j][2], sc[j][3]));
-      }
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 1));
-      x0 = fmaxf(x0, __shfl_xor_sync(0xffffffffu, x0, 2));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 1));
-      x1 = fmaxf(x1, __shfl_xor_sync(0xffffffffu, x1, 2));
-      x0 = fmaxf(x0, m0);
-      x1 = fmaxf(x1, m1);
-      // a row that has seen nothing yet: every exponential below is 2^(-inf)
-      const float r0 = x0 == -INFINITY ? 0.f : x0, r1 = x1 == -INFINITY ? 0.f : x1;
-      const float c0 = ex2(m0 - r0), c1 = ex2(m1 - r1);
-      m0 = x0;
-      m1 = x1;
-      l0 *= c0;
-      l1 *= c1;
-      uint32_t p[4][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float e0 = ex2(sc[j][0] - r0), e1 = ex2(sc[j][1] - r0);
-        l0 += e0 + e1;
-        p[j >> 1][(j & 1) * 2] = kv::pack16<false>(e0, e1);
-        p[j >> 1][(j & 1) * 2 + 1] = 0u;
-      }
-      if (two) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float e0 = ex2(sc[j][2] - r1), e1 = ex2(sc[j][3] - r1);
-          l1 += e0 + e1;
-          p[j >> 1][(j & 1) * 2 + 1] = kv::pack16<false>(e0, e1);
-        }
-      }
-      uint2 vw[16];  // keys 16 s + 2 t, + 1, + 8, + 9 of every step s of 16 keys, dimensions 8 g .. 8 g + 7
-#pragma unroll
-      for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          vw[4 * s + i] = *reinterpret_cast<const uint2*>(vp + (16 * s + 2 * t + ((i & 1) ^ odd) + 4 * (i & 2)) * 64 + 8 * g);
-      __syncwarp();  // the slot has been read
-      request(st, b + kStages * step);
-      look(st, b + 2 * kStages * step);
-      // output: column c of 8-column tile j is dimension 8 c + j
-      float acc[8][4];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint2* w = vw + 4 * s;
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {  // dimensions 8 g + 4 half .. + 3
-          const uint32_t ka = half ? w[0].y : w[0].x, kb = half ? w[1].y : w[1].x;
-          const uint32_t kc = half ? w[2].y : w[2].x, kd = half ? w[3].y : w[3].x;
-          const uint32_t ab0 = C::prepare(kv::prmt(ka, kb, 0x5140u)), ab1 = C::prepare(kv::prmt(ka, kb, 0x7362u));
-          const uint32_t cd0 = C::prepare(kv::prmt(kc, kd, 0x5140u)), cd1 = C::prepare(kv::prmt(kc, kd, 0x7362u));
-          mma16816(acc[4 * half], p[s], C::template pair<0>(ab0), C::template pair<0>(cd0));
-          mma16816(acc[4 * half + 1], p[s], C::template pair<2>(ab0), C::template pair<2>(cd0));
-          mma16816(acc[4 * half + 2], p[s], C::template pair<0>(ab1), C::template pair<0>(cd1));
-          mma16816(acc[4 * half + 3], p[s], C::template pair<2>(ab1), C::template pair<2>(cd1));
-        }
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        o[j][0] = fmaf(acc[j][0], v_scale, o[j][0] * c0);
-        o[j][1] = fmaf(acc[j][1], v_scale, o[j][1] * c0);
-      }
-      if (two) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          o[j][2] = fmaf(acc[j][2], v_scale, o[j][2] * c1);
-          o[j][3] = fmaf(acc[j][3], v_scale, o[j][3] * c1);
-        }
-      }
-    }
+  Tile rows;
+  rows.g = lane >> 2;
+  rows.t = lane & 3;
+  rows.begin(a, sr, head, row0);
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    const uint8_t* kp = feed.wait(ab);
+    if (!kp) break;
+    if (!rows.block(kp, feed.ks[0], feed.vs[0], b0 + i * step, [&] { feed.keys_read(i); }, [&] { return feed.wait(ab); },
+                    [&] { feed.values_read(i); }))
+      break;
   }
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 1);
-  l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-  l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
 
-  // ---- the warps of the CTA.  Thread (g, t) holds dimensions 16 t .. 16 t + 15 of rows g and g + 8.
-  auto out_of = [&](int w) { return reinterpret_cast<float(*)[64]>(sm.ring[w][0][0]); };
-  if (t == 0) {
-    sm.ml[warp][g] = make_float2(m0, l0);
-    sm.ml[warp][g + 8] = make_float2(m1, l1);
-  }
-#pragma unroll
-  for (int c = 0; c < 2; ++c)
-#pragma unroll
-    for (int j = 0; j < 8; j += 4) {
-      *reinterpret_cast<float4*>(&out_of(warp)[g][16 * t + 8 * c + j]) = make_float4(o[j][c], o[j + 1][c], o[j + 2][c], o[j + 3][c]);
-      if (two)
-        *reinterpret_cast<float4*>(&out_of(warp)[g + 8][16 * t + 8 * c + j]) =
-            make_float4(o[j][2 + c], o[j + 1][2 + c], o[j + 2][2 + c], o[j + 3][2 + c]);
-    }
+  // ---- the warps of the CTA
+  auto out_of = [&](int w) { return reinterpret_cast<float(*)[64]>(sm.ring[w].codes[0]); };
+  rows.put(out_of(warp), sm.ml[warp], valid);
   __syncthreads();
-  auto store = [&](int r, int d, float4 v, float l) {
-    const float inv = l > 0.f ? 1.0f / l : (l == 0.f ? 0.f : l);  // NaN stays
-    uint2 w;
-    w.x = kv::pack16<BF16>(v.x * inv, v.y * inv);
-    w.y = kv::pack16<BF16>(v.z * inv, v.w * inv);
-    *reinterpret_cast<uint2*>(seq_rows.output(a, head, row0 + r) + d) = w;
-  };
-  const int valid = min(16, rows - row0);
+  auto store = [&](int r, int d, const float4& v, float l) { store4<BF16>(sr.output(a, head, row0 + r) + d, v, l); };
   for (int i = threadIdx.x; i < valid * 16; i += kWarps * 32) {
     const int r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
@@ -376,6 +550,7 @@ __global__ void __launch_bounds__(kWarps * 32, 3) few_rows_kernel(const Args a) 
     const uint32_t ml_at = ptx::smem_u32(&sm.sum_ml[r]), o_at = ptx::smem_u32(&sm.sum[r][d]);
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll 4
     for (int w = 0; w < a.splits; ++w) M = fmaxf(M, kv::ld_cluster_f2(kv::peer_address(ml_at, w)).x);
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll 4
@@ -395,14 +570,25 @@ __global__ void __launch_bounds__(kWarps * 32, 3) few_rows_kernel(const Args a) 
   ptx::cluster_wait();
 }
 
-rt_status launch_few_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) {
-  auto kern = bf16 ? (int8 ? few_rows_kernel<true, true> : few_rows_kernel<true, false>)
-                   : (int8 ? few_rows_kernel<false, true> : few_rows_kernel<false, false>);
-  const int64_t grid = static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits;
+constexpr int kSms = 148;
+
+// CTAs that share a tile's keys, a power of two (clusters of 3 or 6 run slower than of 2 or 4): as many as have a block for every warp and do not
+// make more than 1.35 rounds of CTAs.  One round is best for equal lengths (8 x 4096 tokens, 12 heads: 16.3 us with 4, 20.1 with 8),
+// two with the long sequences first for ragged ones (24 x 1000 to 16384 tokens, 4 key heads: 38.6 us with 4, 31 with 8).
+// With 16 rows a tile results weigh more, and one round it is.
+int splits_of(int64_t units, int tile_rows, int64_t keys) {
+  const int64_t slots = kSms * ctas_per_sm(tile_rows / 8), room = tile_rows == 8 ? slots * 135 / 100 : slots;
+  int splits = 1;
+  while (splits < kMaxSplits && units * splits * 2 <= room && keys > 64 * kWarps * splits) splits *= 2;
+  return splits;
+}
+
+template <bool BF16, bool INT8, int NT>
+rt_status launch_few_rows(const Args& a, cudaStream_t st) {
+  auto kern = few_rows_kernel<BF16, INT8, NT>;
   RT_TRY(ensure_kernel_smem(reinterpret_cast<const void*>(kern), sizeof(Smem), true));
-  if (a.splits > 8) RT_TRY(ensure_large_clusters(reinterpret_cast<const void*>(kern)));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = st;
@@ -419,6 +605,11 @@ rt_status launch_few_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) 
   count_launch();
   RT_CHECK_CUDA(cudaGetLastError());
   return RT_OK;
+}
+
+template <bool BF16, bool INT8>
+rt_status launch_by_rows(const Args& a, cudaStream_t st) {
+  return a.tile_rows == 8 ? launch_few_rows<BF16, INT8, 1>(a, st) : launch_few_rows<BF16, INT8, 2>(a, st);
 }
 
 }  // namespace
@@ -441,7 +632,6 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   RT_REQUIRE(out && q, RT_ERR_INVALID, "cached_attention: null pointer");
   RT_REQUIRE(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0 && q_stride % 8 == 0 && q_stride >= 0,
              RT_ERR_INVALID, "cached_attention: queries and output must be 16-byte aligned, the query stride a multiple of 8 values");
-  max_q = std::min(max_q, tokens);
   a.out = static_cast<uint16_t*>(out);
   a.q = static_cast<const uint16_t*>(q);
   a.q_stride = q_stride;
@@ -451,32 +641,33 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   a.first = first;
   a.n_seq = n_seq;
   a.tokens = tokens;
-  a.max_q = max_q;
+  a.max_q = std::min(max_q, tokens);
   a.heads = heads;
   a.group = heads / a.cache.heads;
-  RT_REQUIRE(static_cast<int64_t>(max_q) * a.group < (int64_t{1} << 30), RT_ERR_UNSUPPORTED, "cached_attention: too many query rows");
-  const int rows = max_q * a.group;
-  const bool many = rows > kFewRows;
-  a.tiles = many ? (rows + 255) / 256 : (rows + 15) / 16;
-  const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
-  RT_REQUIRE(heads_of_all < (int64_t{1} << 28) && heads_of_all * a.tiles < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
-             "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.causal = causal != 0;
+  RT_REQUIRE(static_cast<int64_t>(a.max_q) * a.group < (int64_t{1} << 30), RT_ERR_UNSUPPORTED, "cached_attention: too many query rows");
+  const int rows = a.max_q * a.group;
+  const bool many = rows > kFewRows;
+  a.tile_rows = many ? 256 : rows <= 8 ? 8 : 16;
+  a.tiles = (rows + a.tile_rows - 1) / a.tile_rows;
+  const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
+  RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * a.tiles < (int64_t{1} << 26), RT_ERR_UNSUPPORTED,
+             "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
   a.err = device_error_word();
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "cached_attention: cannot allocate the device error word");
-  const int64_t widest = static_cast<int64_t>(table_stride) * 64;
+  const int64_t widest = static_cast<int64_t>(table_stride) * 64, units = heads_of_all * a.tiles;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
-  a.splits = 1;
-  if (many) {
-    // tiles of up to 256 rows see very different numbers of keys under the causal rule: four CTAs per SM over the call balance them
-    while (a.splits < 8 && heads_of_all * a.tiles * a.splits < 4 * 148 && keys > 512 * a.splits) a.splits *= 2;
-  } else {
-    // 16 blocks a CTA, four a warp; fewer, down to one a warp, until the chip is full
-    while (a.splits < kMaxSplits && (keys > 1024 * a.splits || (heads_of_all * a.tiles * a.splits < 4 * 148 && keys > 256 * a.splits)))
-      a.splits *= 2;
-  }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == RT_BF16, int8 = cache->format == RT_KV_INT8;
-  return many ? launch_cached_attention_many_rows(a, bf16, int8, st) : launch_few_rows(a, bf16, int8, st);
+  if (many) {
+    // tiles of up to 256 rows see very different numbers of keys under the causal rule: four CTAs per SM over the call balance them
+    a.splits = 1;
+    while (a.splits < 8 && units * a.splits < 4 * kSms && keys > 512 * a.splits) a.splits *= 2;
+    return launch_cached_attention_many_rows(a, bf16, int8, st);
+  }
+  a.splits = splits_of(units, a.tile_rows, keys);
+  a.sorted = n_seq > 1 && n_seq <= kWarps * 32 && units * a.splits > kSms * ctas_per_sm(a.tile_rows / 8);
+  if (bf16) return int8 ? launch_by_rows<true, true>(a, st) : launch_by_rows<true, false>(a, st);
+  return int8 ? launch_by_rows<false, true>(a, st) : launch_by_rows<false, false>(a, st);
 }

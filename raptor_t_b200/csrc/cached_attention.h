@@ -15,8 +15,9 @@ struct CachedAttentionArgs {
   const int32_t* context;
   const int32_t* first;
   int n_seq, tokens, max_q, heads, group;  // group: query heads of a key head
-  int tiles;                               // row tiles of the longest sequence
+  int tile_rows, tiles;                    // rows of a tile, tiles of the longest sequence
   int splits;                              // CTAs of a cluster that share a tile's keys
+  int sorted;                              // long sequences first
   float scale_log2;
   int causal;
   int* err;
@@ -34,7 +35,7 @@ struct CachedRows {
     n = rows = 0;
     if (!ok) return;
     if (f0 < 0 || f1 > a.tokens || f1 - f0 > a.max_q || ctx < 0 || ctx > static_cast<int64_t>(a.table_stride) * 64) {
-      if (threadIdx.x == 0) kv::index_error(a.err, kSiteCachedAttention);
+      kv::index_error(a.err, kSiteCachedAttention);
       ok = false;
       return;
     }
@@ -51,6 +52,22 @@ struct CachedRows {
     return a.out + (static_cast<int64_t>(f0 + row / a.group) * a.heads + head * a.group + row % a.group) * 64;
   }
 };
+
+// The `place`-th largest of `n` costs (equal ones in order of their index), n at most the CTA's threads; cost[] in shared memory, n + 1 ints.
+// All threads of the CTA call it; `mine` is the cost of the calling thread's index.
+// CTAs start in order of their index: with the longest work first the last ones to end are short.
+__device__ __forceinline__ int index_by_cost(int* cost, int n, int mine, int place) {
+  const int tid = threadIdx.x;
+  if (tid < n) cost[tid] = mine;
+  __syncthreads();
+  if (tid < n) {
+    int before = 0;
+    for (int i = 0; i < n; ++i) before += cost[i] > mine || (cost[i] == mine && i < tid);
+    if (before == place) cost[n] = tid;
+  }
+  __syncthreads();
+  return cost[n];
+}
 
 namespace kv {
 

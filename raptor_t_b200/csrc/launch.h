@@ -12,9 +12,6 @@ namespace rt {
 // pair: sets them the first time `func` is launched on the current device.
 rt_status ensure_kernel_smem(const void* func, int smem_bytes, bool max_carveout);
 
-// Clusters of more than eight CTAs (up to 16) for `func` on the current device, from its first launch on.
-rt_status ensure_large_clusters(const void* func);
-
 template <typename... KArgs, typename... Args>
 cudaError_t launch_kernel(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
   cudaLaunchConfig_t cfg{};

@@ -45,17 +45,6 @@ rt_status ensure_kernel_smem(const void* func, int smem_bytes, bool max_carveout
   return RT_OK;
 }
 
-rt_status ensure_large_clusters(const void* func) {
-  static std::set<std::pair<const void*, int>> done;
-  int dev = 0;
-  RT_CHECK_CUDA(cudaGetDevice(&dev));
-  std::lock_guard<std::mutex> lk(g_attr_mu);
-  if (done.count({func, dev})) return RT_OK;
-  RT_CHECK_CUDA(cudaFuncSetAttribute(func, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  done.insert({func, dev});
-  return RT_OK;
-}
-
 namespace {
 std::mutex g_err_mu;
 int* g_err_words[64] = {nullptr};

@@ -84,6 +84,26 @@ def test_queries_with_a_stride(ops):
     _case(ops, torch.float8_e4m3fn, torch.bfloat16, 4, 2, [1, 20, 150], [100, 20, 400], True, stride=3 * 4 * 64)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,most", [(2, 2, 1), (6, 2, 1), (8, 1, 4), (2, 1, 20)])
+def test_many_sequences(ops, fmt, causal, heads, kv_heads, most):
+    """Calls whose blocks are one list that all warps share: more than 128 sequences, some without rows, some without keys, lengths
+    from one token to some that several warps work on."""
+    import random
+    rng = random.Random(heads + most)
+    counts = [rng.choice([0, 1, 1, rng.randint(1, most)]) for _ in range(300)]
+    context = [rng.choice([0, 1, 64, 65, rng.randint(1, 700), rng.randint(1, 2000)]) for _ in range(300)]
+    counts[0], context[0], counts[-1], context[-1] = 0, 0, most, 3000
+    for dtype in DTYPES:
+        _case(ops, fmt, dtype, heads, kv_heads, counts, context, causal, spare_rows=2, max_q=most)
+
+
+@pytest.mark.parametrize("counts,context", [([1] * 8, [6000, 1, 4096, 4097, 0, 63, 5000, 3333]), ([1], [60000]), ([3, 16], [17000, 16001])])
+def test_long_contexts(ops, counts, context):
+    _case(ops, torch.int8, torch.bfloat16, 12, 12, counts, context, True)
+
+
 @pytest.mark.parametrize("rows", [1, 40, 200])
 @pytest.mark.parametrize("max_context", [1, 64, 100000])
 def test_max_context_only_guides(ops, rows, max_context):
