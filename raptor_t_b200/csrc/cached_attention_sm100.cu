@@ -1,25 +1,28 @@
 // Attention of many query rows over the 8-bit key/value cache (layout: kv_cache.cuh) on tcgen05: whole questions and
 // continuations.
 //
-// A CTA owns up to 256 rows (token x query head of the group) of one sequence and key head, as two streams of 128: rows 0-127 and rows
-// 128-255 over the same keys, or, where the tile has at most 128 rows, the same rows over the even and the odd steps.  A step is 128 keys
-// (two blocks of the cache).  Two streams keep the exponential unit busy: one computes while the other loads, stores and waits.
+// A CTA owns up to 256 rows (token x query head of the group) of one sequence and key head.  Its work is four streams of 128 rows that know
+// nothing of one another until the end: two row tiles times even and odd blocks of 64 keys, or, where there are at most 128 rows, one row tile
+// times every fourth block.  A stream's step is one block: scores, softmax, output, one after the other; the four streams fill each other's waits.
 //
-//   warps 0-3, 4-7   softmax of stream 0, 1: thread r owns row r (TMEM lane r), as in attention_sm100.cu: score row from TMEM, running
-//                    maximum and sum in fp32, 16-bit probabilities back to TMEM, output rescaled only when the maximum has grown by
-//                    more than 2^8.
-//   warps 8-11       bring the codes: bulk copies of whole blocks (4 KB) a few steps ahead into a ring, from there exact conversion to
-//                    halves and stores into the 128-byte-swizzled operand tiles (keys K-major, values MN-major).  The tile that 256
-//                    rows share is converted once.
-//   warps 12-15      issue the MMAs: scores and outputs of stream 0, scores and outputs of stream 1.
+//   warps 0-15       softmax, four warps a stream: thread r owns row r (TMEM lane r).  Score row from TMEM, running maximum and sum in fp32
+//                    (base-2 exponentials, every eighth pair on the FMA pipe), probabilities as halves over the scores' columns, output
+//                    rescaled only when the maximum has grown by more than 2^8.
+//   warps 16-19      bring the codes: bulk copies of whole blocks a few blocks ahead into a ring, from there exact conversion to
+//                    halves and stores into the 128-byte-swizzled operand tiles (keys K-major, values MN-major).  The block that two row
+//                    tiles share is converted once.
+//   warps 20-23      issue the MMAs, one warp a stream: S = Q K^T (M 128, N 64, K 64), and when the probabilities are there O += P V (P
+//                    from TMEM), then the next block's scores.
 // A block's key scale multiplies its scores.  Its value scale goes into the probabilities, relative to the largest one of the keys that the CTA
 // visits: p' = p * scale / largest * 2^7 (2^7: halves keep all their bits down to p = 2^-21 of the row's maximum; p' <= 2^15).
 //
-// Bound by the exponentials (16 a clock and SM) and the softmax warps' issue slots.
+// Bound by the softmax warps' issue slots and the exponentials (16 a clock and SM).  Two streams of 128 keys a step, eight softmax warps an SM, took
+// 2.0 us for 256 rows x 128 keys: eight warps do not cover each other's latencies.
 // Few tiles over many keys are split over the CTAs of a cluster; partial results, of streams and of CTAs, meet in (distributed) shared memory.
 #include "cached_attention.h"
 
 #include <algorithm>
+#include <type_traits>
 
 #include "device_error.h"
 #include "launch.h"
@@ -34,35 +37,42 @@ using namespace ptx;
 using namespace softmax;
 using Args = CachedAttentionArgs;
 
-constexpr int kThreads = 512;
-constexpr int kStages = 3;               // of keys, and of values
-constexpr int kRaw = 4;                  // steps of codes on their way
-constexpr int kBlock = 4096;             // codes of a block
-constexpr int kRing = 16;                // scales of a step, read up to two steps after its keys' slot is free
-constexpr int kHalfTile = 64 * 128;      // 64 rows of 64 halves
-constexpr int kTile = 2 * kHalfTile;
+constexpr int kThreads = 768;
+constexpr int kSoftmaxThreads = 512;
+constexpr int kStreams = 4;
+constexpr int kMaxSplits = 8;            // CTAs of a cluster
+constexpr int kStages = 4;               // operand tiles of keys, and of values: one for each warp that fills them
+constexpr int kRaw = 8;                  // blocks of codes on their way
+constexpr int kBlock = 4096;             // codes of a block's keys, or values
+constexpr int kRing = 32;                // scales of a block, read after its operand slots are free again
+constexpr int kTile = 64 * 128;          // 64 rows of 64 halves
 constexpr int kTmemCols = 512;
-constexpr int kColS = 0, kColO = 256, kColP = 384;  // 2 x 128 scores, 2 x 64 outputs, 2 x 64 packed probabilities
+constexpr int kColS = 0, kColO = 256;    // 4 x 64 scores (probabilities in the first half of them), 4 x 64 outputs
 constexpr float kRescaleThreshold = 8.0f;
+constexpr int kPolyEvery = 8;            // pairs; 256 rows, 64 blocks: 81.8 us, with 4 83.6, with none 82.5
 constexpr float kShift = 7.0f;           // p' is 2^7 times larger than p * scale / largest scale
-// 8 x 200 + 4 x 72 + 4 x 40 = 16 x 128 registers a lane, what the launch has
-constexpr int kRegsSoftmax = 200, kRegsBring = 72, kRegsIssue = 40;
+// 16 x 96 + 4 x 56 + 4 x 40 = 24 x 80 registers a lane, what the launch has
+constexpr int kRegsSoftmax = 96, kRegsBring = 56, kRegsIssue = 40;
 
 struct Smem {
-  uint8_t q[2][kTile];
+  uint8_t q[2][2 * kTile];
+  // afterwards k, v and raw hold partial results, [4 streams][128 rows][64] fp32
   uint8_t k[kStages][kTile];
   uint8_t v[kStages][kTile];
-  uint8_t raw[kRaw][4 * kBlock];  // keys of block 0, 1, values of block 0, 1; afterwards: partial results, [2][128 rows][64] fp32
-  uint64_t raw_full[kRaw], raw_empty[kRaw];
+  uint8_t raw[kRaw][2 * kBlock];  // keys, values
+  uint64_t raw_full[kRaw];
   uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[2], s_free[2], p_full[2][2], pv_done[2];
-  float4 scales[kRing];  // {key scale of block 0, 1, value scale of block 0, 1}
-  float2 ml[2][128];
-  float vmax[8];
+  uint64_t s_full[kStreams], p_full[kStreams], o_full[kStreams];
+  float2 scales[kRing];  // key and value scale of a block; a negative key scale: nobody sees its keys
+  float2 ml[kStreams][128];
+  float2 ml_cta[256];
+  float weight[kStreams][128];
+  float vmax[kSoftmaxThreads / 32];
+  int cost[kThreads + 1];
   uint32_t tmem_slot;
   int abort_flag;
 };
-static_assert(kRaw * 4 * kBlock >= 2 * 128 * 64 * 4, "partial results fit the ring of codes");
+static_assert(kStages * 2 * kTile + kRaw * 2 * kBlock >= kStreams * 128 * 64 * 4, "partial results fit the operand tiles and the ring");
 static_assert(sizeof(Smem) <= 227 * 1024, "one CTA per SM");
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
@@ -71,7 +81,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of t
   return r;
 }
 
-__device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+__device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
 // Contiguous copy global -> shared (16-byte aligned), completion on an mbarrier.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -105,56 +115,58 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   RT_PDL_LAUNCH_DEPENDENTS();
   RT_PDL_WAIT();
-  // ---- what this CTA works on; the same for all CTAs of a cluster but for the keys.  The last tiles, which see most
-  // under the causal rule, start first.
+  // ---- what this CTA works on; the same for all CTAs of a cluster but for the keys.  Tiles that see most start first.
   const int rank = blockIdx.x % a.splits;
-  const int item = blockIdx.x / a.splits;
-  const int per_tile = a.n_seq * a.cache.heads;
-  const int tile = a.tiles - 1 - item / per_tile;
-  const int head = item % per_tile % a.cache.heads, seq = item % per_tile / a.cache.heads;
+  const int head = blockIdx.x / a.splits % a.cache.heads;
+  int item = blockIdx.x / a.splits / a.cache.heads;  // (sequence, tile), the last tiles first
+  const int items = a.n_seq * a.tiles;
+  if (a.sorted) {
+    int cost = -1;
+    if (tid < items) {
+      const int s = tid % a.n_seq, first_row = (a.tiles - 1 - tid / a.n_seq) * 256;
+      const int rows = (a.first[s + 1] - a.first[s]) * a.group, last = min(first_row + 256, rows) - 1;
+      if (last >= first_row) cost = a.causal ? a.context[s] - (rows - 1 - last) / a.group : a.context[s];
+    }
+    item = index_by_cost(sm.cost, items, cost, item);
+  }
+  const int tile = a.tiles - 1 - item / a.n_seq, seq = item % a.n_seq;
   const CachedRows sr(a, seq);
   if (!sr.ok) return;
   const int row0 = tile * 256, here = min(256, sr.rows - row0);
   if (here <= 0) return;
-  const bool two = here > 128;  // two row tiles; otherwise one whose steps the streams share
+  const bool two = here > 128;  // two row tiles, each with two streams; otherwise one with four
   const int most = sr.limit(a, row0 + here - 1);
-  const int n_blocks = (most + 63) / 64;
-  const int all_steps = (n_blocks + 1) / 2, each = (all_steps + a.splits - 1) / a.splits;
-  const int j0 = min(rank * each, all_steps);
-  const int n_steps = min(j0 + each, all_steps) - j0;
-  // steps of stream x: the first steps_of(0) of a first row tile that sees less, or every second one
-  const int steps0 = two ? min(n_steps, max(0, (sr.limit(a, row0 + 127) + 127) / 128 - j0)) : (n_steps + 1) / 2;
-  auto steps_of = [&](int x) { return x == 0 ? steps0 : two ? n_steps : n_steps / 2; };
-  auto uses = [&](int x, int j) { return two ? (x == 1 || j < steps0) : (j & 1) == x; };
-  const bool combine = !two || a.splits > 1;
+  const int all_blocks = (most + 63) / 64, each = (all_blocks + a.splits - 1) / a.splits;
+  const int j0 = min(rank * each, all_blocks);
+  const int n_blocks = min(j0 + each, all_blocks) - j0;
+  // Stream x takes blocks first_of(x), + stride, ... below end_of(x): a first row tile may see less.
+  const int stride = two ? 2 : 4;
+  const int end0 = two ? min(n_blocks, max(0, (sr.limit(a, row0 + 127) + 63) / 64 - j0)) : n_blocks;
+  auto first_of = [&](int x) { return two ? x & 1 : x; };
+  auto end_of = [&](int x) { return two && x < 2 ? end0 : n_blocks; };
 
   if ((smem_u32(smem_raw) & 1023u) != 0) {  // the swizzled tiles need 1024-byte alignment
     if (tid == 0) atomicCAS(a.err, 0, 399);
     return;
   }
   if (tid == 0) {
-    for (int x = 0; x < 2; ++x) {
-      mbar_init(&sm.q_full[x], 4);
+    for (int x = 0; x < 2; ++x) mbar_init(&sm.q_full[x], two ? 8 : 16);  // the warps of its streams
+    for (int x = 0; x < kStreams; ++x) {
       mbar_init(&sm.s_full[x], 1);
-      mbar_init(&sm.s_free[x], 4);
-      mbar_init(&sm.p_full[x][0], 4);
-      mbar_init(&sm.p_full[x][1], 4);
-      mbar_init(&sm.pv_done[x], 1);
+      mbar_init(&sm.p_full[x], 4);
+      mbar_init(&sm.o_full[x], 1);
     }
-    for (int s = 0; s < kRaw; ++s) {
-      mbar_init(&sm.raw_full[s], 1);
-      mbar_init(&sm.raw_empty[s], 4);
-    }
+    for (int s = 0; s < kRaw; ++s) mbar_init(&sm.raw_full[s], 1);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&sm.k_full[s], 4);
-      mbar_init(&sm.k_empty[s], 2);  // both streams, whether they use the step or not
-      mbar_init(&sm.v_full[s], 4);
-      mbar_init(&sm.v_empty[s], 2);
+      mbar_init(&sm.k_full[s], 1);
+      mbar_init(&sm.k_empty[s], two ? 2 : 1);  // the streams that take the block
+      mbar_init(&sm.v_full[s], 1);
+      mbar_init(&sm.v_empty[s], two ? 2 : 1);
     }
     sm.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 20) {
     tmem_alloc(&sm.tmem_slot, kTmemCols);
     tmem_relinquish();
   }
@@ -167,78 +179,56 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, ab, site)) != 0;
   };
-  const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
-  const int64_t slots = static_cast<int64_t>(a.cache.heads);
+  const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride + j0;
 
-  if (warp >= 12) {
+  if (warp >= 20) {
     // ---------------------------------------------------------------- MMA issuers
     reg_dealloc<kRegsIssue>();
-    const int x = (warp - 12) >> 1;
+    const int x = warp - 20;
     const bool leader = elect_one();
-    int c = 0;  // steps of this stream so far
-    if (((warp - 12) & 1) == 0) {
-      constexpr uint32_t idesc128 = make_idesc_f16(128, 128, 0, false), idesc64 = make_idesc_f16(128, 64, 0, false);
-      const uint64_t dq = make_smem_desc_sw128(smem_u32(sm.q[x]));
-      const uint32_t d = tmem + kColS + x * 128;
-      if (steps_of(x) > 0 && wait(&sm.q_full[x], 0, 310)) {
-        for (int j = 0; j < n_steps; ++j) {
-          const int s = j % kStages;
-          const bool mine = uses(x, j);
-          if (mine && c > 0 && !wait(&sm.s_free[x], (c - 1) & 1, 311)) break;
-          if (!wait(&sm.k_full[s], (j / kStages) & 1, 312)) break;
-          if (mine) {
-            tc_fence_after_sync();
-            const uint64_t dk = make_smem_desc_sw128(smem_u32(sm.k[s]));
-            if (leader) {
-              const uint32_t idesc = 2 * (j0 + j) + 1 < n_blocks ? idesc128 : idesc64;
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ss(d, dq + (k * 32 >> 4), dk + (k * 32 >> 4), idesc, k ? 1u : 0u);
-              tc_commit(&sm.k_empty[s]);
-              tc_commit(&sm.s_full[x]);
-            }
-            ++c;
-          } else if (leader) {
-            mbar_arrive(&sm.k_empty[s]);
-          }
-          __syncwarp();
-        }
-      } else if (steps_of(x) == 0) {
-        for (int j = 0; j < n_steps; ++j) {
-          if (!wait(&sm.k_full[j % kStages], (j / kStages) & 1, 313)) break;
-          if (leader) mbar_arrive(&sm.k_empty[j % kStages]);
-          __syncwarp();
-        }
-      }
-    } else {
-      constexpr uint32_t idesc = make_idesc_f16(128, 64, 0, true);
-      const uint32_t d = tmem + kColO + x * 64, p = tmem + kColP + x * 64;
-      for (int j = 0; j < n_steps; ++j) {
-        const int s = j % kStages;
-        if (!wait(&sm.v_full[s], (j / kStages) & 1, 314)) break;
-        if (uses(x, j)) {
-          const uint64_t dv = make_smem_desc_sw128(smem_u32(sm.v[s]));
-          if (!wait(&sm.p_full[x][0], c & 1, 315)) break;
-          tc_fence_after_sync();
-          if (leader) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma_ts(d, p + k * 8, dv + (k * 2048 >> 4), idesc, c > 0 || k ? 1u : 0u);
-          }
-          if (!wait(&sm.p_full[x][1], c & 1, 316)) break;
-          tc_fence_after_sync();
-          if (leader) {
-            if (2 * (j0 + j) + 1 < n_blocks) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k) mma_ts(d, p + 32 + k * 8, dv + ((kHalfTile + k * 2048) >> 4), idesc, 1u);
-            }
-            tc_commit(&sm.v_empty[s]);
-            tc_commit(&sm.pv_done[x]);
-          }
-          ++c;
-        } else if (leader) {
-          mbar_arrive(&sm.v_empty[s]);
-        }
+    constexpr uint32_t idesc_s = make_idesc_f16(128, 64, 0, false), idesc_o = make_idesc_f16(128, 64, 0, true);
+    const uint64_t dq = make_smem_desc_sw128(smem_u32(sm.q[two ? x >> 1 : 0]));
+    const uint32_t d_s = tmem + kColS + x * 64, d_o = tmem + kColO + x * 64;
+    const int end = end_of(x);
+    bool ok = true;
+    uint32_t c = 0;  // steps so far
+    if (first_of(x) < end) ok = wait(&sm.q_full[two ? x >> 1 : 0], 0, 310);
+    for (int j = first_of(x); ok && j < n_blocks; j += stride) {
+      const int s = j % kStages;
+      const uint32_t round = (j / kStages) & 1;
+      ok = wait(&sm.k_full[s], round, 311);
+      if (!ok) break;
+      if (j >= end) {  // keys that this row tile does not see
+        if (leader) mbar_arrive(&sm.k_empty[s]);
+        ok = wait(&sm.v_full[s], round, 312);
+        if (leader && ok) mbar_arrive(&sm.v_empty[s]);
         __syncwarp();
+        continue;
       }
+      // the scores go over the probabilities of the step before, which its product reads
+      if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 315);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (leader) {
+        const uint64_t dk = make_smem_desc_sw128(smem_u32(sm.k[s]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_ss(d_s, dq + (k * 32 >> 4), dk + (k * 32 >> 4), idesc_s, k ? 1u : 0u);
+        tc_commit(&sm.k_empty[s]);
+        tc_commit(&sm.s_full[x]);
+      }
+      __syncwarp();
+      ok = wait(&sm.v_full[s], round, 313) && wait(&sm.p_full[x], c & 1, 314);
+      if (!ok) break;
+      tc_fence_after_sync();
+      if (leader) {
+        const uint64_t dv = make_smem_desc_sw128(smem_u32(sm.v[s]));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) mma_ts(d_o, d_s + k * 8, dv + (k * 2048 >> 4), idesc_o, c > 0 || k ? 1u : 0u);
+        tc_commit(&sm.v_empty[s]);
+        tc_commit(&sm.o_full[x]);
+      }
+      __syncwarp();
+      ++c;
     }
     __syncwarp();
     if (a.splits > 1) {
@@ -247,84 +237,67 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       cluster_arrive();
       cluster_wait();
     }
-  } else if (warp >= 8) {
+  } else if (warp >= 16) {
     // ---------------------------------------------------------------- codes to operand tiles
     reg_dealloc<kRegsBring>();
-    const int p = tid - 256;
-    auto page_of = [&](int b) { return b < n_blocks ? __ldg(table + b) : 0; };
-    // the first code of a block, and its key scale: negative where the table has no such block, whose keys nobody sees then
-    auto place_of = [&](int page, float* scale) {
+    // Every fourth block a warp: a block is one chain of waits, copies and a fence, and four chains run side by side.  Lane 0 requests the
+    // warp's blocks; their table entries were read a block earlier.
+    const int first = warp - 16;
+    auto request = [&](int j, int page) {
+      const int s = j % kRaw;
       const bool bad = page < 0 || page >= a.cache.blocks;
       if (bad) kv::index_error(a.err, kSiteCachedAttention);
-      const int64_t slot = (bad ? 0 : page) * slots + head;
-      *scale = bad ? -1.f : a.cache.k_scale[slot];
-      return slot;
+      const int64_t slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
+      mbar_arrive_expect_tx(&sm.raw_full[s], 2 * kBlock);
+      bulk_load(sm.raw[s], a.cache.k + slot * kBlock, kBlock, &sm.raw_full[s]);
+      bulk_load(sm.raw[s] + kBlock, a.cache.v + slot * kBlock, kBlock, &sm.raw_full[s]);
+      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], a.cache.v_scale[slot]);
     };
-    // thread 0 requests step j: pages and scales were read a step earlier
-    int pa = 0, pb = 0;
-    auto look = [&](int j) {
-      pa = page_of(2 * (j0 + j));
-      pb = page_of(2 * (j0 + j) + 1);
-    };
-    auto request = [&](int j) {
-      const int s = j % kRaw;
-      const bool pair = 2 * (j0 + j) + 1 < n_blocks;
-      float ka, kb;
-      const int64_t sa = place_of(pa, &ka), sb = place_of(pb, &kb);
-      const int64_t oa = sa * kBlock, ob = sb * kBlock;
-      mbar_arrive_expect_tx(&sm.raw_full[s], pair ? 4 * kBlock : 2 * kBlock);
-      bulk_load(sm.raw[s], a.cache.k + oa, kBlock, &sm.raw_full[s]);
-      if (pair) bulk_load(sm.raw[s] + kBlock, a.cache.k + ob, kBlock, &sm.raw_full[s]);
-      bulk_load(sm.raw[s] + 2 * kBlock, a.cache.v + oa, kBlock, &sm.raw_full[s]);
-      if (pair) bulk_load(sm.raw[s] + 3 * kBlock, a.cache.v + ob, kBlock, &sm.raw_full[s]);
-      sm.scales[j % kRing] = make_float4(ka, kb, a.cache.v_scale[sa], a.cache.v_scale[sb]);
-    };
-    // two of a block's 256 chunks of 16 codes a thread, of both blocks; a second block that a step does not have is what was there before
-    auto convert = [&](uint8_t* dst, const uint8_t* src) {
-      const uint4* w = reinterpret_cast<const uint4*>(src) + p;
-      const uint4 w0 = w[0], w1 = w[128], w2 = w[256], w3 = w[384];
-      put_codes<INT8>(dst, p >> 2, p & 3, w0);
-      put_codes<INT8>(dst, (p >> 2) + 32, p & 3, w1);
-      put_codes<INT8>(dst + kHalfTile, p >> 2, p & 3, w2);
-      put_codes<INT8>(dst + kHalfTile, (p >> 2) + 32, p & 3, w3);
-    };
-    int asked = 0;
-    if (p == 0) {
-      for (; asked < min(kRaw, n_steps); ++asked) {
-        look(asked);
-        request(asked);
-      }
-      if (asked < n_steps) look(asked);
+    // A slot that two warps filled in turn would need an order between them: one of them ahead by two rounds reads the parity of the
+    // round before last as the last one's.
+    static_assert(kRaw % 4 == 0 && kStages % 4 == 0, "a warp's blocks keep to its own slots");
+    int page = 0;
+    if (lane == 0) {
+      for (int j = first; j < min(kRaw, n_blocks); j += 4) request(j, __ldg(table + j));
+      if (first + kRaw < n_blocks) page = __ldg(table + first + kRaw);
     }
-    for (int j = 0; j < n_steps; ++j) {
+    // 256 chunks of 16 codes, eight a lane
+    auto convert = [&](uint8_t* dst, const uint8_t* src) {
+      const uint4* w = reinterpret_cast<const uint4*>(src) + lane;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 in[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) in[i] = w[128 * h + 32 * i];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_codes<INT8>(dst, 32 * h + 8 * i + (lane >> 2), lane & 3, in[i]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    int j = first;
+    for (; j < n_blocks; j += 4) {
       const int s = j % kStages, rs = j % kRaw;
+      const uint32_t before = ((j / kStages) & 1) ^ 1;
       if (!wait(&sm.raw_full[rs], (j / kRaw) & 1, 322)) break;
-      if (!wait(&sm.k_empty[s], ((j / kStages) & 1) ^ 1, 317)) break;
+      if (!wait(&sm.k_empty[s], before, 317)) break;
       convert(sm.k[s], sm.raw[rs]);
-      fence_proxy_async_smem();
-      __syncwarp();
       if (lane == 0) mbar_arrive(&sm.k_full[s]);
-      if (!wait(&sm.v_empty[s], ((j / kStages) & 1) ^ 1, 318)) break;
-      convert(sm.v[s], sm.raw[rs] + 2 * kBlock);
-      fence_proxy_async_smem();
-      __syncwarp();
+      if (!wait(&sm.v_empty[s], before, 318)) break;
+      convert(sm.v[s], sm.raw[rs] + kBlock);
       if (lane == 0) {
         mbar_arrive(&sm.v_full[s]);
-        mbar_arrive(&sm.raw_empty[rs]);
-      }
-      if (j + kRaw < n_steps && warp == 8) {  // into the slot that this step has just left
-        if (!wait(&sm.raw_empty[rs], (j / kRaw) & 1, 323)) break;
-        if (p == 0) {
-          request(asked++);
-          if (asked < n_steps) look(asked);
+        if (j + kRaw < n_blocks) {  // into the slot that this block has just left
+          request(j + kRaw, page);
+          if (j + kRaw + 4 < n_blocks) page = __ldg(table + j + kRaw + 4);
         }
-        __syncwarp();
       }
+      __syncwarp();
     }
-    if (p == 0 && *ab.cta_flag) {  // gave up: copies in flight land before the CTA ends
+    if (lane == 0 && j < n_blocks) {  // gave up: copies in flight land before the CTA ends
       const long long t0 = clock64();
-      for (int j = max(0, asked - kRaw); j < asked; ++j)
-        while (!mbar_try_wait(&sm.raw_full[j % kRaw], (j / kRaw) & 1) && clock64() - t0 < kWaitCycles) {
+      for (int k = j; k < min(j + kRaw, n_blocks); k += 4)
+        while (!mbar_try_wait(&sm.raw_full[k % kRaw], (k / kRaw) & 1) && clock64() - t0 < kWaitCycles) {
         }
     }
     __syncwarp();
@@ -338,100 +311,93 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     // ---------------------------------------------------------------- softmax
     reg_alloc<kRegsSoftmax>();
     const int x = warp >> 2, r = tid & 127;
-    const int row = row0 + (two ? x * 128 : 0) + r;
+    const int row = row0 + (two ? (x >> 1) * 128 : 0) + r;
     const int row_c = min(row, row0 + here - 1);  // rows behind the last one do as it does and are not stored
-    const int lim = sr.limit(a, row_c);
-    const bool live = row0 + (two ? x * 128 : 0) + (r & ~31) < row0 + here;  // the warp has a row
+    const int lim = sr.limit(a, row_c) - j0 * 64;   // keys that it sees, from this CTA's first on
+    const bool live = row - lane < row0 + here;   // the warp has a row
     const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
-    const int steps = steps_of(x);
-    // ---- the query row, as halves
+    // ---- the query row, as halves.  The streams of a row tile share its operand tile: with four of them each writes two of the row's
+    // eight chunks, with two each four.
     float unit;
     {
       const uint4* src = reinterpret_cast<const uint4*>(sr.query(a, head, row_c));
-      uint32_t w[32];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint4 t = __ldg(src + i);
-        w[4 * i] = t.x;
-        w[4 * i + 1] = t.y;
-        w[4 * i + 2] = t.z;
-        w[4 * i + 3] = t.w;
-      }
       // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
       const float sign = a.scale_log2 > 0.f ? 1.f : a.scale_log2 < 0.f ? -1.f : 0.f;
       int up = 0;
       if constexpr (BF16) {
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = max(top, max((w[i] << 16) & 0x7fffffffu, w[i] & 0x7fff0000u));
+        for (int i = 0; i < 8; ++i) {
+          const uint4 t = __ldg(src + i);
+          const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
+        }
         up = kv::query_shift(top);
       }
       const float f = kv::pow2(up) * sign;
+      uint8_t* at = sm.q[two ? x >> 1 : 0] + r * 128;
+      const int chunks = two ? 4 : 2, c0 = first_of(x) * chunks;
+      for (int i = c0; i < c0 + chunks; ++i) {
+        const uint4 t = __ldg(src + i);
+        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+        uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const float2 t = kv::unpack16<BF16>(w[i]);
-        w[i] = kv::pack16<false>(t.x * f, t.y * f);
+        for (int k = 0; k < 4; ++k) {
+          const float2 v = kv::unpack16<BF16>(w[k]);
+          h[k] = kv::pack16<false>(v.x * f, v.y * f);
+        }
+        *reinterpret_cast<uint4*>(at + ((i ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
       }
-      uint8_t* at = sm.q[x] + r * 128;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        *reinterpret_cast<uint4*>(at + ((i ^ (r & 7)) << 4)) = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.q_full[x]);
+      if (lane == 0) mbar_arrive(&sm.q_full[two ? x >> 1 : 0]);
       unit = kv::pow2(-up) * (sign == 0.f ? 1.f : fabsf(a.scale_log2)) * C::kUnit;
     }
     // ---- the largest value scale of the keys visited here
     float vref = 0.f;
-    for (int b = 2 * j0 + tid; b < min(2 * (j0 + n_steps), n_blocks); b += 256) {
-      const int page = table[b];
-      if (page >= 0 && page < a.cache.blocks) vref = fmaxf(vref, a.cache.v_scale[page * slots + head]);
+    for (int b = tid; b < n_blocks; b += kSoftmaxThreads) {
+      const int page = __ldg(table + b);
+      if (page >= 0 && page < a.cache.blocks) vref = fmaxf(vref, a.cache.v_scale[static_cast<int64_t>(page) * a.cache.heads + head]);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
     if (lane == 0) sm.vmax[warp] = vref;
     softmax_barrier();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) vref = fmaxf(vref, sm.vmax[i]);
+    for (int i = 0; i < kSoftmaxThreads / 32; ++i) vref = fmaxf(vref, sm.vmax[i]);
     if (!(vref > 0.f)) vref = 1.f;
     const float inv_vref = 1.f / vref;
 
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + lanes + kColS + x * 128, to = tmem + lanes + kColO + x * 64, tp = tmem + lanes + kColP + x * 64;
+    const uint32_t ts = tmem + lanes + kColS + x * 64, to = tmem + lanes + kColO + x * 64;
     float m_ref = -INFINITY, l = 0.f;
-    bool pzero0 = false, pzero1 = false;
     bool ok = true;
-    for (int c = 0; c < steps; ++c) {
-      const int j = two ? c : 2 * c + x;
-      const int key0 = (j0 + j) * 128;
-      const bool pair = 2 * (j0 + j) + 1 < n_blocks;
-      if (!wait(&sm.s_full[x], c & 1, 319)) { ok = false; break; }
+    uint32_t c = 0;
+    const int end = end_of(x);
+    for (int j = first_of(x); j < end; j += stride, ++c) {
+      const int key0 = j * 64;
+      // the scores, and with them: the product of the step before is done, the output tile at rest
+      ok = wait(&sm.s_full[x], c & 1, 319);
+      if (!ok) break;
       tc_fence_after_sync();
-      const float4 sc = sm.scales[j % kRing];
-      const bool act0 = live && key0 < wmax && sc.x >= 0.f, act1 = live && pair && key0 + 64 < wmax && sc.y >= 0.f;
-      uint32_t s[128];
+      const float2 sc = sm.scales[j % kRing];
+      const bool act = live && key0 < wmax && sc.x >= 0.f;
+      uint32_t s[64];
       tmem_ld32(ts, s);
       tmem_ld32(ts + 32, s + 32);
-      tmem_ld32(ts + 64, s + 64);
-      tmem_ld32(ts + 96, s + 96);
       tc_wait_ld();
-      tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.s_free[x]);
-
-      if (key0 + 128 > wmin) {  // keys that some row of the warp does not see
-        const int left = lim - key0;
+      if (act) {
+        if (key0 + 64 > wmin) {  // keys that some row of the warp does not see
+          const int left = lim - key0;
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i >= left) s[i] = 0xff800000u;
-      }
-      // at least the smallest normal number: -inf * 0 would be NaN
-      const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f), c1 = fmaxf(unit * sc.y, 1.17549435e-38f);
-      float alpha = 1.f;
-      bool fix = false;
-      if (act0 || act1) {
-        float m_new = act0 ? max64(s) * c0 : -INFINITY;
-        if (act1) m_new = fmaxf(m_new, max64(s + 64) * c1);
+          for (int i = 0; i < 64; ++i)
+            if (i >= left) s[i] = 0xff800000u;
+        }
+        const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
+        const float m_new = max64(s) * c0;
+        float alpha = 1.f;
+        bool fix = false;
         if (m_ref == -INFINITY) {
           m_ref = m_new;
         } else if (m_new > m_ref + kRescaleThreshold) {
@@ -439,168 +405,159 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           m_ref = m_new;
           fix = true;
         }
-      }
-      const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-      const float e0 = __log2f(fmaxf(sc.z * inv_vref, 8.7e-19f)) + kShift, e1 = __log2f(fmaxf(sc.w * inv_vref, 8.7e-19f)) + kShift;
-      uint32_t p[32];
-      l *= alpha;
-      if (act0) l = fmaf(exp64<false>(s, p, c0, ref - e0), ex2(-e0), l);
-      if (c > 0) {
-        if (!wait(&sm.pv_done[x], (c - 1) & 1, 320)) { ok = false; break; }
-        tc_fence_after_sync();
-      }
-      if (__any_sync(0xffffffffu, fix) && c > 0) {
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        const float e0 = __log2f(fmaxf(sc.y * inv_vref, 8.7e-19f)) + kShift;
+        l *= alpha;
+        if (__any_sync(0xffffffffu, fix) && c > 0) {
 #pragma unroll 1
-        for (int i = 0; i < 64; i += 16) {
-          uint32_t o[16];
-          tmem_ld16(to + i, o);
-          tc_wait_ld();
+          for (int i = 0; i < 64; i += 16) {
+            uint32_t o[16];
+            tmem_ld16(to + i, o);
+            tc_wait_ld();
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-          tmem_st16(to + i, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st16(to + i, o);
+          }
         }
-      }
-      if (act0) {
-        tmem_st32(tp, p);
-        pzero0 = false;
-      } else if (!pzero0) {
+        // half a row at a time: the registers hold 64 scores and 32 packed probabilities at once no more than barely
+        const float back = ex2(-e0);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) p[i] = 0u;
-        tmem_st32(tp, p);
-        pzero0 = true;
+        for (int h = 0; h < 2; ++h) {
+          uint32_t p[16];
+          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref - e0), back, l);
+          tmem_st16(ts + 16 * h, p);
+        }
+      } else {
+        uint32_t p[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) p[i] = 0u;
+        tmem_st16(ts, p);
+        tmem_st16(ts + 16, p);
       }
       tc_wait_st();
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.p_full[x][0]);
-      if (pair) {
-        if (act1) {
-          l = fmaf(exp64<false>(s + 64, p, c1, ref - e1), ex2(-e1), l);
-          tmem_st32(tp + 32, p);
-          pzero1 = false;
-        } else if (!pzero1) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) p[i] = 0u;
-          tmem_st32(tp + 32, p);
-          pzero1 = true;
-        }
-        tc_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-      }
-      if (lane == 0) mbar_arrive(&sm.p_full[x][1]);
+      if (lane == 0) mbar_arrive(&sm.p_full[x]);
     }
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok && steps > 0) {
-      ok = wait(&sm.pv_done[x], (steps - 1) & 1, 321);
-      ok = __all_sync(0xffffffffu, ok);
+    if (ok && c > 0) {
+      ok = wait(&sm.o_full[x], (c - 1) & 1, 321);
       tc_fence_after_sync();
     }
-    const bool any = ok && steps > 0 && live;  // there is an output tile to read; the same for the whole warp
-    const float unit_o = vref * C::kUnit * 0.0078125f;  // 2^-kShift
-    if (!combine) {
-      if (any) {  // warp-uniform: TMEM loads are for whole warps
-        const float inv = lim > 0 ? unit_o / l : 0.f;
-        uint16_t* dst = sr.output(a, head, row_c);
+    const bool any = ok && c > 0 && live;  // there is an output tile to read; the same for the whole warp
+    softmax_barrier();  // all streams have seen their last block: operand tiles and ring are free
+    {
+      float* part = reinterpret_cast<float*>(sm.k) + x * 128 * 64 + r * 64;
+      sm.ml[x][r] = make_float2(any ? m_ref : -INFINITY, any ? l : 0.f);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t o[32];
+      for (int h = 0; h < 2; ++h) {
+        uint32_t o[32];
+        if (any) {
           tmem_ld32(to + 32 * h, o);
-          tc_wait_ld();
-          if (row < row0 + here) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float lo = __uint_as_float(o[8 * q + 2 * e]), hi = __uint_as_float(o[8 * q + 2 * e + 1]);
-                w[e] = lim > 0 ? pack2<BF16>(lo * inv, hi * inv) : 0u;
-              }
-              *reinterpret_cast<uint4*>(dst + 32 * h + 8 * q) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          }
-        }
-      } else if (row < row0 + here) {  // no key at all
-#pragma unroll
-        for (int q = 0; q < 8; ++q) *reinterpret_cast<uint4*>(sr.output(a, head, row) + 8 * q) = make_uint4(0, 0, 0, 0);
-      }
-    } else {
-      softmax_barrier();  // both streams have seen the last step: its codes have been converted, the ring is free
-      float* part = reinterpret_cast<float*>(sm.raw) + x * 128 * 64 + r * 64;
-      sm.ml[x][r] = make_float2(any && lim > 0 ? m_ref : -INFINITY, any && m_ref != -INFINITY ? l : 0.f);
-      const bool keep = any;
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        uint32_t o[16];
-        if (keep) {
-          tmem_ld16(to + 16 * h, o);
           tc_wait_ld();
         } else {
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0u;
+          for (int k = 0; k < 32; ++k) o[k] = 0u;
         }
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float4 f = make_float4(__uint_as_float(o[4 * q]) * unit_o, __uint_as_float(o[4 * q + 1]) * unit_o,
-                                       __uint_as_float(o[4 * q + 2]) * unit_o, __uint_as_float(o[4 * q + 3]) * unit_o);
-          *reinterpret_cast<float4*>(part + (((4 * h + q) ^ (r & 15)) << 2)) = f;
+        for (int q = 0; q < 8; ++q)
+          *reinterpret_cast<uint4*>(part + (((8 * h + q) ^ (r & 15)) << 2)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+      }
+    }
+    softmax_barrier();
+    // ---- the streams of this CTA: a weight for each row and stream, then four dimensions of a row a thread
+    const int streams = two ? 2 : 4;
+    if (tid < here) {
+      const int x0 = two ? (tid >> 7) * 2 : 0, pr = tid & 127;
+      float M = -INFINITY, L = 0.f;
+      for (int y = 0; y < streams; ++y) M = max_nan(M, sm.ml[x0 + y][pr].x);
+      float f[kStreams];
+#pragma unroll
+      for (int y = 0; y < kStreams; ++y) {
+        if (y >= streams) continue;
+        const float2 ml = sm.ml[x0 + y][pr];
+        f[y] = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        L = fmaf(ml.y, f[y], L);
+      }
+      const float unit_o = vref * C::kUnit * 0.0078125f;  // 2^-kShift
+      const float w = a.splits > 1 ? unit_o : M == -INFINITY ? 0.f : unit_o / L;
+#pragma unroll
+      for (int y = 0; y < kStreams; ++y)
+        if (y < streams) sm.weight[x0 + y][pr] = f[y] * w;
+      if (a.splits > 1) sm.ml_cta[tid] = make_float2(M, L);
+    }
+    softmax_barrier();
+    auto store = [&](int rr, int d, const float4& v) {
+      *reinterpret_cast<uint2*>(sr.output(a, head, row0 + rr) + d) = make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
+    };
+    auto merge = [&](auto count) {
+      constexpr int N = decltype(count)::value;
+#pragma unroll 2
+      for (int i = tid; i < here * 16; i += kSoftmaxThreads) {
+        const int rr = i >> 4, quad = i & 15, x0 = N == 2 ? (rr >> 7) * 2 : 0, pr = rr & 127;
+        float* at = reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2);
+        float4 v = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int y = 0; y < N; ++y) {
+          const float w = sm.weight[x0 + y][pr];
+          const float4 o = *reinterpret_cast<const float4*>(at + y * 128 * 64);
+          v.x = fmaf(o.x, w, v.x);
+          v.y = fmaf(o.y, w, v.y);
+          v.z = fmaf(o.z, w, v.z);
+          v.w = fmaf(o.w, w, v.w);
         }
+        if (a.splits == 1) store(rr, 4 * quad, v);
+        else *reinterpret_cast<float4*>(at) = v;
       }
-      if (a.splits > 1) {
-        __syncwarp();
-        cluster_arrive();
-        cluster_wait();
-      } else {
-        softmax_barrier();
-      }
-      // a quarter of a row (16 dimensions) a thread, over all threads of the cluster
-      for (int i = rank * 256 + tid; i < here * 4; i += a.splits * 256) {
-        const int rr = i >> 2, quarter = i & 3;
-        const int x0 = two ? rr >> 7 : 0, xs = two ? 1 : 2, pr = rr & 127;
-        const uint32_t ml_at = smem_u32(&sm.ml[x0][pr]), o_at = smem_u32(reinterpret_cast<float*>(sm.raw) + (x0 * 128 + pr) * 64);
+    };
+    if (two) merge(std::integral_constant<int, 2>());
+    else merge(std::integral_constant<int, 4>());
+    // ... then the CTAs of the cluster, each of which finishes its share of the tile; all parts are requested before one is used
+    if (a.splits > 1) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      for (int i = rank * kSoftmaxThreads + tid; i < here * 16; i += a.splits * kSoftmaxThreads) {
+        const int rr = i >> 4, quad = i & 15, x0 = two ? (rr >> 7) * 2 : 0, pr = rr & 127;
+        const uint32_t ml_at = smem_u32(&sm.ml_cta[rr]);
+        const uint32_t o_at = smem_u32(reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2));
+        float2 ml[kMaxSplits];
+        float4 o[kMaxSplits];
+#pragma unroll
+        for (int w = 0; w < kMaxSplits; ++w) {
+          ml[w] = make_float2(-INFINITY, 0.f);
+          o[w] = make_float4(0, 0, 0, 0);
+          if (w < a.splits) {
+            ml[w] = kv::ld_cluster_f2(kv::peer_address(ml_at, w));
+            o[w] = kv::ld_cluster_f4(kv::peer_address(o_at, w));
+          }
+        }
         float M = -INFINITY, L = 0.f;
-        for (int w = 0; w < a.splits; ++w)
-          for (int y = 0; y < xs; ++y) M = max_nan(M, kv::ld_cluster_f2(kv::peer_address(ml_at + y * 1024, w)).x);
-        float acc[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) acc[k] = 0.f;
-        if (M != -INFINITY) {
-          for (int w = 0; w < a.splits; ++w)
-            for (int y = 0; y < xs; ++y) {
-              const float2 ml = kv::ld_cluster_f2(kv::peer_address(ml_at + y * 1024, w));
-              if (ml.x == -INFINITY) continue;
-              const float f = ex2(ml.x - M);
-              L = fmaf(ml.y, f, L);
-              const uint32_t at = kv::peer_address(o_at + y * 32768, w);
+        for (int w = 0; w < kMaxSplits; ++w) M = max_nan(M, ml[w].x);
+        float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float4 v = kv::ld_cluster_f4(at + (((4 * quarter + q) ^ (pr & 15)) << 4));
-                acc[4 * q] = fmaf(v.x, f, acc[4 * q]);
-                acc[4 * q + 1] = fmaf(v.y, f, acc[4 * q + 1]);
-                acc[4 * q + 2] = fmaf(v.z, f, acc[4 * q + 2]);
-                acc[4 * q + 3] = fmaf(v.w, f, acc[4 * q + 3]);
-              }
-            }
+        for (int w = 0; w < kMaxSplits; ++w) {
+          const float f = ml[w].x == -INFINITY ? 0.f : ex2(ml[w].x - M);
+          L = fmaf(ml[w].y, f, L);
+          v.x = fmaf(o[w].x, f, v.x);
+          v.y = fmaf(o[w].y, f, v.y);
+          v.z = fmaf(o[w].z, f, v.z);
+          v.w = fmaf(o[w].w, f, v.w);
         }
-        const float inv = M != -INFINITY ? 1.f / L : 0.f;
-        uint32_t w[8];
-#pragma unroll
-        for (int k = 0; k < 8; ++k) w[k] = pack2<BF16>(acc[2 * k] * inv, acc[2 * k + 1] * inv);
-        uint4* dst = reinterpret_cast<uint4*>(sr.output(a, head, row0 + rr) + 16 * quarter);
-        dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-        dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        const float inv = M == -INFINITY ? 0.f : 1.f / L;
+        store(rr, 4 * quad, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       }
-      if (a.splits > 1) {
-        __syncwarp();
-        cluster_arrive();  // no CTA leaves while another one reads its shared memory
-        cluster_wait();
-      }
+    }
+    if (a.splits > 1) {
+      __syncwarp();
+      cluster_arrive();  // no CTA leaves while another one reads its shared memory
+      cluster_wait();
     }
   }
 
   tc_fence_before_sync();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 20) {
     tc_fence_after_sync();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -608,7 +565,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
 
 }  // namespace
 
-rt_status launch_cached_attention_many_rows(const Args& a, bool bf16, bool int8, cudaStream_t st) {
+rt_status launch_cached_attention_many_rows(const Args& args, bool bf16, bool int8, cudaStream_t st) {
+  Args a = args;
+  a.sorted = a.n_seq * a.tiles > 1 && a.n_seq * a.tiles <= kThreads;
   auto kern = bf16 ? (int8 ? many_rows_kernel<true, true> : many_rows_kernel<true, false>)
                    : (int8 ? many_rows_kernel<false, true> : many_rows_kernel<false, false>);
   RT_TRY(ensure_kernel_smem(reinterpret_cast<const void*>(kern), sizeof(Smem), true));

@@ -89,21 +89,21 @@ __device__ __forceinline__ void ex2_fma_pair(float x0, float x1, float& r0, floa
   r1 = __int_as_float(__float_as_int(a1) + (__float_as_int(b1) << 23));
 }
 
-// p[i] = 2^(s[2i] * c - m), 2^(s[2i+1] * c - m) packed to 16 bits, for 64 scores; returns their sum.
-// Every kPolyEvery-th pair is computed on the FMA pipe.
+// p[i] = 2^(s[2i] * c - m), 2^(s[2i+1] * c - m) packed to 16 bits, for N scores; returns their sum.
+// Every EVERY-th pair is computed on the FMA pipe.
 constexpr int kPolyEvery = 4;  // measured: 3 and 4 are equal within noise, 2 is slower (issue slots)
-template <bool BF16>
-__device__ __forceinline__ float exp64(const uint32_t* s, uint32_t* p, float scale_log2, float m_ref) {
+template <bool BF16, int N, int EVERY = kPolyEvery>
+__device__ __forceinline__ float exp_columns(const uint32_t* s, uint32_t* p, float scale_log2, float m_ref) {
   const unsigned long long c2 = f2_pack(scale_log2, scale_log2);
   const unsigned long long nm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = 0ull, acc1 = 0ull;  // two packed partial sums (+0.0f, +0.0f)
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < N / 2; ++i) {
     const unsigned long long t = f2_fma(f2_pack(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), c2, nm2);
     float t0, t1;
     f2_unpack(t, t0, t1);
     float p0, p1;
-    if (kPolyEvery > 0 && i % kPolyEvery == kPolyEvery - 1) {
+    if (i % EVERY == EVERY - 1) {
       ex2_fma_pair(t0, t1, p0, p1);
     } else {
       p0 = ex2(t0);
@@ -116,6 +116,10 @@ __device__ __forceinline__ float exp64(const uint32_t* s, uint32_t* p, float sca
   float s0, s1;
   f2_unpack(f2_add(acc0, acc1), s0, s1);
   return s0 + s1;
+}
+template <bool BF16>
+__device__ __forceinline__ float exp64(const uint32_t* s, uint32_t* p, float scale_log2, float m_ref) {
+  return exp_columns<BF16, 64>(s, p, scale_log2, m_ref);
 }
 
 // setmaxnreg: executed by all four warps of a warpgroup at one place.
