@@ -4,7 +4,7 @@
 
 Output: raptor_t_b200/lib/libraptor_b200.so - the C-ABI library - and
 raptor_t_b200/lib/raptor_t.so - the pybind11 module `raptor_t` with the reference's operator
-classes on top of it (both git-ignored).  nvcc cross-compiles without a GPU, so this also
+classes on top of it - and raptor_t_b200/lib/raptor_ops.so - the short calls of ops.py (all git-ignored).  nvcc cross-compiles without a GPU, so this also
 works on a CPU-only build machine.
 """
 import contextlib
@@ -62,40 +62,52 @@ def _build_lock():
 
 SHIM = os.path.join(LIB_DIR, "raptor_t.so")
 SHIM_SRC = os.path.join(CSRC, "pybind_shim.cpp")
+OPS_SHIM = os.path.join(LIB_DIR, "raptor_ops.so")
+OPS_SHIM_SRC = os.path.join(CSRC, "ops_shim.cpp")
 
 
 def build_shim(force=False):
     """Compile the pybind11 module `raptor_t` (csrc/pybind_shim.cpp) against torch's headers and
     link it to libraptor_b200.so; returns its path."""
+    return _build_module(SHIM_SRC, SHIM, LIB, force)
+
+
+def build_ops(force=False):
+    """The pybind11 module `raptor_ops` (csrc/ops_shim.cpp) that ops.py makes its short calls through; returns its path.
+    It takes the library's entry points at run time and is not linked to it."""
+    return _build_module(OPS_SHIM_SRC, OPS_SHIM, None, force)
+
+
+def _build_module(src, out, lib, force):
     def fresh():
-        return os.path.exists(SHIM) and os.path.getmtime(SHIM) >= max(
-            os.path.getmtime(SHIM_SRC), os.path.getmtime(LIB),
-            os.path.getmtime(os.path.join(HERE, "..", "include", "raptor_b200.h")))
+        deps = [src, os.path.join(HERE, "..", "include", "raptor_b200.h")] + ([lib] if lib else [])
+        return os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps)
     if not force and fresh():
-        return SHIM
+        return out
     with _build_lock():
         if not force and fresh():
-            return SHIM
-        return _build_shim_locked()
+            return out
+        return _build_module_locked(src, out, lib)
 
 
-def _build_shim_locked():
+def _build_module_locked(src, out, lib):
     import sysconfig
 
     import torch
     tdir = os.path.dirname(torch.__file__)
     cuda_home = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else "/usr/local/cuda"
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", SHIM_SRC, "-o", SHIM, "-DTORCH_EXTENSION_NAME=raptor_t",
+    name = os.path.basename(out)[:-len(".so")]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", src, "-o", out, f"-DTORCH_EXTENSION_NAME={name}",
            "-DTORCH_API_INCLUDE_EXTENSION_H", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f"-I{tdir}/include", f"-I{tdir}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
            f"-I{cuda_home}/include", f"-L{tdir}/lib", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-lc10", "-lc10_cuda",
-           "-ltorch_cuda", f"-L{cuda_home}/lib64", "-lcudart", f"-L{LIB_DIR}", "-lraptor_b200", "-Wl,-rpath,$ORIGIN",
-           f"-Wl,-rpath,{tdir}/lib"]
+           "-ltorch_cuda", f"-L{cuda_home}/lib64", "-lcudart"]
+    cmd += ([f"-L{LIB_DIR}", "-lraptor_b200"] if lib else []) + ["-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tdir}/lib"]
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if r.returncode != 0:
         sys.stderr.write(r.stdout)
-        raise RuntimeError("raptor_t_b200: building the pybind11 module failed")
-    return SHIM
+        raise RuntimeError(f"raptor_t_b200: building the pybind11 module {name} failed")
+    return out
 
 
 def build(force=False, verbose=False):
@@ -135,3 +147,4 @@ def _build_locked(verbose):
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="-v" in sys.argv))
     print(build_shim(force="--force" in sys.argv))
+    print(build_ops(force="--force" in sys.argv))

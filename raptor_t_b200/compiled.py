@@ -20,3 +20,18 @@ def load():
     spec.loader.exec_module(mod)
     sys.modules["raptor_t"] = mod
     return mod
+
+
+def load_ops():
+    """Build (if stale) and import the module `raptor_ops` (csrc/ops_shim.cpp), bound to the library that capi has loaded."""
+    import ctypes
+
+    import torch  # noqa: F401
+    path = _build.build_ops()
+    spec = importlib.util.spec_from_file_location("raptor_ops", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    at = lambda name: ctypes.cast(getattr(capi.lib, name), ctypes.c_void_p).value  # noqa: E731
+    mod.bind(*[at(n) for n in ("rt_last_error", "rt_kv_cache_write", "rt_kv_cache_read", "rt_cached_attention",
+                               "rt_token_logprobs", "rt_token_logprobs_backward")])
+    return mod

@@ -56,34 +56,6 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                : "memory");
 }
 
-// Codes as operands of the products, two codes a register, to be multiplied with kUnit after kBias has been taken off.
-//   int8: the code with its sign bit flipped is an unsigned byte u = code + 128; the half with the bits u is the subnormal number
-//     u 2^-24, so a byte move does it.  128 of each code is taken off the sums: 128 sum q is the same for every key, and 128 sum p
-//     comes from the product that sums the probabilities anyway.  fp32 sums keep 2^-17 of a code that way.
-//   e4m3: the hardware's conversion.  A code that is NaN, which the writer never stores, stays NaN; the caller keeps those of places that hold no
-//     token out of P V.
-template <bool INT8>
-struct Operand;
-template <>
-struct Operand<true> {
-  static constexpr float kUnit = 16777216.f, kBias = 128.f;
-  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
-  template <int LO>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) { return kv::prmt(w, 0u, LO == 0 ? 0x4140u : 0x4342u); }
-};
-template <>
-struct Operand<false> {
-  static constexpr float kUnit = 1.f, kBias = 0.f;
-  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
-  template <int LO>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    uint32_t r;
-    if constexpr (LO == 0) asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}" : "=r"(r) : "r"(w));
-    else asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, hi;}" : "=r"(r) : "r"(w));
-    return r;
-  }
-};
-
 // 8 x 8 halves: thread (g, t) gives row g, columns 2 t and 2 t + 1, and gets them of the transposed matrix.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t r;
@@ -123,7 +95,7 @@ __device__ __forceinline__ float load_query(const uint16_t* row, int t, float si
 // not have.  Thread (g, t) = (lane / 4, lane % 4) has columns (rows of the tile) 8 n + 2 t, + 1.
 template <bool BF16, bool INT8, int NT>
 struct RowTile {
-  using C = Operand<INT8>;
+  using C = kv::Operand<INT8>;
   static constexpr int kRows = 8 * NT;
   int g, t;
   int ctx, least;         // keys of the sequence, and of those what the tile's first row sees
@@ -583,6 +555,24 @@ int splits_of(int64_t units, int tile_rows, int64_t keys) {
   return splits;
 }
 
+// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 9 us and 1.05 us a block of keys (0.56 for
+// at most 128 rows), 4 us more where a cluster joins its results.
+int many_rows_splits(int64_t units, int rows, int64_t keys, double* us) {
+  const double block = rows > 128 ? 1.05 : 0.56, blocks = static_cast<double>((keys + 63) / 64);
+  int best = 1;
+  double least = 1e30;
+  for (int splits = 1; splits <= 8; splits *= 2) {
+    const double rounds = static_cast<double>((units * splits + kSms - 1) / kSms);
+    const double cost = rounds * (9.0 + (splits > 1 ? 4.0 : 0.0) + block * blocks / splits);
+    if (cost < least) {
+      least = cost;
+      best = splits;
+    }
+  }
+  *us = least;
+  return best;
+}
+
 template <bool BF16, bool INT8, int NT>
 rt_status launch_few_rows(const Args& a, cudaStream_t st) {
   auto kern = few_rows_kernel<BF16, INT8, NT>;
@@ -648,22 +638,27 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   a.causal = causal != 0;
   RT_REQUIRE(static_cast<int64_t>(a.max_q) * a.group < (int64_t{1} << 30), RT_ERR_UNSUPPORTED, "cached_attention: too many query rows");
   const int rows = a.max_q * a.group;
-  const bool many = rows > kFewRows;
+  const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
+  RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * (rows / 8 + 1) < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
+             "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
+  const int64_t widest = static_cast<int64_t>(table_stride) * 64;
+  const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
+  // Which kernel: the one of few rows pays for every 16 rows (1.65 ns a tile and block of keys on the full chip), the one of many rows for
+  // tiles of 128 and 256.  12 x 4096 keys, 12 heads, 64 rows: 60.5 and 46 us; 16 x 2000 keys 43.7 and 54.
+  const int64_t big = heads_of_all * ((rows + 255) / 256);
+  double many_us = 0;
+  const int many_splits = many_rows_splits(big, rows, keys, &many_us);
+  const bool many = rows > kFewRows ||
+                    (rows > 48 && many_us < 5.0 + 1.65e-3 * static_cast<double>(heads_of_all * ((rows + 15) / 16)) * ((keys + 63) / 64));
   a.tile_rows = many ? 256 : rows <= 8 ? 8 : 16;
   a.tiles = (rows + a.tile_rows - 1) / a.tile_rows;
-  const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
-  RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * a.tiles < (int64_t{1} << 26), RT_ERR_UNSUPPORTED,
-             "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
+  const int64_t units = heads_of_all * a.tiles;
   a.err = device_error_word();
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "cached_attention: cannot allocate the device error word");
-  const int64_t widest = static_cast<int64_t>(table_stride) * 64, units = heads_of_all * a.tiles;
-  const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == RT_BF16, int8 = cache->format == RT_KV_INT8;
   if (many) {
-    // tiles of up to 256 rows see very different numbers of keys under the causal rule: four CTAs per SM over the call balance them
-    a.splits = 1;
-    while (a.splits < 8 && units * a.splits < 4 * kSms && keys > 512 * a.splits) a.splits *= 2;
+    a.splits = many_splits;
     return launch_cached_attention_many_rows(a, bf16, int8, st);
   }
   a.splits = splits_of(units, a.tile_rows, keys);

@@ -41,8 +41,8 @@ constexpr int kThreads = 768;
 constexpr int kSoftmaxThreads = 512;
 constexpr int kStreams = 4;
 constexpr int kMaxSplits = 8;            // CTAs of a cluster
-constexpr int kStages = 4;               // operand tiles of keys, and of values: one for each warp that fills them
-constexpr int kRaw = 8;                  // blocks of codes on their way
+constexpr int kStages = 8;               // operand tiles of keys, and of values: two for each warp that fills them
+constexpr int kRaw = 4;                  // blocks of codes on their way, one for each of these warps
 constexpr int kBlock = 4096;             // codes of a block's keys, or values
 constexpr int kRing = 32;                // scales of a block, read after its operand slots are free again
 constexpr int kTile = 64 * 128;          // 64 rows of 64 halves
@@ -60,7 +60,7 @@ struct Smem {
   uint8_t k[kStages][kTile];
   uint8_t v[kStages][kTile];
   uint8_t raw[kRaw][2 * kBlock];  // keys, values
-  uint64_t raw_full[kRaw];
+  uint64_t raw_k[kRaw], raw_v[kRaw];
   uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[kStreams], p_full[kStreams], o_full[kStreams];
   float2 scales[kRing];  // key and value scale of a block; a negative key scale: nobody sees its keys
@@ -91,9 +91,8 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 // 16 bytes of codes (16 dimensions of row `row`, chunk `c` of four) as 32 bytes of halves into a swizzled tile.
-template <bool INT8>
+template <typename C>
 __device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, const uint4& w) {
-  using C = kv::Codes<INT8>;
   const uint32_t in[4] = {w.x, w.y, w.z, w.w};
   uint32_t h[8];
 #pragma unroll
@@ -109,7 +108,8 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, const u
 
 template <bool BF16, bool INT8>
 __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
-  using C = kv::Codes<INT8>;
+  using Keys = kv::Operand<INT8>;
+  using Values = std::conditional_t<INT8, kv::Codes<true>, kv::Operand<false>>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -156,7 +156,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       mbar_init(&sm.p_full[x], 4);
       mbar_init(&sm.o_full[x], 1);
     }
-    for (int s = 0; s < kRaw; ++s) mbar_init(&sm.raw_full[s], 1);
+    for (int s = 0; s < kRaw; ++s) {
+      mbar_init(&sm.raw_k[s], 1);
+      mbar_init(&sm.raw_v[s], 1);
+    }
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&sm.k_full[s], 1);
       mbar_init(&sm.k_empty[s], two ? 2 : 1);  // the streams that take the block
@@ -242,63 +245,84 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     reg_dealloc<kRegsBring>();
     // Every fourth block a warp: a block is one chain of waits, copies and a fence, and four chains run side by side.  Lane 0 requests the
     // warp's blocks; their table entries were read a block earlier.
-    const int first = warp - 16;
-    auto request = [&](int j, int page) {
-      const int s = j % kRaw;
-      const bool bad = page < 0 || page >= a.cache.blocks;
-      if (bad) kv::index_error(a.err, kSiteCachedAttention);
-      const int64_t slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
-      mbar_arrive_expect_tx(&sm.raw_full[s], 2 * kBlock);
-      bulk_load(sm.raw[s], a.cache.k + slot * kBlock, kBlock, &sm.raw_full[s]);
-      bulk_load(sm.raw[s] + kBlock, a.cache.v + slot * kBlock, kBlock, &sm.raw_full[s]);
-      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], a.cache.v_scale[slot]);
-    };
+    const int own = warp - 16;
     // A slot that two warps filled in turn would need an order between them: one of them ahead by two rounds reads the parity of the
     // round before last as the last one's.
-    static_assert(kRaw % 4 == 0 && kStages % 4 == 0, "a warp's blocks keep to its own slots");
+    static_assert(kRaw == 4 && kStages % 4 == 0, "a warp's blocks keep to its own slots");
+    uint8_t* raw = sm.raw[own];
+    int64_t slot = 0;  // of the block that is requested next
+    auto find = [&](int page, int j) {
+      const bool bad = page < 0 || page >= a.cache.blocks;
+      if (bad) kv::index_error(a.err, kSiteCachedAttention);
+      slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
+      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], a.cache.v_scale[slot]);
+    };
+    auto request = [&](uint8_t* dst, const uint8_t* base, uint64_t* bar) {
+      mbar_arrive_expect_tx(bar, kBlock);
+      bulk_load(dst, base + slot * kBlock, kBlock, bar);
+    };
     int page = 0;
-    if (lane == 0) {
-      for (int j = first; j < min(kRaw, n_blocks); j += 4) request(j, __ldg(table + j));
-      if (first + kRaw < n_blocks) page = __ldg(table + first + kRaw);
+    if (lane == 0 && own < n_blocks) {
+      find(__ldg(table + own), own);
+      request(raw, a.cache.k, &sm.raw_k[own]);
+      request(raw + kBlock, a.cache.v, &sm.raw_v[own]);
+      if (own + 4 < n_blocks) page = __ldg(table + own + 4);
     }
-    // 256 chunks of 16 codes, eight a lane
-    auto convert = [&](uint8_t* dst, const uint8_t* src) {
+    // 256 chunks of 16 codes, eight a lane; rows from `rows` on hold no token: zeros, so that no code NaN meets a probability of 0
+    auto convert = [&](auto codes, uint8_t* dst, const uint8_t* src, int rows) {
       const uint4* w = reinterpret_cast<const uint4*>(src) + lane;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint4 in[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) in[i] = w[128 * h + 32 * i];
+        if (rows < 64) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) put_codes<INT8>(dst, 32 * h + 8 * i + (lane >> 2), lane & 3, in[i]);
+          for (int i = 0; i < 4; ++i)
+            if (32 * h + 8 * i + (lane >> 2) >= rows) in[i] = make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) put_codes<decltype(codes)>(dst, 32 * h + 8 * i + (lane >> 2), lane & 3, in[i]);
       }
       fence_proxy_async_smem();
       __syncwarp();
     };
-    int j = first;
-    for (; j < n_blocks; j += 4) {
-      const int s = j % kStages, rs = j % kRaw;
+    int j = own;
+    bool keys_done = false;
+    for (uint32_t c = 0; j < n_blocks; j += 4, ++c) {
+      const int s = j % kStages;
       const uint32_t before = ((j / kStages) & 1) ^ 1;
-      if (!wait(&sm.raw_full[rs], (j / kRaw) & 1, 322)) break;
-      if (!wait(&sm.k_empty[s], before, 317)) break;
-      convert(sm.k[s], sm.raw[rs]);
-      if (lane == 0) mbar_arrive(&sm.k_full[s]);
-      if (!wait(&sm.v_empty[s], before, 318)) break;
-      convert(sm.v[s], sm.raw[rs] + kBlock);
+      keys_done = false;
+      if (!wait(&sm.raw_k[own], c & 1, 322) || !wait(&sm.k_empty[s], before, 317)) break;
+      convert(Keys(), sm.k[s], raw, 64);
+      if (lane == 0) {
+        mbar_arrive(&sm.k_full[s]);
+        if (j + 4 < n_blocks) {
+          find(page, j + 4);
+          request(raw, a.cache.k, &sm.raw_k[own]);
+          if (j + 8 < n_blocks) page = __ldg(table + j + 8);
+        }
+      }
+      __syncwarp();
+      keys_done = true;
+      if (!wait(&sm.raw_v[own], c & 1, 324) || !wait(&sm.v_empty[s], before, 318)) break;
+      convert(Values(), sm.v[s], raw + kBlock, INT8 ? 64 : sr.ctx - (j0 + j) * 64);
       if (lane == 0) {
         mbar_arrive(&sm.v_full[s]);
-        if (j + kRaw < n_blocks) {  // into the slot that this block has just left
-          request(j + kRaw, page);
-          if (j + kRaw + 4 < n_blocks) page = __ldg(table + j + kRaw + 4);
-        }
+        if (j + 4 < n_blocks) request(raw + kBlock, a.cache.v, &sm.raw_v[own]);
       }
       __syncwarp();
     }
     if (lane == 0 && j < n_blocks) {  // gave up: copies in flight land before the CTA ends
       const long long t0 = clock64();
-      for (int k = j; k < min(j + kRaw, n_blocks); k += 4)
-        while (!mbar_try_wait(&sm.raw_full[k % kRaw], (k / kRaw) & 1) && clock64() - t0 < kWaitCycles) {
+      const uint32_t c = (j / 4) & 1;
+      auto land = [&](uint64_t* bar, uint32_t parity) {
+        while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {
         }
+      };
+      if (!keys_done) land(&sm.raw_k[own], c);
+      else if (j + 4 < n_blocks) land(&sm.raw_k[own], c ^ 1);
+      land(&sm.raw_v[own], c);
     }
     __syncwarp();
     if (a.splits > 1) {
@@ -318,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
     // ---- the query row, as halves.  The streams of a row tile share its operand tile: with four of them each writes two of the row's
     // eight chunks, with two each four.
-    float unit;
+    float unit, bias = 0.f;  // a score in base 2 is (product - bias) * unit * key scale
     {
       const uint4* src = reinterpret_cast<const uint4*>(sr.query(a, head, row_c));
       // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
@@ -336,6 +360,20 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         up = kv::query_shift(top);
       }
       const float f = kv::pow2(up) * sign;
+      if constexpr (INT8) {  // the keys' bias times the sum of the row, as the product sees it
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint4 t = __ldg(src + i);
+          const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 v = kv::unpack16<BF16>(w[k]);
+            const float2 h = kv::unpack16<false>(kv::pack16<false>(v.x * f, v.y * f));
+            bias += h.x + h.y;
+          }
+        }
+        bias *= Keys::kBias / Keys::kUnit;
+      }
       uint8_t* at = sm.q[two ? x >> 1 : 0] + r * 128;
       const int chunks = two ? 4 : 2, c0 = first_of(x) * chunks;
       for (int i = c0; i < c0 + chunks; ++i) {
@@ -352,7 +390,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[two ? x >> 1 : 0]);
-      unit = kv::pow2(-up) * (sign == 0.f ? 1.f : fabsf(a.scale_log2)) * C::kUnit;
+      unit = kv::pow2(-up) * (sign == 0.f ? 1.f : fabsf(a.scale_log2)) * Keys::kUnit;
     }
     // ---- the largest value scale of the keys visited here
     float vref = 0.f;
@@ -395,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
             if (i >= left) s[i] = 0xff800000u;
         }
         const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
-        const float m_new = max64(s) * c0;
+        const float off = bias * c0, m_new = max64(s) * c0 - off;
         float alpha = 1.f;
         bool fix = false;
         if (m_ref == -INFINITY) {
@@ -424,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[16];
-          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref - e0), back, l);
+          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref - e0 + off), back, l);
           tmem_st16(ts + 16 * h, p);
         }
       } else {
@@ -478,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         f[y] = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
         L = fmaf(ml.y, f[y], L);
       }
-      const float unit_o = vref * C::kUnit * 0.0078125f;  // 2^-kShift
+      const float unit_o = vref * Values::kUnit * 0.0078125f;  // 2^-kShift
       const float w = a.splits > 1 ? unit_o : M == -INFINITY ? 0.f : unit_o / L;
 #pragma unroll
       for (int y = 0; y < kStreams; ++y)

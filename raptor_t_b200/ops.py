@@ -193,32 +193,16 @@ def sparse_attention_static(q, k, v, cfg, lens_tokens, kv_ptr, kv_idx, scale=1.0
 
 # ---- answering from encoded documents: 8-bit key/value cache, attention over it, scores of tokens ------------------
 
-_KV_FORMATS = {torch.float8_e4m3fn: capi.RT_KV_E4M3, torch.int8: capi.RT_KV_INT8}
-_LOGIT_TYPES = {torch.float16: capi.RT_F16, torch.bfloat16: capi.RT_BF16, torch.float32: capi.RT_F32}
+_native_module = None
 
 
-def _need(cond, what):
-    if not cond:
-        raise ValueError(what)
-
-
-def _here(index):
-    """Kernels run on the current device's current stream: the tensors have to be there, too.  Returns the stream."""
-    if index < 0:
-        raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
-    if index != torch._C._cuda_getDevice():
-        raise RuntimeError(f"tensors on cuda:{index}, but the current device is cuda:{torch.cuda.current_device()}")
-    return torch._C._cuda_getCurrentRawStream(index)
-
-
-def _flat(t, name, dtype, shape, index):
-    """Address of a contiguous tensor of that type and shape on that device."""
-    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
-        return t.data_ptr()
-    if t.dtype != dtype:
-        raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
-    raise ValueError(f"{name}: expected a contiguous tensor of shape {tuple(shape)} on cuda:{index}, got {tuple(t.shape)} "
-                     f"with strides {t.stride()} on {t.device}")
+def _native():
+    """The compiled half of these calls (csrc/ops_shim.cpp): argument checks, output tensors, the call."""
+    global _native_module
+    if _native_module is None:
+        from . import compiled
+        _native_module = compiled.load_ops()
+    return _native_module
 
 
 class KvCache:
@@ -228,19 +212,9 @@ class KvCache:
     64 j .. 64 j + 63.  Sequences may share blocks that none of them writes to."""
 
     def __init__(self, k, v, k_scale, v_scale):
-        if k.dtype not in _KV_FORMATS:
-            raise TypeError(f"expected float8_e4m3fn or int8, got {k.dtype}")
-        _need(k.dim() == 4 and k.shape[2] == 64 and k.shape[3] == 64, "a cache is [blocks, kv_heads, 64, 64]")
-        if k.device.type != "cuda":
-            raise RuntimeError("raptor_t_b200 ops need CUDA tensors (there is no CPU path)")
+        self._c = _native().Cache(k, v, k_scale, v_scale)
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.blocks, self.kv_heads, self.device = k.shape[0], k.shape[1], k.device
-        two, at = k.shape[:2], k.get_device()
-        self._c = capi.RtKvCache(_flat(k, "k", k.dtype, k.shape, at), _flat(v, "v", k.dtype, k.shape, at),
-                                 _flat(k_scale, "k_scale", torch.float32, two, at),
-                                 _flat(v_scale, "v_scale", torch.float32, two, at), self.blocks, self.kv_heads,
-                                 _KV_FORMATS[k.dtype], 0)
-        self._ref, self._at, self._row = C.byref(self._c), at, (self.kv_heads, 64)
 
     @staticmethod
     def empty(blocks, kv_heads, dtype=torch.float8_e4m3fn, device="cuda"):
@@ -249,52 +223,19 @@ class KvCache:
         return KvCache(k, v, *(torch.empty(blocks, kv_heads, dtype=torch.float32, device=device) for _ in range(2)))
 
 
-def _table(block_table, lengths, first, index):
-    """The arguments that say which tokens a call is about, as addresses and sizes."""
-    n, width = lengths.shape[0], block_table.shape[-1]
-    return (_flat(block_table, "block table", torch.int32, (n, width), index), width,
-            _flat(lengths, "lengths", torch.int32, (n,), index), _flat(first, "first rows", torch.int32, (n + 1,), index), n)
-
-
 def kv_cache_write(cache, k, v, block_table, start, first, max_tokens=None, head_major=False):
     """Quantises new tokens into the cache (rt_kv_cache_write; the rule for the scales stands there).
     k, v [tokens, kv_heads, 64] 16-bit, rows may be strided (columns of a projection); head_major: the buffers of
     gemm_qkv / qkv_bias_transpose instead, [tokens, kv_heads * 64] storage.  Sequence s writes rows first[s] .. first[s + 1] - 1 to
     its positions from start[s] on (int32 device tensors).  max_tokens: the most new tokens of one sequence (default: all rows)."""
-    at = cache._at
-    st = _here(at)
-    dt, tokens = _dt(k), k.shape[0]
-    if head_major:
-        shape = (tokens, cache.kv_heads * 64)
-        kp, vp, ts, hs = _flat(k, "k", k.dtype, shape, at), _flat(v, "v", k.dtype, shape, at), 0, 0
-    else:
-        strides = k.stride()
-        if not (len(strides) == 3 and strides[2] == 1 and v.stride() == strides and k.shape == v.shape == (tokens, *cache._row) and
-                v.dtype is k.dtype and k.get_device() == v.get_device() == at):
-            raise ValueError("k and v: expected [tokens, kv_heads, 64] of the same type and strides, on the cache's device")
-        kp, vp, ts, hs = k.data_ptr(), v.data_ptr(), strides[0], strides[1]
-        if ts == 0:
-            _need(tokens <= 1, "k and v: rows without a stride")
-            ts = 64 * cache.kv_heads
-    tp, width, sp, fp, n = _table(block_table, start, first, at)
-    check(lib.rt_kv_cache_write(cache._ref, kp, vp, ts, hs, tp, width, sp, fp, n, tokens, tokens if max_tokens is None else max_tokens,
-                                dt, st))
+    _native().kv_cache_write(cache._c, k, v, block_table, start, first, -1 if max_tokens is None else max_tokens, head_major)
 
 
 def kv_cache_read(cache, block_table, start, first, tokens, dtype, max_tokens=None, out=None):
     """Values of the positions from start[s] on, in 16 bits: (k, v), each [tokens, kv_heads, 64]; sequence s fills rows
     first[s] .. first[s + 1] - 1 (rt_kv_cache_read)."""
-    at = cache._at
-    st = _here(at)
-    shape = (tokens, *cache._row)
-    if out is None:
-        k = torch.empty(shape, dtype=dtype, device=cache.device)
-        out = (k, torch.empty_like(k))
-    k, v = out
-    tp, width, sp, fp, n = _table(block_table, start, first, at)
-    check(lib.rt_kv_cache_read(cache._ref, _flat(k, "k", dtype, shape, at), _flat(v, "v", dtype, shape, at), tp, width, sp, fp, n,
-                               tokens, tokens if max_tokens is None else max_tokens, _dt(k), st))
-    return out
+    k, v = (None, None) if out is None else out
+    return _native().kv_cache_read(cache._c, block_table, start, first, tokens, dtype, -1 if max_tokens is None else max_tokens, k, v)
 
 
 def cached_attention(q, cache, block_table, context, first, max_q=None, max_context=0, scale=1.0, causal=False, out=None):
@@ -302,19 +243,8 @@ def cached_attention(q, cache, block_table, context, first, max_q=None, max_cont
     [tokens, heads, 64].  Sequence s has the query rows first[s] .. first[s + 1] - 1 and context[s] cached tokens; causal: its
     rows are its last tokens, row i of n sees the first context - n + i + 1.  max_q: the most query rows of one sequence (default:
     all rows); max_context only guides how the work is split."""
-    at = cache._at
-    st = _here(at)
-    dt = _dt(q)
-    tokens, heads, dim = q.shape
-    qs, hs, ds = q.stride()
-    if not (dim == 64 and ds == 1 and (hs == 64 or heads == 1) and q.get_device() == at):
-        raise ValueError("q: expected [tokens, heads, 64] with adjacent heads, on the cache's device")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    tp, width, cp, fp, n = _table(block_table, context, first, at)
-    check(lib.rt_cached_attention(_flat(out, "out", q.dtype, q.shape, at), q.data_ptr(), qs, cache._ref, tp, width, cp, fp, n, tokens,
-                                  tokens if max_q is None else max_q, max_context, heads, scale, causal, dt, st))
-    return out
+    return _native().cached_attention(q, cache._c, block_table, context, first, -1 if max_q is None else max_q, max_context, scale, causal,
+                                      out)
 
 
 class TokenScores(NamedTuple):
@@ -327,68 +257,17 @@ class TokenScores(NamedTuple):
     top_logp: Optional[torch.Tensor]
 
 
-def _logits(z, name="logits"):
-    dt = _LOGIT_TYPES.get(z.dtype)
-    if dt is None:
-        raise TypeError(f"{name}: expected float16, bfloat16 or float32, got {z.dtype}")
-    rows, vocab = z.shape
-    pitch, step = z.stride()
-    _need(step == 1 or vocab == 1, f"{name}: expected rows of adjacent values")
-    return rows, vocab, pitch if rows > 1 else max(pitch, vocab), dt
-
-
 def token_logprobs(logits, targets=None, top_k=0):
     """Log probabilities of given tokens, entropy and the top_k (0 to 32) best alternatives of each row of logits [rows, vocab]
     (rt_token_logprobs).  targets int32 [rows], negative: no token given, its logp is 0; None: no logp."""
-    rows, vocab, pitch, dt = _logits(logits)
-    at = logits.get_device()
-    st = _here(at)
-    # empty_like and new_empty cost the host 1.3 and 1.8 us a tensor, torch.empty 2.2
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=logits.device)
-    entropy = stats.new_empty(rows)
-    tp = logp = ids = best = lp = ip = bp = None
-    if targets is not None:
-        tp, logp = _flat(targets, "targets", torch.int32, (rows,), at), torch.empty_like(entropy)
-        lp = logp.data_ptr()
-    if top_k > 0:
-        best = stats.new_empty((rows, top_k))
-        ids = torch.empty_like(best, dtype=torch.int32)
-        ip, bp = ids.data_ptr(), best.data_ptr()
-    check(lib.rt_token_logprobs(logits.data_ptr(), pitch, tp, rows, vocab, top_k, lp, entropy.data_ptr(), stats.data_ptr(), ip, bp, dt, st))
-    return TokenScores(logp, entropy, stats, ids, best)
+    return TokenScores._make(_native().token_logprobs(logits, targets, top_k))
 
 
 def token_logprobs_backward(logits, targets, stats, entropy=None, grad_logp=None, grad_entropy=None, top_ids=None, grad_top=None,
                             out=None):
     """Gradient of token_logprobs' logp, entropy and top_logp with respect to the logits (rt_token_logprobs_backward), in their type.
     grad_logp, grad_entropy fp32 [rows], grad_top fp32 [rows, k] for top_ids; None: no such term.  out may be the logits."""
-    rows, vocab, pitch, dt = _logits(logits)
-    at = logits.get_device()
-    st = _here(at)
-    if out is None:
-        # the logits' own row pitch: rows then have the same alignment
-        out = torch.empty((rows, pitch), dtype=logits.dtype, device=logits.device)
-        if pitch != vocab:
-            out = out[:, :vocab]
-    if out.shape != logits.shape or out.get_device() != at:
-        raise ValueError("out: expected the logits' shape and device")
-    if out.dtype != logits.dtype:
-        raise TypeError(f"out: expected {logits.dtype}, got {out.dtype}")
-    out_pitch = _logits(out, "out")[2]
-    f = lambda t, name, shape: None if t is None else _flat(t, name, torch.float32, shape, at)  # noqa: E731
-    top, ip = 0, None
-    if grad_top is not None and grad_top.shape[1] > 0:
-        top = grad_top.shape[1]
-        _need(top_ids is not None, "grad_top needs top_ids")
-        ip = _flat(top_ids, "top_ids", torch.int32, (rows, top), at)
-    _need(grad_logp is None or targets is not None, "grad_logp needs the targets")
-    _need(grad_entropy is None or entropy is not None, "grad_entropy needs the entropy")
-    row = (rows,)
-    check(lib.rt_token_logprobs_backward(
-        out.data_ptr(), out_pitch, logits.data_ptr(), pitch, None if targets is None else _flat(targets, "targets", torch.int32, row, at),
-        f(stats, "stats", (rows, 2)), f(entropy, "entropy", row), rows, vocab, f(grad_logp, "grad_logp", row),
-        f(grad_entropy, "grad_entropy", row), top, ip, f(grad_top, "grad_top", (rows, top)), dt, st))
-    return out
+    return _native().token_logprobs_backward(logits, targets, stats, entropy, grad_logp, grad_entropy, top_ids, grad_top, out)
 
 
 def check_device():
