@@ -365,17 +365,17 @@ struct Feed {
       bulk_load(ring->codes[s], base + at * kBlock, kBlock, &full[s]);
     }
   }
-  __device__ __forceinline__ void begin() {
+  // entries: of the list's first blocks, as far as there are any
+  __device__ __forceinline__ void begin(const int* entries) {
     static_assert(kSlots == 3, "keys and values of the first block, keys of the second");
-    const int p0 = look(0), p1 = count > 1 ? look(1) : 0;
-    const int64_t at = resolve(p0, &ks[0], &vs[0]);
+    const int64_t at = resolve(entries[0], &ks[0], &vs[0]);
     request(0, a.cache.k, at);
     request(1, a.cache.v, at);
     if (count > 1) {
-      next = resolve(p1, &ks[1], &vs[1]);
+      next = resolve(entries[1], &ks[1], &vs[1]);
       request(2, a.cache.k, next);
     }
-    if (count > 2) later = look(2);
+    later = entries[2];
   }
   // The next piece, once it is there; nullptr: gave up, with the pieces on their way landed.
   __device__ __forceinline__ const uint8_t* wait(const ptx::AbortCtx& ab) {
@@ -421,8 +421,9 @@ struct Feed {
 
 struct Smem {
   Ring ring[kWarps];  // afterwards the first 4 KB of a warp's ring are its output, fp32 [16][64]
-  float sum[16][64];  // of the CTA
-  float2 sum_ml[16];
+  // of the cluster's CTAs, written by them: quads of the output that this CTA finishes, and {m, l} of all rows
+  float4 part[16 * 16];
+  float2 part_ml[kMaxSplits][16];
   float2 ml[kWarps][16];
   uint64_t full[kWarps][kSlots];
   int cost[kWarps * 32 + 1];
@@ -448,15 +449,20 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
     seq = index_by_cost(sm.cost, a.n_seq, tid < a.n_seq ? a.context[tid] : 0, seq);
   }
 
+  // the warp's first table entries, before it is known how many of them there are
+  const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
+  const int step = a.splits * kWarps, b0 = rank * kWarps + warp;  // this warp's blocks: every step-th one
+  int entry[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) entry[i] = b0 + i * step < a.table_stride ? __ldg(table + b0 + i * step) : -1;
   const CachedRows sr(a, seq);
   if (!sr.ok) return;
   using Tile = RowTile<BF16, INT8, NT>;
   const int row0 = tile * Tile::kRows;
   if (row0 >= sr.rows) return;
   const int valid = min(Tile::kRows, sr.rows - row0);
-  const int n_blocks = (sr.limit(a, row0 + valid - 1) + 63) / 64, step = a.splits * kWarps;
-  const int32_t* table = a.table + static_cast<int64_t>(seq) * a.table_stride;
-  const int b0 = rank * kWarps + warp;  // this warp's blocks: every step-th one
+  if (a.splits > 1) ptx::cluster_arrive();  // waited for before another CTA's shared memory is written
+  const int n_blocks = (sr.limit(a, row0 + valid - 1) + 63) / 64;
   if (threadIdx.x == 0) {
     for (int w = 0; w < kWarps; ++w)
       for (int s = 0; s < kSlots; ++s) ptx::mbar_init(&sm.full[w][s], 1);
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
   const int count = b0 < n_blocks ? (n_blocks - b0 + step - 1) / step : 0;
   auto look = [&](int i) { return __ldg(table + b0 + i * step); };
   Feed<decltype(look)> feed(a, &sm.ring[warp], sm.full[warp], head, count, look);
-  if (count > 0) feed.begin();
+  if (count > 0) feed.begin(entry);
 
   Tile rows;
   rows.g = lane >> 2;
@@ -488,6 +494,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
   rows.put(out_of(warp), sm.ml[warp], valid);
   __syncthreads();
   auto store = [&](int r, int d, const float4& v, float l) { store4<BF16>(sr.output(a, head, row0 + r) + d, v, l); };
+  const int per = 256 / a.splits;  // quads that a CTA finishes at most
+  if (a.splits > 1) ptx::cluster_wait();  // the others run: their shared memory can be written
   for (int i = threadIdx.x; i < valid * 16; i += kWarps * 32) {
     const int r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
@@ -508,27 +516,27 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
     }
     if (a.splits == 1) {
       store(r, d, v, L);
-    } else {
-      *reinterpret_cast<float4*>(&sm.sum[r][d]) = v;
-      if (d == 0) sm.sum_ml[r] = make_float2(M, L);
+      continue;
     }
+    const int owner = i % a.splits;
+    kv::st_cluster_f4(kv::peer_address(ptx::smem_u32(&sm.part[rank * per + i / a.splits]), owner), v);
+    if (d == 0)
+      for (int w = 0; w < a.splits; ++w) kv::st_cluster_f2(kv::peer_address(ptx::smem_u32(&sm.part_ml[rank][r]), w), make_float2(M, L));
   }
   if (a.splits == 1) return;
-  // ---- the CTAs of the cluster: each finishes its share of the tile's quads of dimensions
+  // ---- the CTAs of the cluster: each finishes its share of the tile's quads of dimensions, which the others have written to it
+  __syncwarp();
   ptx::cluster_arrive();
   ptx::cluster_wait();
-  for (int i = rank + a.splits * static_cast<int>(threadIdx.x); i < valid * 16; i += a.splits * kWarps * 32) {
-    const int r = i >> 4, d = (i & 15) * 4;
-    const uint32_t ml_at = ptx::smem_u32(&sm.sum_ml[r]), o_at = ptx::smem_u32(&sm.sum[r][d]);
+  for (int k = threadIdx.x; rank + a.splits * k < valid * 16; k += kWarps * 32) {
+    const int i = rank + a.splits * k, r = i >> 4, d = (i & 15) * 4;
     float M = -INFINITY, L = 0.f;
     float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-    for (int w = 0; w < a.splits; ++w) M = fmaxf(M, kv::ld_cluster_f2(kv::peer_address(ml_at, w)).x);
+    for (int w = 0; w < a.splits; ++w) M = fmaxf(M, sm.part_ml[w][r].x);
     const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
     for (int w = 0; w < a.splits; ++w) {
-      const float2 ml = kv::ld_cluster_f2(kv::peer_address(ml_at, w));
-      const float4 x = kv::ld_cluster_f4(kv::peer_address(o_at, w));
+      const float2 ml = sm.part_ml[w][r];
+      const float4 x = sm.part[w * per + k];
       const float f = ex2(ml.x - ref);
       L = fmaf(ml.y, f, L);
       v.x = fmaf(x.x, f, v.x);
@@ -538,8 +546,6 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
     }
     store(r, d, v, L);
   }
-  ptx::cluster_arrive();  // no CTA leaves while another one reads its shared memory
-  ptx::cluster_wait();
 }
 
 constexpr int kSms = 148;

@@ -75,28 +75,15 @@ namespace kv {
 //   int8: the code with its sign bit flipped is an unsigned byte u = code + 128; the half with the bits u is the subnormal number
 //     u 2^-24, so a byte move does it.  128 of each code is taken off the sums: 128 sum q is the same for every key, and 128 sum p
 //     comes from the product that sums the probabilities anyway.  fp32 sums keep 2^-17 of a code that way.
-//   e4m3: the hardware's conversion.  A code that is NaN, which the writer never stores, stays NaN; the caller keeps those of places that hold no
-//     token out of P V.
+//   e4m3: as everywhere (kv_cache.cuh).
 template <bool INT8>
-struct Operand;
+struct Operand : Codes<false> {};
 template <>
 struct Operand<true> {
   static constexpr float kUnit = 16777216.f, kBias = 128.f;
   static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w ^ 0x80808080u; }
   template <int LO>
   static __device__ __forceinline__ uint32_t pair(uint32_t w) { return prmt(w, 0u, LO == 0 ? 0x4140u : 0x4342u); }
-};
-template <>
-struct Operand<false> {
-  static constexpr float kUnit = 1.f, kBias = 0.f;
-  static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
-  template <int LO>
-  static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    uint32_t r;
-    if constexpr (LO == 0) asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}" : "=r"(r) : "r"(w));
-    else asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, hi;}" : "=r"(r) : "r"(w));
-    return r;
-  }
 };
 
 // 2^up that brings a row's largest magnitude (its bf16 or fp32 bits, sign removed) into [2^14, 2^15), so that the row can be
@@ -116,6 +103,12 @@ __device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
   float2 v;
   asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
+}
+__device__ __forceinline__ void st_cluster_f4(uint32_t addr, const float4& v) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+}
+__device__ __forceinline__ void st_cluster_f2(uint32_t addr, const float2& v) {
+  asm volatile("st.shared::cluster.v2.f32 [%0], {%1, %2};" ::"r"(addr), "f"(v.x), "f"(v.y) : "memory");
 }
 // The address of the same variable in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t peer_address(uint32_t addr, int rank) {

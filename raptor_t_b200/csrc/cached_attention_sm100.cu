@@ -109,7 +109,7 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, const u
 template <bool BF16, bool INT8>
 __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   using Keys = kv::Operand<INT8>;
-  using Values = std::conditional_t<INT8, kv::Codes<true>, kv::Operand<false>>;
+  using Values = kv::Codes<INT8>;  // the sum of the rounded probabilities, which kv::Operand's values need, is not at hand here
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;

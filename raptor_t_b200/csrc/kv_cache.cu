@@ -9,7 +9,7 @@
 // between two codes is at least 2^-17 away from it, more than a correctly rounded fp32 division moves it (2^-18 at 127).  So every
 // implementation of the definition gets the same codes.
 //
-// Both kernels move bytes: 2 in and 1 out a value, or the reverse.  A warp takes one block of one head, keys or values: its
+// Both kernels move bytes: 2 in and 1 out a value, or the reverse.  Two warps take one block of one head, keys or values: its
 // 64 rows of 128 bytes stay in registers between the maximum and the rounding, one pass over the data.
 #include "kv_cache.cuh"
 
@@ -156,11 +156,10 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
   using C = kv::Codes<INT8>;
   const uint32_t p = C::prepare(w);
   const float2 a = kv::unpack16<false>(C::template pair<0>(p)), b = kv::unpack16<false>(C::template pair<2>(p));
-  const float s = scale * C::kUnit;  // an exact product: a power of two
-  x[0] = a.x * s;
-  x[1] = a.y * s;
-  x[2] = b.x * s;
-  x[3] = b.y * s;
+  x[0] = a.x * scale;
+  x[1] = a.y * scale;
+  x[2] = b.x * scale;
+  x[3] = b.y * scale;
 }
 
 // grid: (block of the sequence, head) pairs of every sequence; warps 0 and 1 take the keys, 2 and 3 the values, 32 tokens each.
@@ -269,9 +268,9 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
   if ((warp & 1) == 0 && lane == 0 && !keep) *scale_at = scale;
 }
 
-// The same grid; out_k / out_v are token-major [tokens][heads * 64].
+// The same grid and warps; out_k / out_v are token-major [tokens][heads * 64].
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(64)
+__global__ void __launch_bounds__(kWriteThreads, 8)
 kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, const int32_t* __restrict__ table,
                int table_stride, const int32_t* __restrict__ start, const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
   RT_PDL_LAUNCH_DEPENDENTS();
@@ -279,26 +278,25 @@ kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ ou
   const int head = blockIdx.x % c.heads;
   const int nth = blockIdx.x / c.heads % spans;
   const int seq = blockIdx.x / c.heads / spans;
-  const int lane = threadIdx.x & 31;
-  const bool values = threadIdx.x >= 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool values = warp >= 2;
   const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheRead);
   if (s.page < 0) return;
   const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
-  const uint8_t* src = (values ? c.v : c.k) + slot * 4096;
+  const int row0 = (warp & 1) * 32 + (lane >> 3), col = (lane & 7) * 8;
+  const int lo = static_cast<int>(s.lo - s.base), hi = static_cast<int>(s.hi - s.base);
+  const uint8_t* src = (values ? c.v : c.k) + slot * 4096 + row0 * 64 + col;
   const float scale = (values ? c.v_scale : c.k_scale)[slot];
-  uint16_t* out = values ? out_v : out_k;
-  const int sub = lane >> 3, col = (lane & 7) * 8;
-  uint2 w[16];
+  uint16_t* out = (values ? out_v : out_k) + ((s.row0 + s.base + row0) * c.heads + head) * 64 + col;
+  uint2 w[8];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t pos = s.base + 4 * i + sub;
+  for (int i = 0; i < 8; ++i) {
     w[i] = make_uint2(0, 0);
-    if (pos >= s.lo && pos < s.hi) w[i] = *reinterpret_cast<const uint2*>(src + (4 * i + sub) * 64 + col);
+    if (row0 + 4 * i >= lo && row0 + 4 * i < hi) w[i] = __ldg(reinterpret_cast<const uint2*>(src + 256 * i));
   }
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t pos = s.base + 4 * i + sub;
-    if (pos < s.lo || pos >= s.hi) continue;
+  for (int i = 0; i < 8; ++i) {
+    if (row0 + 4 * i < lo || row0 + 4 * i >= hi) continue;
     float f[8];
     values4<INT8>(w[i].x, scale, f);
     values4<INT8>(w[i].y, scale, f + 4);
@@ -307,7 +305,7 @@ kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ ou
     o.y = kv::pack16<BF16>(f[2], f[3]);
     o.z = kv::pack16<BF16>(f[4], f[5]);
     o.w = kv::pack16<BF16>(f[6], f[7]);
-    *reinterpret_cast<uint4*>(out + ((s.row0 + pos) * c.heads + head) * 64 + col) = o;
+    *reinterpret_cast<uint4*>(out + static_cast<int64_t>(i) * 4 * c.heads * 64) = o;
   }
 }
 
@@ -372,7 +370,7 @@ extern "C" rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* out_k, voi
   const bool int8 = cache->format == RT_KV_INT8;
   auto kern = dtype == RT_BF16 ? (int8 ? kv_read_kernel<true, true> : kv_read_kernel<true, false>)
                                : (int8 ? kv_read_kernel<false, true> : kv_read_kernel<false, false>);
-  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(64), 0, static_cast<cudaStream_t>(stream), c,
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
                               static_cast<uint16_t*>(out_k), static_cast<uint16_t*>(out_v), table, table_stride, start, first, tokens,
                               max_tokens, static_cast<int>(spans_of(max_tokens)), err));
   count_launch();

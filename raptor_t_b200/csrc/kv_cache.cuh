@@ -38,9 +38,8 @@ __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
 
 // Codes as half2, exactly.
 //   int8: the code with its sign bit flipped is an unsigned byte u = code + 128; the half with bits 0x6400 | u is 1024 + u.
-//   e4m3: sign, exponent and mantissa bits moved to where a half has them: the half is the value times 2^-8 (the exponents' biases
-//     differ by 8), subnormal codes included.  kUnit is what brings it back.  The NaN code, which the writer never stores, reads
-//     as 480, so that bytes nobody wrote are finite numbers, too.
+//   e4m3: the hardware's conversion.  The writer never stores the code NaN; where it stands in a place that holds no token, the kernels
+//     that would multiply it take a zero instead.
 template <bool INT8>
 struct Codes;
 
@@ -59,12 +58,14 @@ struct Codes<true> {
 
 template <>
 struct Codes<false> {
-  static constexpr float kUnit = 256.f;
+  static constexpr float kUnit = 1.f, kBias = 0.f;
   static __device__ __forceinline__ uint32_t prepare(uint32_t w) { return w; }
   template <int LO>
   static __device__ __forceinline__ uint32_t pair(uint32_t w) {
-    const uint32_t x = prmt(w, 0u, LO == 0 ? 0x1404u : 0x3424u);
-    return (x & 0x80008000u) | ((x >> 1) & 0x3f803f80u);
+    uint32_t r;
+    if constexpr (LO == 0) asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, lo;}" : "=r"(r) : "r"(w));
+    else asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.rn.f16x2.e4m3x2 %0, hi;}" : "=r"(r) : "r"(w));
+    return r;
   }
 };
 
