@@ -28,6 +28,7 @@ constexpr int kThreads = 256;
 constexpr int kGroup = 4;  // threads of a group
 constexpr int kGroups = kThreads / kGroup;
 constexpr int kMaxTop = 32;
+constexpr int kMaxRanks = 4;  // CTAs of a row
 constexpr int kListed = 1024;  // candidates that a CTA can list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 5.5f;  // the reference follows a share's maximum when e^z has grown by more than 2^8
@@ -289,6 +290,17 @@ __device__ __forceinline__ int index_of(unsigned long long key) { return static_
 
 __device__ __forceinline__ unsigned long long max_u64(unsigned long long a, unsigned long long b) { return a > b ? a : b; }
 
+// How many of n keys are better; eight loads at a time.
+__device__ __forceinline__ int better(const unsigned long long* keys, int n, unsigned long long key) {
+  int before = 0, i = 0;
+  for (; i + 8 <= n; i += 8) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) before += keys[i + k] > key;
+  }
+  for (; i < n; ++i) before += keys[i] > key;
+  return before;
+}
+
 struct ScoreArgs {
   const void* logits;
   int64_t pitch;
@@ -305,22 +317,35 @@ struct ScoreArgs {
 template <int TYPE>
 __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const ScoreArgs a) {
   using L = Logits<TYPE>;
-  __shared__ Stats s_warp[kThreads / 32];
-  __shared__ Stats s_cta;                            // of the CTA, then of the row
+  constexpr int kRowWarps = kMaxRanks * kThreads / 32;
+  // of the row's first CTA: what every warp of the row has found, written by them, and what comes of it
+  __shared__ Stats s_warp[kRowWarps];
+  __shared__ float s_warp_max[kRowWarps];
+  __shared__ unsigned long long s_all[kMaxRanks * kMaxTop];  // the best of each CTA, in order; 0: none
+  __shared__ unsigned long long s_best[kMaxTop];
+  __shared__ Stats s_row;
+  __shared__ float s_max;
+  // of each CTA
   __shared__ __align__(16) float s_group[kGroups];
-  __shared__ float s_warp_max[kThreads / 32];
-  __shared__ float s_max;                            // of the CTA
-  __shared__ int s_flagged[kThreads], s_flags;       // threads whose share holds candidates
-  __shared__ float s_bar;                            // what a candidate reaches
+  __shared__ int s_flagged[kThreads], s_flags;  // threads whose share holds candidates
+  __shared__ float s_bar;                       // what a candidate reaches
   __shared__ int s_count;
   __shared__ unsigned long long s_list[kListed];
-  __shared__ unsigned long long s_best[kMaxTop];     // the CTA's best, in order; 0: none
-  __shared__ unsigned long long s_all[8 * kMaxTop];  // those of the cluster
   RT_PDL_LAUNCH_DEPENDENTS();
   RT_PDL_WAIT();
   const int rank = blockIdx.x % a.ranks, row = blockIdx.x / a.ranks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Share<TYPE> share(static_cast<const typename L::T*>(a.logits) + row * a.pitch, a.vocab, rank, a.ranks);
+  static_assert(kMaxRanks * kMaxTop <= kThreads && kRowWarps <= 64, "");
+  if (tid < kMaxRanks * kMaxTop) s_all[tid] = 0;
+  if (tid == 0) s_count = s_flags = 0;
+  if (a.ranks > 1) ptx::cluster_arrive();  // waited for before another CTA's shared memory is written
+  int target = -1;
+  float z_target = 0.f;
+  if (tid == 0 && rank == 0 && a.logp) {  // on its way with the row
+    target = a.targets[row];
+    if (target >= 0 && target < a.vocab) z_target = L::one(share.row + target);
+  }
 
   Stats mine;
   float my_most = -INFINITY;
@@ -401,26 +426,26 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Score
   }
   join_warp(mine);
   const float warp_most = warp_max(my_most);
+  // the address of a variable in the row's first CTA
+  auto home = [&](const void* p) {
+    uint32_t at = ptx::smem_u32(p);
+    if (a.ranks > 1) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(at));
+    return at;
+  };
+  auto put = [](uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); };
+  auto put_key = [&](int place, unsigned long long key) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(home(&s_all[rank * a.top + place])), "l"(key) : "memory");
+  };
+  if (a.ranks > 1) ptx::cluster_wait();
   if (lane == 0) {
-    s_warp[warp] = mine;
-    s_warp_max[warp] = warp_most;
+    const int w = rank * (kThreads / 32) + warp;
+    const uint32_t at = home(&s_warp[w]);
+    put(at, mine.r);
+    put(at + 4, mine.s);
+    put(at + 8, mine.w);
+    put(home(&s_warp_max[w]), warp_most);
   }
-  if (tid == 0) s_count = s_flags = 0;
   __syncthreads();
-  if (warp == kThreads / 32 - 1) {
-    Stats all;
-    float most = -INFINITY;
-    if (lane < kThreads / 32) {
-      all = s_warp[lane];
-      most = s_warp_max[lane];
-    }
-    join_warp(all);
-    most = warp_max(most);
-    if (lane == 0) {
-      s_cta = all;
-      s_max = most;
-    }
-  }
   if (a.top > 0) {
     if (tid < kGroups) {  // the top-th largest of the groups' maxima: equal ones by place
       const float x = s_group[tid];
@@ -443,34 +468,37 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Score
         if (at < kListed) s_list[at] = key_of(z, index);
       }
     };
-    if (my_most >= bar) s_flagged[atomicAdd(&s_flags, 1)] = tid;
     if (tid < 2 * L::kVec) {
       const int at = share.outside(tid);
       if (at >= 0) list(L::one(share.row + at), at);
     }
-    __syncthreads();
-    {  // the vectors of those threads, one a thread and turn
-      const int per = (share.hi - share.lo + kThreads - 1) / kThreads, n = s_flags * per;
+    auto look = [&](int i) {
+      float x[L::kVec];
+      L::unpack(__ldg(share.vectors() + i), x);
+#pragma unroll
+      for (int j = 0; j < L::kVec; ++j) list(x[j], share.head + i * L::kVec + j);
+    };
+    const int per = (share.hi - share.lo + kThreads - 1) / kThreads;
+    if (per <= 4) {
+      if (my_most >= bar)
+        for (int i = share.lo + tid; i < share.hi; i += kThreads) look(i);
+    } else {  // the vectors of all these threads, one a thread and turn
+      if (my_most >= bar) s_flagged[atomicAdd(&s_flags, 1)] = tid;
+      __syncthreads();
+      const int n = s_flags * per;
       for (int q = tid; q < n; q += kThreads) {
         const int i = share.lo + s_flagged[q / per] + q % per * kThreads;
-        if (i >= share.hi) continue;
-        float x[L::kVec];
-        L::unpack(__ldg(share.vectors() + i), x);
-#pragma unroll
-        for (int j = 0; j < L::kVec; ++j) list(x[j], share.head + i * L::kVec + j);
+        if (i < share.hi) look(i);
       }
     }
-    if (tid < kMaxTop) s_best[tid] = 0;
     __syncthreads();
     const int count = s_count;
     if (count <= kListed) {
       for (int c = tid; c < count; c += kThreads) {
         const unsigned long long key = s_list[c];
-        int before = 0;
-        for (int i = 0; i < count && before < a.top; ++i) before += s_list[i] > key;
-        if (before < a.top) s_best[before] = key;
+        const int before = better(s_list, count, key);
+        if (before < a.top) put_key(before, key);
       }
-      __syncthreads();
     } else {  // too many: one search for each place, for the best below the one before
       unsigned long long last = ~0ull;
       for (int k = 0; k < a.top; ++k) {
@@ -488,66 +516,60 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Score
         __syncthreads();
         best = s_list[0];
         for (int w = 1; w < kThreads / 32; ++w) best = max_u64(best, s_list[w]);
-        if (tid == 0) s_best[k] = best;
+        if (tid == 0) put_key(k, best);
         last = best;
         __syncthreads();
       }
     }
   }
-  __syncthreads();
-  const unsigned long long* best = s_best;
+  // ---- the row's first CTA has everything
+  __syncwarp();
   if (a.ranks > 1) {
     ptx::cluster_arrive();
-    ptx::cluster_wait();
-    if (rank == 0) {
-      auto peer = [](const void* p, int r) {
-        uint32_t at;
-        asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(ptx::smem_u32(p)), "r"(r));
-        return at;
-      };
-      const int n = a.ranks * a.top;
-      if (tid < n) {
-        unsigned long long key;
-        asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(key) : "r"(peer(&s_best[tid % a.top], tid / a.top)) : "memory");
-        s_all[tid] = key;
-      }
-      if (warp == kThreads / 32 - 1) {
-        Stats x;
-        float most = -INFINITY;
-        if (lane < a.ranks) {
-          const uint32_t at = peer(&s_cta, lane);
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.r) : "r"(at) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.s) : "r"(at + 4) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x.w) : "r"(at + 8) : "memory");
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(most) : "r"(peer(&s_max, lane)) : "memory");
-        }
-        join_warp(x);
-        most = warp_max(most);
-        if (lane == 0) {
-          s_warp[0] = x;
-          s_warp_max[0] = most;
-        }
-      }
-      __syncthreads();
-      if (tid == 0) {
-        s_cta = s_warp[0];
-        s_max = s_warp_max[0];
-      }
-      if (tid < kMaxTop) s_best[tid] = 0;
-      __syncthreads();
-      if (tid < n) {
-        const unsigned long long key = s_all[tid];
-        int before = 0;
-        for (int i = 0; i < n; ++i) before += s_all[i] > key;
-        if (key != 0 && before < a.top) s_best[before] = key;
-      }
-      __syncthreads();
-    }
-    ptx::cluster_arrive();  // no CTA leaves while rank 0 reads its shared memory
-    ptx::cluster_wait();
     if (rank != 0) return;
+    ptx::cluster_wait();
+  } else {
+    __syncthreads();
   }
-  const Stats all = s_cta;
+  if (warp == kThreads / 32 - 1) {
+    const int n = a.ranks * (kThreads / 32);
+    Stats x, y;
+    float most = -INFINITY;
+    if (lane < n) {
+      x = s_warp[lane];
+      most = s_warp_max[lane];
+    }
+    if (lane + 32 < n) {
+      y = s_warp[lane + 32];
+      most = fmaxf(most, s_warp_max[lane + 32]);
+      const float to = fmaxf(x.r, y.r);
+      if (to != x.r) x.raise(to);
+      if (to != y.r) y.raise(to);
+      x.s += y.s;
+      x.w += y.w;
+    }
+    join_warp(x);
+    most = warp_max(most);
+    if (lane == 0) {
+      s_row = x;
+      s_max = most;
+    }
+  } else if (a.ranks > 1 && tid < a.top) {
+    s_best[tid] = 0;
+  }
+  const unsigned long long* best = s_all;
+  __syncthreads();
+  if (a.ranks > 1 && a.top > 0) {
+    const int n = a.ranks * a.top;
+    if (tid < n) {
+      const unsigned long long key = s_all[tid];
+      const int before = better(s_all, n, key);
+      if (key != 0 && before < a.top) s_best[before] = key;
+    }
+    best = s_best;
+    __syncthreads();
+  }
+  const Stats all = s_row;
   const float m = s_max;
   const bool nothing = m == -INFINITY && all.s == 0.f;  // a row of -inf
   const float log2_s = log2f(all.s);
@@ -556,13 +578,12 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const Score
     a.stats[row] = make_float2(m, log_s);
     if (a.entropy) a.entropy[row] = nothing ? 0.f : kLn2 * (log2_s - all.w / all.s);
     if (a.logp) {
-      const int t = a.targets[row];
       float r = 0.f;
-      if (t >= a.vocab) {
+      if (target >= a.vocab) {
         atomicCAS(a.err, 0, kSiteToken);
         r = NAN;
-      } else if (t >= 0) {
-        r = nothing ? -INFINITY : (L::one(share.row + t) - m) - log_s;
+      } else if (target >= 0) {
+        r = nothing ? -INFINITY : (z_target - m) - log_s;
       }
       a.logp[row] = r;
     }
@@ -712,7 +733,7 @@ extern "C" rt_status rt_token_logprobs(const void* logits, int64_t pitch, const 
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "token_logprobs: cannot allocate the device error word");
   // few rows: several CTAs for each, as long as every thread has four vectors
   const int vectors = vocab / (16 / type_size(dtype));
-  while (a.ranks < 8 && static_cast<int64_t>(rows) * a.ranks < 148 && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
+  while (a.ranks < kMaxRanks && static_cast<int64_t>(rows) * a.ranks * 2 <= 148 && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
   RT_REQUIRE(static_cast<int64_t>(rows) * a.ranks < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
   auto kern = dtype == RT_F32 ? token_logprobs_kernel<RT_F32> : dtype == RT_BF16 ? token_logprobs_kernel<RT_BF16> : token_logprobs_kernel<RT_F16>;
   cudaLaunchConfig_t cfg{};
