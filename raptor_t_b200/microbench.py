@@ -7,6 +7,9 @@ python/benchmark/attention_test.py and mem_bound_op.py, re-stated for this libra
     python -m raptor_t_b200.microbench --kernel transpose --seq 4096 --batch 8
     python -m raptor_t_b200.microbench --kernel gemm --m 16384 --n 3072 --k 768
     python -m raptor_t_b200.microbench --kernel gemm_ln --m 16384 --n 768 --k 3072
+    python -m raptor_t_b200.microbench --kernel kv_cache --seq 4096 --batch 8 --format int8
+    python -m raptor_t_b200.microbench --kernel cached_attention --seq 4096 --batch 32 --queries 1
+    python -m raptor_t_b200.microbench --kernel scores --rows 2048 --vocab 50358 --top 5
     python -m raptor_t_b200.microbench --kernel all
 
 Each line of output is one JSON object: algorithmic FLOPs or bytes, the median CUDA-event
@@ -162,10 +165,71 @@ def bench_gemm_ln(m, n, k, dtype, iters):
             "two_kernel_ms": med2, "peak": tf, "peak_source": src}
 
 
+def _cache(seq, batch, kv_heads, fmt):
+    """A filled cache, its block table and the sequences' lengths."""
+    width = -(-seq // 64)
+    blocks = width * batch
+    dt = torch.int8 if fmt == "int8" else torch.float8_e4m3fn
+    codes = [(torch.randn(blocks, kv_heads, 64, 64, device="cuda") * 40).clamp(-127, 127).to(dt) for _ in range(2)]
+    cache = ops.KvCache(*codes, *(torch.full((blocks, kv_heads), 0.0234375, device="cuda") for _ in range(2)))
+    table = torch.randperm(blocks, device="cuda").int().view(batch, width).contiguous()
+    return cache, table, torch.full((batch,), seq, dtype=torch.int32, device="cuda")
+
+
+def _i32(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def bench_kv_cache(seq, batch, dtype, iters, heads=12, fmt="e4m3"):
+    """Whole documents into the cache, and back."""
+    hbm, tf, src = _peaks()
+    dt = _dtype(dtype)
+    cache, table, _ = _cache(seq, batch, heads, fmt)
+    T = seq * batch
+    k, v = (torch.randn(T, heads, 64, device="cuda").to(dt) for _ in range(2))
+    start, first = _i32([0] * batch), _i32([i * seq for i in range(batch + 1)])
+    w, w_best = _time(lambda: ops.kv_cache_write(cache, k, v, table, start, first, seq), iters)
+    r, r_best = _time(lambda: ops.kv_cache_read(cache, table, start, first, T, dt, seq, out=(k, v)), iters)
+    nbytes = 3.0 * T * heads * 128
+    return [{"kernel": name, "tokens": T, "heads": heads, "dtype": dtype, "format": fmt, "bytes": nbytes, "ms": med, "ms_min": best,
+             "gbs": nbytes / med / 1e6, "frac_of_hbm_peak": nbytes / med / 1e6 / hbm, "peak": hbm, "peak_source": src}
+            for name, med, best in (("kv_cache_write", w, w_best), ("kv_cache_read", r, r_best))]
+
+
+def bench_cached_attention(seq, batch, rows, dtype, iters, heads=12, kv_heads=12, fmt="e4m3"):
+    """`rows` query tokens of every sequence over `seq` cached ones."""
+    hbm, tf, src = _peaks()
+    cache, table, ctx = _cache(seq, batch, kv_heads, fmt)
+    q = torch.randn(batch * rows, heads, 64, device="cuda").to(_dtype(dtype))
+    first, out = _i32([i * rows for i in range(batch + 1)]), torch.empty_like(q)
+    med, best = _time(lambda: ops.cached_attention(q, cache, table, ctx, first, rows, scale=0.125, out=out), iters)
+    nbytes, flops = 128.0 * seq * batch * kv_heads + 4.0 * q.numel(), 256.0 * batch * rows * heads * seq
+    return {"kernel": "cached_attention", "seq": seq, "batch": batch, "rows": rows, "heads": heads, "kv_heads": kv_heads, "dtype": dtype,
+            "format": fmt, "bytes": nbytes, "flops": flops, "ms": med, "ms_min": best, "gbs": nbytes / med / 1e6,
+            "tflops": flops / med / 1e9, "frac_of_floor": max(nbytes / hbm / 1e6, flops / tf / 1e9) / med, "peak": [hbm, tf],
+            "peak_source": src}
+
+
+def bench_scores(rows, vocab, top, dtype, iters):
+    """Log probabilities, entropy and the best alternatives of rows of logits, and their gradient."""
+    hbm, tf, src = _peaks()
+    z = torch.randn(rows, vocab, device="cuda").to(_dtype(dtype))
+    t = torch.randint(0, vocab, (rows,), dtype=torch.int32, device="cuda")
+    s = ops.token_logprobs(z, t, top)
+    g, d = torch.ones(rows, device="cuda"), torch.empty_like(z)
+    f, f_best = _time(lambda: ops.token_logprobs(z, t, top), iters)
+    b, b_best = _time(lambda: ops.token_logprobs_backward(z, t, s.stats, grad_logp=g, out=d), iters)
+    return [{"kernel": name, "rows": rows, "vocab": vocab, "top_k": top, "dtype": dtype, "bytes": n, "ms": med, "ms_min": best,
+             "gbs": n / med / 1e6, "frac_of_hbm_peak": n / med / 1e6 / hbm, "peak": hbm, "peak_source": src}
+            for name, med, best, n in (("token_logprobs", f, f_best, 2.0 * rows * vocab),
+                                       ("token_logprobs_backward", b, b_best, 4.0 * rows * vocab))]
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--kernel", default="all",
-                    choices=["all", "attention", "layernorm", "gelu", "transpose", "gemm", "gemm_ln", "attention_sweep"])
+                    choices=["all", "attention", "layernorm", "gelu", "transpose", "gemm", "gemm_ln", "attention_sweep", "kv_cache",
+                             "cached_attention", "scores"])
     ap.add_argument("--seq", type=int, default=4096)
     ap.add_argument("--batch", type=int, default=8)
     ap.add_argument("--heads", type=int, default=12)
@@ -176,6 +240,11 @@ def main():
     ap.add_argument("--k", type=int, default=768)
     ap.add_argument("--dtype", default="bf16", choices=["bf16", "f16"])
     ap.add_argument("--pattern", default="bigbird", choices=["bigbird", "band"])
+    ap.add_argument("--queries", type=int, default=1)
+    ap.add_argument("--kv-heads", type=int, default=12)
+    ap.add_argument("--format", default="e4m3", choices=["e4m3", "int8"])
+    ap.add_argument("--vocab", type=int, default=50358)
+    ap.add_argument("--top", type=int, default=5)
     ap.add_argument("--iters", type=int, default=20)
     a = ap.parse_args()
     if not torch.cuda.is_available():
@@ -199,7 +268,17 @@ def main():
         out.append(bench_gemm(a.m, a.n, a.k, a.dtype, a.iters))
     if a.kernel == "gemm_ln":
         out.append(bench_gemm_ln(a.m, a.n, a.k, a.dtype, a.iters))
+    if a.kernel == "kv_cache":
+        out += bench_kv_cache(a.seq, a.batch, a.dtype, a.iters, a.heads, a.format)
+    if a.kernel == "cached_attention":
+        out.append(bench_cached_attention(a.seq, a.batch, a.queries, a.dtype, a.iters, a.heads, a.kv_heads, a.format))
+    if a.kernel == "scores":
+        out += bench_scores(min(a.rows, 8192), a.vocab, a.top, a.dtype, a.iters)
     if a.kernel == "all":
+        out += bench_kv_cache(4096, 8, a.dtype, a.iters)
+        for batch, rows in ((1, 1), (32, 1), (8, 16), (4, 1024)):
+            out.append(bench_cached_attention(4096, batch, rows, a.dtype, a.iters))
+        out += bench_scores(2048, 50358, 5, a.dtype, a.iters)
         out.append(bench_layernorm(32768, 768, a.dtype, a.iters))
         out.append(bench_layernorm(32768, 1024, a.dtype, a.iters))
         out.append(bench_gelu(32768, 3072, a.dtype, a.iters))

@@ -74,6 +74,65 @@ class BertPooler:
         return ops.pooler(input_tensor, seq_position_info_tensor, self.w, self.b, out=output)
 
 
+class BertCachedAttention:
+    """An attention sub-layer whose keys and values are kept: encoded documents join an 8-bit cache (remember), later tokens join
+    them and attend to everything their sequence has so far (__call__).  No counterpart in the reference, whose attention
+    ends with its batch.  Weights as BertAttention takes them: qkv_weight [H, 3H] (query | key | value), dense_weight [H, H], [in, out]."""
+
+    def __init__(self, qkv_weight, qkv_bias, dense_weight, dense_bias, ln_weight, ln_bias, num_attention_heads, eps=1e-12):
+        self.heads, self.H, self.eps = num_attention_heads, dense_weight.shape[0], eps
+        self.qkv_w, self.qkv_b = qkv_weight.t().contiguous(), qkv_bias.contiguous()  # [3H, H]
+        self.kv_w, self.kv_b = self.qkv_w[self.H:].contiguous(), self.qkv_b[self.H:].contiguous()
+        self.out_w, self.out_b = dense_weight.t().contiguous(), dense_bias.contiguous()
+        self.ln_w, self.ln_b = ln_weight.contiguous(), ln_bias.contiguous()
+
+    def remember(self, hidden, cache, block_table, start, first, max_tokens=None):
+        """Keys and values of hidden [tokens, H] go into the cache (the arguments of ops.kv_cache_write)."""
+        kv = ops.gemm(hidden, self.kv_w, self.kv_b, ops.capi.RT_EPI_BIAS)
+        k, v = (t.unflatten(1, (self.heads, 64)) for t in kv.split(self.H, 1))
+        ops.kv_cache_write(cache, k, v, block_table, start, first, max_tokens)
+
+    def __call__(self, hidden, cache, block_table, start, context, first, max_tokens=None, max_context=0):
+        """hidden [tokens, H]: rows first[s] .. first[s + 1] - 1 are new tokens of sequence s, which has start[s] tokens in the cache and
+        context[s] with them.  Returns LayerNorm(attention output + hidden)."""
+        qkv = ops.gemm(hidden, self.qkv_w, self.qkv_b, ops.capi.RT_EPI_BIAS)
+        q, k, v = (t.unflatten(1, (self.heads, 64)) for t in qkv.split(self.H, 1))
+        ops.kv_cache_write(cache, k, v, block_table, start, first, max_tokens)
+        ctx = ops.cached_attention(q, cache, block_table, context, first, max_tokens, max_context, scale=0.125, causal=True)
+        out = ops.gemm(ctx.flatten(1), self.out_w)
+        return ops.bias_residual_layernorm(out, self.out_b, hidden, self.ln_w, self.ln_b, self.eps)
+
+
+class BertLMHead:
+    """The masked-token head of the reference's validation model (python/modeling_big_bird.py, BigBirdLMPredictionHead: dense + GELU +
+    LayerNorm, then the decoder over the vocabulary), which the reference's own module does not have, with scores of tokens instead of a
+    softmax over all of them.  dense_weight [H, H] is [in, out] as from_torch would pass it, decoder_weight [vocab, H] the embedding table."""
+
+    def __init__(self, dense_weight, dense_bias, ln_weight, ln_bias, decoder_weight, decoder_bias, eps=1e-12):
+        self.w, self.b = dense_weight.t().contiguous(), dense_bias.contiguous()
+        self.ln_w, self.ln_b, self.eps = ln_weight.contiguous(), ln_bias.contiguous(), eps
+        self.vocab = decoder_weight.shape[0]
+        pad = -self.vocab % 64  # the projection's columns come in 64
+        self.dec_w = torch.nn.functional.pad(decoder_weight, (0, 0, 0, pad)).contiguous()
+        self.dec_b = torch.nn.functional.pad(decoder_bias, (0, pad)).contiguous()
+
+    def logits(self, hidden):
+        """[rows, vocab] of hidden [rows, H]: a view of rows padded to a multiple of 64 columns."""
+        x = ops.gemm(hidden, self.w, self.b, ops.capi.RT_EPI_BIAS_GELU)
+        ops.bias_residual_layernorm(x, None, None, self.ln_w, self.ln_b, self.eps)
+        return ops.gemm(x, self.dec_w, self.dec_b, ops.capi.RT_EPI_BIAS)[:, :self.vocab]
+
+    def __call__(self, hidden, targets=None, top_k=0):
+        """(ops.TokenScores, logits) of hidden [rows, H], e.g. the rows of the masked tokens."""
+        z = self.logits(hidden)
+        return ops.token_logprobs(z, targets, top_k), z
+
+    def logits_gradient(self, logits, targets, scores, grad_logp=None, grad_entropy=None, grad_top=None, out=None):
+        """Gradient of the scores with respect to the logits; out may be the logits."""
+        return ops.token_logprobs_backward(logits, targets, scores.stats, scores.entropy, grad_logp, grad_entropy, scores.top_ids, grad_top,
+                                           out)
+
+
 class BertModelNoPooler:
     """python/modeling_bert.py:318-394."""
 
