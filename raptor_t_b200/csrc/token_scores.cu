@@ -29,6 +29,7 @@ constexpr int kGroup = 4;  // threads of a group
 constexpr int kGroups = kThreads / kGroup;
 constexpr int kMaxTop = 32;
 constexpr int kMaxRanks = 4;  // CTAs of a row
+constexpr int kSms = 148;
 constexpr int kListed = 1024;  // candidates that a CTA can list
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kSlack = 5.5f;  // the reference follows a share's maximum when e^z has grown by more than 2^8
@@ -314,8 +315,9 @@ struct ScoreArgs {
   int* err;
 };
 
-template <int TYPE>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const ScoreArgs a) {
+// CTAS: how many an SM holds at once; the registers of a thread follow from it.
+template <int TYPE, int CTAS>
+__global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const ScoreArgs a) {
   using L = Logits<TYPE>;
   constexpr int kRowWarps = kMaxRanks * kThreads / 32;
   // of the row's first CTA: what every warp of the row has found, written by them, and what comes of it
@@ -719,6 +721,31 @@ rt_status check_logits(const char* what, const void* logits, int64_t pitch, int 
 
 using namespace rt;
 
+namespace {
+
+// A row takes about as long as all others, so the CTAs come in rounds, and the last round is as long as a full one.  More CTAs on an SM have
+// fewer registers for loads in flight and take longer for a round (592 rows of 50,358 fp16 logits: 4 CTAs an SM 16.3 us, 5: 18.5, 6: 20.7), in
+// the ratio CTAs + 3.5, but there may be fewer rounds: 2,048 rows 53.2, 48.1, 48.0 us, 4,096 rows 95.8, 87.9, 83.4, 700 rows 25.4, 19.1, 21.1.
+int ctas_of_an_sm(int64_t ctas) {
+  int best = 4;
+  double least = 0;
+  for (int n = 4; n <= 6; ++n) {
+    const double cost = static_cast<double>((ctas + kSms * n - 1) / (kSms * n)) * (n + 3.5);
+    if (n == 4 || cost < least) {
+      best = n;
+      least = cost;
+    }
+  }
+  return best;
+}
+
+template <int TYPE>
+void (*kernel_of(int ctas))(const ScoreArgs) {
+  return ctas == 4 ? token_logprobs_kernel<TYPE, 4> : ctas == 5 ? token_logprobs_kernel<TYPE, 5> : token_logprobs_kernel<TYPE, 6>;
+}
+
+}  // namespace
+
 extern "C" rt_status rt_token_logprobs(const void* logits, int64_t pitch, const int32_t* targets, int rows, int vocab, int top,
                                        float* logp, float* entropy, float* stats, int32_t* top_ids, float* top_logp, int dtype,
                                        void* stream) {
@@ -733,9 +760,10 @@ extern "C" rt_status rt_token_logprobs(const void* logits, int64_t pitch, const 
   RT_REQUIRE(a.err != nullptr, RT_ERR_CUDA, "token_logprobs: cannot allocate the device error word");
   // few rows: several CTAs for each, as long as every thread has four vectors
   const int vectors = vocab / (16 / type_size(dtype));
-  while (a.ranks < kMaxRanks && static_cast<int64_t>(rows) * a.ranks * 2 <= 148 && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
+  while (a.ranks < kMaxRanks && static_cast<int64_t>(rows) * a.ranks * 2 <= kSms && vectors >= 4 * kThreads * a.ranks) a.ranks *= 2;
   RT_REQUIRE(static_cast<int64_t>(rows) * a.ranks < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "token_logprobs: too many rows");
-  auto kern = dtype == RT_F32 ? token_logprobs_kernel<RT_F32> : dtype == RT_BF16 ? token_logprobs_kernel<RT_BF16> : token_logprobs_kernel<RT_F16>;
+  const int held = ctas_of_an_sm(static_cast<int64_t>(rows) * a.ranks);
+  auto kern = dtype == RT_F32 ? kernel_of<RT_F32>(held) : dtype == RT_BF16 ? kernel_of<RT_BF16>(held) : kernel_of<RT_F16>(held);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(rows * a.ranks));
   cfg.blockDim = dim3(kThreads);

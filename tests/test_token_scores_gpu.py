@@ -58,6 +58,14 @@ def test_scores(ops, dtype, rows, vocab, pitch, top):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows", [592, 593, 741, 889])
+def test_more_rows_than_an_sm_holds(ops, dtype, rows):
+    z, t = _rows(rows, 5003, dtype)
+    _check_forward(ops.token_logprobs(z, t, top_k=7), z, t, 7)
+    ops.check_device()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("rows", [2, 200])
 def test_equal_logits(ops, dtype, rows):
     """Constant rows, two values, and the best ones in the last places: ties go to the lower id."""
