@@ -41,13 +41,13 @@ constexpr int kThreads = 768;
 constexpr int kSoftmaxThreads = 512;
 constexpr int kStreams = 4;
 constexpr int kMaxSplits = 8;            // CTAs of a cluster
-constexpr int kStages = 8;               // operand tiles of keys, and of values: two for each warp that fills them
+constexpr int kStages = 4;               // operand tiles of keys, and of values: one for each warp that fills them
 constexpr int kRaw = 4;                  // blocks of codes on their way, one for each of these warps
 constexpr int kBlock = 4096;             // codes of a block's keys, or values
 constexpr int kRing = 32;                // scales of a block, read after its operand slots are free again
 constexpr int kTile = 64 * 128;          // 64 rows of 64 halves
 constexpr int kTmemCols = 512;
-constexpr int kColS = 0, kColO = 256;    // 4 x 64 scores (probabilities in the first half of them), 4 x 64 outputs
+constexpr int kColS = 0, kColO = 256;    // 4 x 64 scores, 4 x 64 outputs
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kPolyEvery = 8;            // pairs; 256 rows, 64 blocks: 81.8 us, with 4 83.6, with none 82.5
 constexpr float kShift = 7.0f;           // p' is 2^7 times larger than p * scale / largest scale
@@ -56,13 +56,14 @@ constexpr int kRegsSoftmax = 96, kRegsBring = 56, kRegsIssue = 40;
 
 struct Smem {
   uint8_t q[2][2 * kTile];
-  // afterwards k, v and raw hold partial results, [4 streams][128 rows][64] fp32
+  // afterwards k, v, raw and p hold partial results, [4 streams][128 rows][64] fp32
   uint8_t k[kStages][kTile];
   uint8_t v[kStages][kTile];
   uint8_t raw[kRaw][2 * kBlock];  // keys, values
+  uint8_t p[kStreams][2 * kTile];  // probabilities
   uint64_t raw_k[kRaw], raw_v[kRaw];
   uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
-  uint64_t s_full[kStreams], p_full[kStreams], o_full[kStreams];
+  uint64_t s_full[kStreams], s_free[kStreams], p_full[kStreams], o_full[kStreams];
   float2 scales[kRing];  // key and value scale of a block; a negative key scale: nobody sees its keys
   float2 ml[kStreams][128];
   float2 ml_cta[256];
@@ -72,7 +73,7 @@ struct Smem {
   uint32_t tmem_slot;
   int abort_flag;
 };
-static_assert(kStages * 2 * kTile + kRaw * 2 * kBlock >= kStreams * 128 * 64 * 4, "partial results fit the operand tiles and the ring");
+static_assert(kStages * 2 * kTile + kRaw * 2 * kBlock + kStreams * 2 * kTile >= kStreams * 128 * 64 * 4, "partial results fit");
 static_assert(sizeof(Smem) <= 227 * 1024, "one CTA per SM");
 
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
@@ -153,6 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     for (int x = 0; x < 2; ++x) mbar_init(&sm.q_full[x], two ? 8 : 16);  // the warps of its streams
     for (int x = 0; x < kStreams; ++x) {
       mbar_init(&sm.s_full[x], 1);
+      mbar_init(&sm.s_free[x], 4);
       mbar_init(&sm.p_full[x], 4);
       mbar_init(&sm.o_full[x], 1);
     }
@@ -193,45 +195,53 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const uint64_t dq = make_smem_desc_sw128(smem_u32(sm.q[two ? x >> 1 : 0]));
     const uint32_t d_s = tmem + kColS + x * 64, d_o = tmem + kColO + x * 64;
     const int end = end_of(x);
+    const uint64_t dp = make_smem_desc_sw128(smem_u32(sm.p[x]));
     bool ok = true;
     uint32_t c = 0;  // steps so far
-    if (first_of(x) < end) ok = wait(&sm.q_full[two ? x >> 1 : 0], 0, 310);
-    for (int j = first_of(x); ok && j < n_blocks; j += stride) {
+    auto round_of = [](int j) { return static_cast<uint32_t>(j / kStages) & 1; };
+    auto scores = [&](int j) {
       const int s = j % kStages;
-      const uint32_t round = (j / kStages) & 1;
-      ok = wait(&sm.k_full[s], round, 311);
-      if (!ok) break;
-      if (j >= end) {  // keys that this row tile does not see
-        if (leader) mbar_arrive(&sm.k_empty[s]);
-        ok = wait(&sm.v_full[s], round, 312);
-        if (leader && ok) mbar_arrive(&sm.v_empty[s]);
-        __syncwarp();
-        continue;
-      }
-      // the scores go over the probabilities of the step before, which its product reads
-      if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 315);
-      if (!ok) break;
       tc_fence_after_sync();
       if (leader) {
         const uint64_t dk = make_smem_desc_sw128(smem_u32(sm.k[s]));
 #pragma unroll
         for (int k = 0; k < 4; ++k) mma_ss(d_s, dq + (k * 32 >> 4), dk + (k * 32 >> 4), idesc_s, k ? 1u : 0u);
-        tc_commit(&sm.k_empty[s]);
         tc_commit(&sm.s_full[x]);
+        tc_commit(&sm.k_empty[s]);
       }
       __syncwarp();
-      ok = wait(&sm.v_full[s], round, 313) && wait(&sm.p_full[x], c & 1, 314);
+    };
+    int j = first_of(x);
+    if (j < end) {
+      ok = wait(&sm.q_full[two ? x >> 1 : 0], 0, 310) && wait(&sm.k_full[j % kStages], round_of(j), 311);
+      if (ok) scores(j);
+    }
+    for (; ok && j < end; j += stride, ++c) {
+      const int next = j + stride, s = j % kStages;
+      if (next < end) {  // as soon as the softmax warps have read this step's scores
+        ok = wait(&sm.k_full[next % kStages], round_of(next), 316) && wait(&sm.s_free[x], c & 1, 315);
+        if (!ok) break;
+        scores(next);
+      }
+      ok = wait(&sm.v_full[s], round_of(j), 313) && wait(&sm.p_full[x], c & 1, 314);
       if (!ok) break;
       tc_fence_after_sync();
       if (leader) {
         const uint64_t dv = make_smem_desc_sw128(smem_u32(sm.v[s]));
 #pragma unroll
-        for (int k = 0; k < 4; ++k) mma_ts(d_o, d_s + k * 8, dv + (k * 2048 >> 4), idesc_o, c > 0 || k ? 1u : 0u);
-        tc_commit(&sm.v_empty[s]);
+        for (int k = 0; k < 4; ++k) mma_ss(d_o, dp + (k * 32 >> 4), dv + (k * 2048 >> 4), idesc_o, c > 0 || k ? 1u : 0u);
         tc_commit(&sm.o_full[x]);
+        tc_commit(&sm.v_empty[s]);
       }
       __syncwarp();
-      ++c;
+    }
+    for (; ok && j < n_blocks; j += stride) {  // keys that this row tile does not see
+      const int s = j % kStages;
+      ok = wait(&sm.k_full[s], round_of(j), 320);
+      if (leader && ok) mbar_arrive(&sm.k_empty[s]);
+      ok = ok && wait(&sm.v_full[s], round_of(j), 312);
+      if (leader && ok) mbar_arrive(&sm.v_empty[s]);
+      __syncwarp();
     }
     __syncwarp();
     if (a.splits > 1) {
@@ -250,22 +260,23 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     // round before last as the last one's.
     static_assert(kRaw == 4 && kStages % 4 == 0, "a warp's blocks keep to its own slots");
     uint8_t* raw = sm.raw[own];
-    int64_t slot = 0;  // of the block that is requested next
+    int64_t slot_k = 0, slot_v = 0;  // of the blocks whose keys and values are requested next
     auto find = [&](int page, int j) {
       const bool bad = page < 0 || page >= a.cache.blocks;
       if (bad) kv::index_error(a.err, kSiteCachedAttention);
-      slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
+      const int64_t slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
       sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], a.cache.v_scale[slot]);
+      return slot;
     };
-    auto request = [&](uint8_t* dst, const uint8_t* base, uint64_t* bar) {
+    auto request = [&](uint8_t* dst, const uint8_t* base, int64_t slot, uint64_t* bar) {
       mbar_arrive_expect_tx(bar, kBlock);
       bulk_load(dst, base + slot * kBlock, kBlock, bar);
     };
     int page = 0;
     if (lane == 0 && own < n_blocks) {
-      find(__ldg(table + own), own);
-      request(raw, a.cache.k, &sm.raw_k[own]);
-      request(raw + kBlock, a.cache.v, &sm.raw_v[own]);
+      slot_k = slot_v = find(__ldg(table + own), own);
+      request(raw, a.cache.k, slot_k, &sm.raw_k[own]);
+      request(raw + kBlock, a.cache.v, slot_v, &sm.raw_v[own]);
       if (own + 4 < n_blocks) page = __ldg(table + own + 4);
     }
     // 256 chunks of 16 codes, eight a lane; rows from `rows` on hold no token: zeros, so that no code NaN meets a probability of 0
@@ -287,42 +298,50 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       fence_proxy_async_smem();
       __syncwarp();
     };
-    int j = own;
-    bool keys_done = false;
-    for (uint32_t c = 0; j < n_blocks; j += 4, ++c) {
+    // The keys go a block ahead of the values: a slot of keys is free once the scores are there, a slot of values a step later.
+    uint32_t nk = 0, nv = 0;  // blocks done
+    auto keys = [&](int j) {
       const int s = j % kStages;
-      const uint32_t before = ((j / kStages) & 1) ^ 1;
-      keys_done = false;
-      if (!wait(&sm.raw_k[own], c & 1, 322) || !wait(&sm.k_empty[s], before, 317)) break;
+      if (!wait(&sm.raw_k[own], nk & 1, 322) || !wait(&sm.k_empty[s], ((j / kStages) & 1) ^ 1, 317)) return false;
       convert(Keys(), sm.k[s], raw, 64);
+      ++nk;
       if (lane == 0) {
         mbar_arrive(&sm.k_full[s]);
         if (j + 4 < n_blocks) {
-          find(page, j + 4);
-          request(raw, a.cache.k, &sm.raw_k[own]);
+          slot_k = find(page, j + 4);
+          request(raw, a.cache.k, slot_k, &sm.raw_k[own]);
           if (j + 8 < n_blocks) page = __ldg(table + j + 8);
         }
       }
       __syncwarp();
-      keys_done = true;
-      if (!wait(&sm.raw_v[own], c & 1, 324) || !wait(&sm.v_empty[s], before, 318)) break;
+      return true;
+    };
+    auto values = [&](int j) {
+      const int s = j % kStages;
+      if (!wait(&sm.raw_v[own], nv & 1, 324) || !wait(&sm.v_empty[s], ((j / kStages) & 1) ^ 1, 318)) return false;
       convert(Values(), sm.v[s], raw + kBlock, INT8 ? 64 : sr.ctx - (j0 + j) * 64);
+      ++nv;
       if (lane == 0) {
         mbar_arrive(&sm.v_full[s]);
-        if (j + 4 < n_blocks) request(raw + kBlock, a.cache.v, &sm.raw_v[own]);
+        if (j + 4 < n_blocks) request(raw + kBlock, a.cache.v, slot_v, &sm.raw_v[own]);
       }
       __syncwarp();
+      return true;
+    };
+    bool ok = own >= n_blocks || keys(own);
+    for (int j = own; ok && j < n_blocks; j += 4) {
+      slot_v = slot_k;  // of block j + 4, if there is one
+      ok = (j + 4 >= n_blocks || keys(j + 4)) && values(j);
     }
-    if (lane == 0 && j < n_blocks) {  // gave up: copies in flight land before the CTA ends
+    if (lane == 0 && !ok) {  // gave up: copies in flight land before the CTA ends
       const long long t0 = clock64();
-      const uint32_t c = (j / 4) & 1;
       auto land = [&](uint64_t* bar, uint32_t parity) {
         while (!mbar_try_wait(bar, parity) && clock64() - t0 < kWaitCycles) {
         }
       };
-      if (!keys_done) land(&sm.raw_k[own], c);
-      else if (j + 4 < n_blocks) land(&sm.raw_k[own], c ^ 1);
-      land(&sm.raw_v[own], c);
+      const uint32_t blocks = (n_blocks - own + 3) / 4;  // of this warp; the next one's copies have been requested
+      if (nk < blocks) land(&sm.raw_k[own], nk & 1);
+      if (nv < blocks) land(&sm.raw_v[own], nv & 1);
     }
     __syncwarp();
     if (a.splits > 1) {
@@ -340,57 +359,60 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const int lim = sr.limit(a, row_c) - j0 * 64;   // keys that it sees, from this CTA's first on
     const bool live = row - lane < row0 + here;   // the warp has a row
     const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
-    // ---- the query row, as halves.  The streams of a row tile share its operand tile: with four of them each writes two of the row's
-    // eight chunks, with two each four.
-    float unit, bias = 0.f;  // a score in base 2 is (product - bias) * unit * key scale
+    // ---- the query rows, as halves.  Eight lanes a row, so that a load covers whole lines (a row a lane took 4 us); the streams of a row
+    // tile share its operand tile, and each writes its part of the rows.
+    float unit = 0.f, bias = 0.f;  // a score in base 2 is (product - bias) * unit * key scale
     {
-      const uint4* src = reinterpret_cast<const uint4*>(sr.query(a, head, row_c));
       // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
       const float sign = a.scale_log2 > 0.f ? 1.f : a.scale_log2 < 0.f ? -1.f : 0.f;
-      int up = 0;
-      if constexpr (BF16) {
-        uint32_t top = 0;
+      const float size = sign == 0.f ? 1.f : fabsf(a.scale_log2);
+      const int first_row = row - lane, chunk = lane & 7, parts = two ? 2 : 4;
+      uint4 t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 t = __ldg(src + i);
-          const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+      for (int i = 0; i < 8; ++i)
+        t[i] = __ldg(reinterpret_cast<const uint4*>(sr.query(a, head, min(first_row + 4 * i + (lane >> 3), row0 + here - 1))) + chunk);
+      uint8_t* tile_q = sm.q[two ? x >> 1 : 0] + (warp & 3) * 32 * 128;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t w[4] = {t[i].x, t[i].y, t[i].z, t[i].w};
+        int up = 0;
+        if constexpr (BF16) {
+          uint32_t top = 0;
 #pragma unroll
           for (int k = 0; k < 4; ++k) top = max(top, max((w[k] << 16) & 0x7fffffffu, w[k] & 0x7fff0000u));
-        }
-        up = kv::query_shift(top);
-      }
-      const float f = kv::pow2(up) * sign;
-      if constexpr (INT8) {  // the keys' bias times the sum of the row, as the product sees it
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint4 t = __ldg(src + i);
-          const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const float2 v = kv::unpack16<BF16>(w[k]);
-            const float2 h = kv::unpack16<false>(kv::pack16<false>(v.x * f, v.y * f));
-            bias += h.x + h.y;
-          }
+          for (int o = 4; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          up = kv::query_shift(top);
         }
-        bias *= Keys::kBias / Keys::kUnit;
-      }
-      uint8_t* at = sm.q[two ? x >> 1 : 0] + r * 128;
-      const int chunks = two ? 4 : 2, c0 = first_of(x) * chunks;
-      for (int i = c0; i < c0 + chunks; ++i) {
-        const uint4 t = __ldg(src + i);
-        const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+        const float f = kv::pow2(up) * sign;
         uint32_t h[4];
+        float sum = 0.f;  // the keys' bias times the sum of the row, as the product sees it
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float2 v = kv::unpack16<BF16>(w[k]);
           h[k] = kv::pack16<false>(v.x * f, v.y * f);
+          if constexpr (INT8) {
+            const float2 y = kv::unpack16<false>(h[k]);
+            sum += y.x + y.y;
+          }
         }
-        *reinterpret_cast<uint4*>(at + ((i ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        const int rr = 4 * i + (lane >> 3);
+        if (i % parts == first_of(x))
+          *reinterpret_cast<uint4*>(tile_q + rr * 128 + ((chunk ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        // lane l's own row is l: the row of step l / 4 and of lanes 8 * (l % 4) on
+        const int from = (lane & 3) * 8;
+        const float its_unit = __shfl_sync(0xffffffffu, kv::pow2(-up) * size, from);
+        if (lane >> 2 == i) unit = its_unit * Keys::kUnit;
+        if constexpr (INT8) {
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          const float its_sum = __shfl_sync(0xffffffffu, sum, from);
+          if (lane >> 2 == i) bias = its_sum * (Keys::kBias / Keys::kUnit);
+        }
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[two ? x >> 1 : 0]);
-      unit = kv::pow2(-up) * (sign == 0.f ? 1.f : fabsf(a.scale_log2)) * Keys::kUnit;
     }
     // ---- the largest value scale of the keys visited here
     float vref = 0.f;
@@ -409,13 +431,13 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
 
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + x * 64, to = tmem + lanes + kColO + x * 64;
+    uint8_t* p_row = sm.p[x] + r * 128;
     float m_ref = -INFINITY, l = 0.f;
     bool ok = true;
     uint32_t c = 0;
     const int end = end_of(x);
     for (int j = first_of(x); j < end; j += stride, ++c) {
       const int key0 = j * 64;
-      // the scores, and with them: the product of the step before is done, the output tile at rest
       ok = wait(&sm.s_full[x], c & 1, 319);
       if (!ok) break;
       tc_fence_after_sync();
@@ -425,6 +447,9 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       tmem_ld32(ts, s);
       tmem_ld32(ts + 32, s + 32);
       tc_wait_ld();
+      tc_fence_before_sync();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.s_free[x]);  // the next block's scores may come
       if (act) {
         if (key0 + 64 > wmin) {  // keys that some row of the warp does not see
           const int left = lim - key0;
@@ -446,7 +471,11 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
         const float e0 = __log2f(fmaxf(sc.y * inv_vref, 8.7e-19f)) + kShift;
         l *= alpha;
+        // the product of the step before is done: its probabilities may be written over, and the output tile is at rest
+        if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 321);
+        if (!ok) break;
         if (__any_sync(0xffffffffu, fix) && c > 0) {
+          tc_fence_after_sync();
 #pragma unroll 1
           for (int i = 0; i < 64; i += 16) {
             uint32_t o[16];
@@ -456,6 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
             for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
             tmem_st16(to + i, o);
           }
+          tc_wait_st();
+          tc_fence_before_sync();
         }
         // half a row at a time: the registers hold 64 scores and 32 packed probabilities at once no more than barely
         const float back = ex2(-e0);
@@ -463,22 +494,22 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         for (int h = 0; h < 2; ++h) {
           uint32_t p[16];
           l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref - e0 + off), back, l);
-          tmem_st16(ts + 16 * h, p);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(p_row + (((4 * h + i) ^ (r & 7)) << 4)) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
         }
       } else {
-        uint32_t p[16];
+        if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 323);
+        if (!ok) break;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) p[i] = 0u;
-        tmem_st16(ts, p);
-        tmem_st16(ts + 16, p);
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(p_row + 16 * i) = make_uint4(0, 0, 0, 0);
       }
-      tc_wait_st();
-      tc_fence_before_sync();
+      fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.p_full[x]);
     }
     if (ok && c > 0) {
-      ok = wait(&sm.o_full[x], (c - 1) & 1, 321);
+      ok = wait(&sm.o_full[x], (c - 1) & 1, 325);
       tc_fence_after_sync();
     }
     const bool any = ok && c > 0 && live;  // there is an output tile to read; the same for the whole warp
