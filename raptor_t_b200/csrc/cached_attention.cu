@@ -561,15 +561,17 @@ int splits_of(int64_t units, int tile_rows, int64_t keys) {
   return splits;
 }
 
-// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 9 us and 1.05 us a block of keys (0.56 for
-// at most 128 rows), 4 us more where a cluster joins its results.
+// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 14 us and 0.85 us a block of keys (11 and 0.51
+// for at most 128 rows, 0.45 for at most 64), 1 us more where a cluster joins its results.  Clusters of 2, 4 and 8 fit 74, 33 and 15 times on the chip.
 int many_rows_splits(int64_t units, int rows, int64_t keys, double* us) {
-  const double block = rows > 128 ? 1.05 : 0.56, blocks = static_cast<double>((keys + 63) / 64);
+  constexpr int kFit[4] = {kSms, 74, 33, 15};
+  const double base = rows > 128 ? 14.0 : 11.0, block = rows > 128 ? 0.85 : rows > 64 ? 0.51 : 0.45, blocks = static_cast<double>((keys + 63) / 64);
   int best = 1;
   double least = 1e30;
-  for (int splits = 1; splits <= 8; splits *= 2) {
-    const double rounds = static_cast<double>((units * splits + kSms - 1) / kSms);
-    const double cost = rounds * (9.0 + (splits > 1 ? 4.0 : 0.0) + block * blocks / splits);
+  for (int k = 0; k < 4; ++k) {
+    const int splits = 1 << k;
+    const double rounds = static_cast<double>((units + kFit[k] - 1) / kFit[k]);
+    const double cost = rounds * (base + (k > 0 ? 1.0 : 0.0) + block * blocks / splits);
     if (cost < least) {
       least = cost;
       best = splits;
@@ -649,13 +651,15 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
              "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
   const int64_t widest = static_cast<int64_t>(table_stride) * 64;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
-  // Which kernel: the one of few rows pays for every 16 rows (1.65 ns a tile and block of keys on the full chip), the one of many rows for
-  // tiles of 128 and 256.  12 x 4096 keys, 12 heads, 64 rows: 60.5 and 46 us; 16 x 2000 keys 43.7 and 54.
+  // Which kernel: the one of few rows pays for every 16 rows that there are (1.65 ns a tile and block of keys on the full chip), the one of many
+  // rows for whole tiles.  12 x 4096 keys, 12 heads, 64 rows each: 60.5 and 39.8 us; 16 x 2000 keys 45.7 and 47.3; 16 x 512 to 4096 keys, 5 to
+  // 64 rows: 41 and 53.
+  const int64_t few_tiles = std::min(n_seq * static_cast<int64_t>((rows + 15) / 16), static_cast<int64_t>(tokens) * a.group / 16 + n_seq / 2);
   const int64_t big = heads_of_all * ((rows + 255) / 256);
   double many_us = 0;
   const int many_splits = many_rows_splits(big, rows, keys, &many_us);
   const bool many = rows > kFewRows ||
-                    (rows > 48 && many_us < 5.0 + 1.65e-3 * static_cast<double>(heads_of_all * ((rows + 15) / 16)) * ((keys + 63) / 64));
+                    (rows > 32 && many_us < 5.0 + 1.65e-3 * static_cast<double>(few_tiles * a.cache.heads) * ((keys + 63) / 64));
   a.tile_rows = many ? 256 : rows <= 8 ? 8 : 16;
   a.tiles = (rows + a.tile_rows - 1) / a.tile_rows;
   const int64_t units = heads_of_all * a.tiles;

@@ -71,6 +71,15 @@ def test_many_rows(ops, fmt, causal, counts, context, heads, kv_heads):
         _case(ops, fmt, dtype, heads, kv_heads, counts, context, causal, spare_rows=2)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("counts,context", [([32] + [3] * 40, [2000] + [64] * 40), ([64] * 33, [1100] * 33), ([256, 256, 65, 33, 32, 31, 1, 97], [4000] * 8),
+                                            ([64] * 3, [64] * 3)])
+def test_copies_of_rows_and_clusters(ops, fmt, causal, counts, context):
+    """Tiles of 32, 64, 128 and 256 rows, with a CTA or a cluster for each; more clusters than fit at once."""
+    _case(ops, fmt, torch.float16, 4, 4, counts, context, causal)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_rows_that_see_nothing(ops, causal):
     """More query rows than context: with the causal rule the first ones see no key."""
