@@ -561,11 +561,11 @@ int splits_of(int64_t units, int tile_rows, int64_t keys) {
   return splits;
 }
 
-// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 14 us and 0.85 us a block of keys (11 and 0.51
+// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 13 us and 0.85 us a block of keys (10 and 0.51
 // for at most 128 rows, 0.45 for at most 64), 1 us more where a cluster joins its results.  Clusters of 2, 4 and 8 fit 74, 33 and 15 times on the chip.
 int many_rows_splits(int64_t units, int rows, int64_t keys, double* us) {
   constexpr int kFit[4] = {kSms, 74, 33, 15};
-  const double base = rows > 128 ? 14.0 : 11.0, block = rows > 128 ? 0.85 : rows > 64 ? 0.51 : 0.45, blocks = static_cast<double>((keys + 63) / 64);
+  const double base = rows > 128 ? 13.0 : 10.0, block = rows > 128 ? 0.85 : rows > 64 ? 0.51 : 0.45, blocks = static_cast<double>((keys + 63) / 64);
   int best = 1;
   double least = 1e30;
   for (int k = 0; k < 4; ++k) {

@@ -107,6 +107,21 @@ __device__ __forceinline__ void put_codes(uint8_t* tile, int row, int c, const u
   *reinterpret_cast<uint4*>(at + (((2 * c + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
 }
 
+// Token and query head of the group of a row that goes up in equal steps: two divisions, not two for each row.
+struct RowWalk {
+  int token, member, tokens, members, group;
+  __device__ __forceinline__ RowWalk(int row, int step, int group_size)
+      : token(row / group_size), member(row % group_size), tokens(step / group_size), members(step % group_size), group(group_size) {}
+  __device__ __forceinline__ void next() {
+    token += tokens;
+    member += members;
+    if (member >= group) {
+      member -= group;
+      ++token;
+    }
+  }
+};
+
 template <bool BF16, bool INT8>
 __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   using Keys = kv::Operand<INT8>;
@@ -358,25 +373,35 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const int x = warp >> 2, r = tid & 127, span = here > 64 ? 128 : here > 32 ? 64 : 32, own_r = r & (span - 1);
     const bool owner = two || r / span == x * 32 / span;
     const int row = row0 + (two ? (x >> 1) * 128 : 0) + own_r;
-    const int row_c = min(row, row0 + here - 1);  // rows behind the last one do as it does and are not stored
+    const int row_c = min(row, row0 + here - 1);  // rows behind the last one are 0 and are not stored
     const int lim = sr.limit(a, row_c) - j0 * 64;   // keys that it sees, from this CTA's first on
     const bool live = owner && row - lane < row0 + here;  // the warp has a row
     const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
-    // ---- the query rows, as halves.  Eight lanes a row, so that a load covers whole lines (a row a lane took 4 us); the streams of a row
-    // tile share its operand tile, and each writes its part of the rows.
-    float unit = 0.f, bias = 0.f;  // a score in base 2 is (product - bias) * unit * key scale
+    // ---- the query rows, as halves.  Eight lanes a row, so that a load covers whole lines (a row a lane took 4 us).  The streams of a row tile share
+    // its operand tile; each brings its part of the rows and leaves a row's unit and bias for the others.
+    const int page0 = tid < n_blocks ? __ldg(table + tid) : -1;
+    float vref = 0.f;  // the largest value scale of the keys visited here
+    float2* found = sm.ml_cta + (two ? (x >> 1) * 128 : 0);
     {
       // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
       const float sign = a.scale_log2 > 0.f ? 1.f : a.scale_log2 < 0.f ? -1.f : 0.f;
       const float size = sign == 0.f ? 1.f : fabsf(a.scale_log2);
-      const int first_row = row - lane, chunk = lane & 7, parts = two ? 2 : 4;
-      uint4 t[8];
+      const int chunk = lane & 7, parts = two ? 2 : 4, steps = 8 / parts, from = 4 * first_of(x) + (lane >> 3);
+      const int left = row0 + here - (row - lane + from);  // rows from this lane's first one on
+      RowWalk at(row - lane + from, 4 * parts, a.group);
+      uint4 t[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        t[i] = __ldg(reinterpret_cast<const uint4*>(sr.query(a, head, min(first_row + 4 * i + (lane >> 3), row0 + here - 1))) + chunk);
-      uint8_t* tile_q = sm.q[two ? x >> 1 : 0] + (warp & 3) * 32 * 128;
+      for (int i = 0; i < 4; ++i) {
+        t[i] = make_uint4(0, 0, 0, 0);
+        if (i < steps && 4 * parts * i < left)
+          t[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (sr.f0 + at.token) * a.q_stride + (head * a.group + at.member) * 64) + chunk);
+        at.next();
+      }
+      if (page0 >= 0 && page0 < a.cache.blocks) vref = a.cache.v_scale[static_cast<int64_t>(page0) * a.cache.heads + head];
+      uint8_t* tile_q = sm.q[two ? x >> 1 : 0];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
+        if (i >= steps) break;
         const uint32_t w[4] = {t[i].x, t[i].y, t[i].z, t[i].w};
         int up = 0;
         if constexpr (BF16) {
@@ -399,27 +424,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
             sum += y.x + y.y;
           }
         }
-        const int rr = 4 * i + (lane >> 3);
-        if (i % parts == first_of(x))
-          *reinterpret_cast<uint4*>(tile_q + rr * 128 + ((chunk ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-        // lane l's own row is l: the row of step l / 4 and of lanes 8 * (l % 4) on
-        const int from = (lane & 3) * 8;
-        const float its_unit = __shfl_sync(0xffffffffu, kv::pow2(-up) * size, from);
-        if (lane >> 2 == i) unit = its_unit * Keys::kUnit;
         if constexpr (INT8) {
 #pragma unroll
           for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          const float its_sum = __shfl_sync(0xffffffffu, sum, from);
-          if (lane >> 2 == i) bias = its_sum * (Keys::kBias / Keys::kUnit);
         }
+        const int rr = (warp & 3) * 32 + 4 * parts * i + from;
+        *reinterpret_cast<uint4*>(tile_q + rr * 128 + ((chunk ^ (rr & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (chunk == 0) found[rr] = make_float2(kv::pow2(-up) * size * Keys::kUnit, sum * (Keys::kBias / Keys::kUnit));
       }
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[two ? x >> 1 : 0]);
     }
-    // ---- the largest value scale of the keys visited here
-    float vref = 0.f;
-    for (int b = tid; b < n_blocks; b += kSoftmaxThreads) {
+    for (int b = tid + kSoftmaxThreads; b < n_blocks; b += kSoftmaxThreads) {
       const int page = __ldg(table + b);
       if (page >= 0 && page < a.cache.blocks) vref = fmaxf(vref, a.cache.v_scale[static_cast<int64_t>(page) * a.cache.heads + head]);
     }
@@ -427,6 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
     if (lane == 0) sm.vmax[warp] = vref;
     softmax_barrier();
+    const float unit = found[r].x, bias = found[r].y;  // a score in base 2 is (product - bias) * unit * key scale
 #pragma unroll
     for (int i = 0; i < kSoftmaxThreads / 32; ++i) vref = fmaxf(vref, sm.vmax[i]);
     if (!(vref > 0.f)) vref = 1.f;
@@ -560,13 +578,15 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       if (a.splits > 1) sm.ml_cta[tid] = make_float2(M, L);
     }
     softmax_barrier();
-    auto store = [&](int rr, int d, const float4& v) {
-      *reinterpret_cast<uint2*>(sr.output(a, head, row0 + rr) + d) = make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
+    auto store = [&](const RowWalk& to, int d, const float4& v) {
+      *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(sr.f0 + to.token) * a.heads + head * a.group + to.member) * 64 + d) =
+          make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
     };
     auto merge = [&](auto count) {
       constexpr int N = decltype(count)::value;
-#pragma unroll 2
-      for (int i = tid; i < here * 16; i += kSoftmaxThreads) {
+      RowWalk to(row0 + (tid >> 4), kSoftmaxThreads / 16, a.group);
+#pragma unroll 4
+      for (int i = tid; i < here * 16; i += kSoftmaxThreads, to.next()) {
         const int rr = i >> 4, quad = i & 15, x0 = N == 2 ? (rr >> 7) * 2 : 0, pr = rr & 127;
         float* at = reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2);
         float4 v = make_float4(0, 0, 0, 0);
@@ -579,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           v.z = fmaf(o.z, w, v.z);
           v.w = fmaf(o.w, w, v.w);
         }
-        if (a.splits == 1) store(rr, 4 * quad, v);
+        if (a.splits == 1) store(to, 4 * quad, v);
         else *reinterpret_cast<float4*>(at) = v;
       }
     };
@@ -590,7 +610,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       __syncwarp();
       cluster_arrive();
       cluster_wait();
-      for (int i = rank * kSoftmaxThreads + tid; i < here * 16; i += a.splits * kSoftmaxThreads) {
+      RowWalk to(row0 + ((rank * kSoftmaxThreads + tid) >> 4), a.splits * kSoftmaxThreads / 16, a.group);
+      for (int i = rank * kSoftmaxThreads + tid; i < here * 16; i += a.splits * kSoftmaxThreads, to.next()) {
         const int rr = i >> 4, quad = i & 15, x0 = two ? (rr >> 7) * 2 : 0, pr = rr & 127;
         const uint32_t ml_at = smem_u32(&sm.ml_cta[rr]);
         const uint32_t o_at = smem_u32(reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2));
@@ -619,7 +640,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           v.w = fmaf(o[w].w, f, v.w);
         }
         const float inv = M == -INFINITY ? 0.f : 1.f / L;
-        store(rr, 4 * quad, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        store(to, 4 * quad, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
       }
     }
     if (a.splits > 1) {
