@@ -6,18 +6,21 @@
 // times every fourth block.  A stream's step is one block: scores, softmax, output, one after the other; the four streams fill each other's waits.
 //
 //   warps 0-15       softmax, four warps a stream: thread r owns row r (TMEM lane r).  Score row from TMEM, running maximum and sum in fp32
-//                    (base-2 exponentials, every eighth pair on the FMA pipe), probabilities as halves over the scores' columns, output
-//                    rescaled only when the maximum has grown by more than 2^8.
+//                    (base-2 exponentials, every eighth pair on the FMA pipe), probabilities as halves into an operand tile of shared memory, output
+//                    rescaled only when the maximum has grown by more than 2^8.  A row's scores are in registers at once, so the next block's are
+//                    computed meanwhile.
 //   warps 16-19      bring the codes: bulk copies of whole blocks a few blocks ahead into a ring, from there exact conversion to
 //                    halves and stores into the 128-byte-swizzled operand tiles (keys K-major, values MN-major).  The block that two row
 //                    tiles share is converted once.
-//   warps 20-23      issue the MMAs, one warp a stream: S = Q K^T (M 128, N 64, K 64), and when the probabilities are there O += P V (P
-//                    from TMEM), then the next block's scores.
+//   warps 20-23      issue the MMAs, one warp a stream: the next block's S = Q K^T (M 128, N 64, K 64) as soon as this one's scores have been read, and
+//                    O += P V when the probabilities are there.
 // A block's key scale multiplies its scores.  Its value scale goes into the probabilities, relative to the largest one of the keys that the CTA
 // visits: p' = p * scale / largest * 2^7 (2^7: halves keep all their bits down to p = 2^-21 of the row's maximum; p' <= 2^15).
 //
-// Bound by the softmax warps' issue slots and the exponentials (16 a clock and SM).  Two streams of 128 keys a step, eight softmax warps an SM, took
-// 2.0 us for 256 rows x 128 keys: eight warps do not cover each other's latencies.
+// Bound by the softmax warps' issue slots (60 % used) and the exponentials (16 a clock and SM, 49 %): 0.85 us for 256 rows and a block of keys, 730 TFLOP/s
+// of the chip, after 13 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.9 us.  Before: two streams of 128
+// keys a step, eight softmax warps an SM, 2.0 us for 256 rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
+// 77.8 us for the whole.
 // Few tiles over many keys are split over the CTAs of a cluster; partial results, of streams and of CTAs, meet in (distributed) shared memory.
 #include "cached_attention.h"
 
@@ -49,7 +52,7 @@ constexpr int kTile = 64 * 128;          // 64 rows of 64 halves
 constexpr int kTmemCols = 512;
 constexpr int kColS = 0, kColO = 256;    // 4 x 64 scores, 4 x 64 outputs
 constexpr float kRescaleThreshold = 8.0f;
-constexpr int kPolyEvery = 8;            // pairs; 256 rows, 64 blocks: 81.8 us, with 4 83.6, with none 82.5
+constexpr int kPolyEvery = 8;            // pairs; 256 rows, 64 blocks: 73.4 us, with 4 78.6, 6 74.3, 16 76.2
 constexpr float kShift = 7.0f;           // p' is 2^7 times larger than p * scale / largest scale
 // 16 x 96 + 4 x 56 + 4 x 40 = 24 x 80 registers a lane, what the launch has
 constexpr int kRegsSoftmax = 96, kRegsBring = 56, kRegsIssue = 40;
@@ -129,8 +132,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& sm = *reinterpret_cast<Smem*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  RT_PDL_LAUNCH_DEPENDENTS();
   RT_PDL_WAIT();
+  RT_PDL_LAUNCH_DEPENDENTS();
   // ---- what this CTA works on; the same for all CTAs of a cluster but for the keys.  Tiles that see most start first.
   const int rank = blockIdx.x % a.splits;
   const int head = blockIdx.x / a.splits % a.cache.heads;
@@ -369,7 +372,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     // ---------------------------------------------------------------- softmax
     reg_alloc<kRegsSoftmax>();
     // With 64 rows or less the operand tile holds them twice or four times, and each stream has the softmax of another copy: a warp reaches
-    // the TMEM lanes of its own scheduler only, and with one copy the same scheduler would do all streams' rows (12 x 4096 keys, 12 heads, 64 rows: 57 us, now 39.8).
+    // the TMEM lanes of its own scheduler only, and with one copy the same scheduler would do all streams' rows (12 x 4096 keys, 12 heads,
+    // 64 rows: 57 us, now 39.0).
     const int x = warp >> 2, r = tid & 127, span = here > 64 ? 128 : here > 32 ? 64 : 32, own_r = r & (span - 1);
     const bool owner = two || r / span == x * 32 / span;
     const int row = row0 + (two ? (x >> 1) * 128 : 0) + own_r;

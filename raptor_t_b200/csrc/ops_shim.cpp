@@ -235,9 +235,10 @@ Tensor token_logprobs_backward(const Tensor& logits, OptTensor targets, const Te
   Tensor d;
   if (out) {
     d = *out;
-  } else {  // the logits' own row pitch: rows then have the same alignment
-    d = empty({z.rows, z.pitch}, logits.scalar_type(), device);
-    if (z.pitch != z.vocab) d = d.narrow(1, 0, z.vocab);
+  } else {  // as few spare columns as give the rows the alignment of the logits' own
+    const int64_t pitch = z.vocab + (z.pitch - z.vocab) % (16 / logits.element_size());
+    d = empty({z.rows, pitch}, logits.scalar_type(), device);
+    if (pitch != z.vocab) d = d.narrow(1, 0, z.vocab);
   }
   if (d.sizes() != logits.sizes() || index_of(d) != device) throw py::value_error("out: expected the logits' shape and device");
   if (d.scalar_type() != logits.scalar_type())

@@ -94,6 +94,7 @@ __device__ __forceinline__ void ex2_fma_pair(float x0, float x1, float& r0, floa
 constexpr int kPolyEvery = 4;  // measured: 3 and 4 are equal within noise, 2 is slower (issue slots)
 template <bool BF16, int N, int EVERY = kPolyEvery>
 __device__ __forceinline__ float exp_columns(const uint32_t* s, uint32_t* p, float scale_log2, float m_ref) {
+  static_assert(EVERY > 0, "every how many pairs");
   const unsigned long long c2 = f2_pack(scale_log2, scale_log2);
   const unsigned long long nm2 = f2_pack(-m_ref, -m_ref);
   unsigned long long acc0 = 0ull, acc1 = 0ull;  // two packed partial sums (+0.0f, +0.0f)
