@@ -232,6 +232,7 @@ struct RowTile {
     }
     // keys 2 t, + 1, + 8, + 9 of key tile i, dimensions 8 g .. 8 g + 7.  With 16 rows a tile they are read as they are needed: all at once
     // would not fit the registers.
+    const int held = k_scale < 0.f ? 0 : ctx;
     uint2 vw[NT == 1 ? 16 : 4];
     const uint8_t* vp = values();
     if (!vp) return false;
@@ -240,7 +241,7 @@ struct RowTile {
       for (int e = 0; e < 4; ++e) {
         const int row = 16 * i + 2 * t + ((e & 1) ^ odd) + 4 * (e & 2);
         w[e] = *reinterpret_cast<const uint2*>(vp + row * 64 + 8 * g);
-        if (!INT8 && b * 64 + row >= ctx) w[e] = make_uint2(0, 0);  // places that hold no token may hold the code NaN
+        if (!INT8 && b * 64 + row >= held) w[e] = make_uint2(0, 0);  // places that hold no token may hold the code NaN
       }
     };
     if constexpr (NT == 1) {

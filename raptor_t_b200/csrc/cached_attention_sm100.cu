@@ -337,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     auto values = [&](int j) {
       const int s = j % kStages;
       if (!wait(&sm.raw_v[own], nv & 1, 324) || !wait(&sm.v_empty[s], ((j / kStages) & 1) ^ 1, 318)) return false;
-      convert(Values(), sm.v[s], raw + kBlock, INT8 ? 64 : sr.ctx - (j0 + j) * 64);
+      convert(Values(), sm.v[s], raw + kBlock, INT8 ? 64 : sm.scales[j % kRing].x < 0.f ? 0 : sr.ctx - (j0 + j) * 64);
       ++nv;
       if (lane == 0) {
         mbar_arrive(&sm.v_full[s]);

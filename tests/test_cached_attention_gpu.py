@@ -165,6 +165,28 @@ def test_bad_indexes_are_reported(ops):
     ops.check_device()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [1, 12, 40, 150, 300])
+def test_a_bad_entry_leaves_out_its_keys(ops, fmt, rows):
+    """Whatever the block holds that is read in its place."""
+    from raptor_t_b200.capi import RtError
+    g = torch.Generator().manual_seed(5)
+    cache = _filled(g, ops, 6, 2, fmt)
+    cache.k_scale.mul_(2.0 ** -2)
+    k, v = ((c.cpu().double() * s.cpu().double()[:, :, None, None]) for c, s in ((cache.k, cache.k_scale), (cache.v, cache.v_scale)))
+    for c in (cache.k, cache.v):
+        c.view(torch.uint8)[0] = 0x7f
+    for s in (cache.k_scale, cache.v_scale):
+        s[0] = float("nan")
+    q = torch.randn(rows, 2, 64, generator=g).half().cuda()
+    got = ops.cached_attention(q, cache, _i32([[4, -1, 2, 6, 1]]), _i32([300]), _i32([0, rows]), scale=0.125)
+    with pytest.raises(RtError):
+        ops.check_device()
+    # keys of the entries 4, 2 and the 44 tokens of 1
+    want, vmax = ref.attention(q.cpu().double(), k, v, [[4, 2, 1]], [172], [0, rows], 1, 0.125, False)
+    assert ((got.cpu().double() - want).abs() <= _tolerance(want, vmax, 172, torch.float16)).all()
+
+
 def test_two_streams_and_a_captured_graph(ops):
     """Calls on two streams at once, and replays with contexts that have grown, give what one call after the other gives."""
     g = torch.Generator().manual_seed(6)
