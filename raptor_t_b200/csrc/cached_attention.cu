@@ -567,17 +567,17 @@ int splits_of(int64_t units, int tile_rows, int64_t keys) {
   return splits;
 }
 
-// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 13 us and 0.85 us a block of keys (10 and 0.51
-// for at most 128 rows, 0.45 for at most 64), 1 us more where a cluster joins its results.  Clusters of 2, 4 and 8 fit 74, 33 and 15 times on the chip.
+// The same for the kernel of many rows, one CTA an SM: rounds of CTAs times the measured cost of one, 12 us and 0.85 us a block of keys (9 and 0.51
+// for at most 128 rows, 0.45 for at most 64), 0.5 us more where a cluster joins its results.  Clusters of 2, 4 and 8 fit 74, 33 and 15 times on the chip.
 int many_rows_splits(int64_t units, int rows, int64_t keys, double* us) {
   constexpr int kFit[4] = {kSms, 74, 33, 15};
-  const double base = rows > 128 ? 13.0 : 10.0, block = rows > 128 ? 0.85 : rows > 64 ? 0.51 : 0.45, blocks = static_cast<double>((keys + 63) / 64);
+  const double base = rows > 128 ? 12.0 : 9.0, block = rows > 128 ? 0.85 : rows > 64 ? 0.51 : 0.45, blocks = static_cast<double>((keys + 63) / 64);
   int best = 1;
   double least = 1e30;
   for (int k = 0; k < 4; ++k) {
     const int splits = 1 << k;
     const double rounds = static_cast<double>((units + kFit[k] - 1) / kFit[k]);
-    const double cost = rounds * (base + (k > 0 ? 1.0 : 0.0) + block * blocks / splits);
+    const double cost = rounds * (base + (k > 0 ? 0.5 : 0.0) + block * blocks / splits);
     if (cost < least) {
       least = cost;
       best = splits;

@@ -18,7 +18,7 @@
 // visits: p' = p * scale / largest * 2^7 (2^7: halves keep all their bits down to p = 2^-21 of the row's maximum; p' <= 2^15).
 //
 // Bound by the softmax warps' issue slots (60 % used) and the exponentials (16 a clock and SM, 49 %): 0.85 us for 256 rows and a block of keys, 730 TFLOP/s
-// of the chip, after 13 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.9 us.  Before: two streams of 128
+// of the chip, after 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.2 us.  Before: two streams of 128
 // keys a step, eight softmax warps an SM, 2.0 us for 256 rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
 // 77.8 us for the whole.
 // Few tiles over many keys are split over the CTAs of a cluster; partial results, of streams and of CTAs, meet in (distributed) shared memory.
@@ -70,7 +70,6 @@ struct Smem {
   float2 scales[kRing];  // key and value scale of a block; a negative key scale: nobody sees its keys
   float2 ml[kStreams][128];
   float2 ml_cta[256];
-  float weight[kStreams][128];
   float vmax[kSoftmaxThreads / 32];
   int cost[kThreads + 1];
   uint32_t tmem_slot;
@@ -373,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     reg_alloc<kRegsSoftmax>();
     // With 64 rows or less the operand tile holds them twice or four times, and each stream has the softmax of another copy: a warp reaches
     // the TMEM lanes of its own scheduler only, and with one copy the same scheduler would do all streams' rows (12 x 4096 keys, 12 heads,
-    // 64 rows: 57 us, now 39.0).
+    // 64 rows: 57 us, now 38.5).
     const int x = warp >> 2, r = tid & 127, span = here > 64 ? 128 : here > 32 ? 64 : 32, own_r = r & (span - 1);
     const bool owner = two || r / span == x * 32 / span;
     const int row = row0 + (two ? (x >> 1) * 128 : 0) + own_r;
@@ -541,74 +540,100 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     }
     const bool any = ok && c > 0 && live;  // there is an output tile to read; the same for the whole warp
     softmax_barrier();  // all streams have seen their last block: operand tiles and ring are free
-    if (owner) {
-      float* part = reinterpret_cast<float*>(sm.k) + x * 128 * 64 + own_r * 64;
-      sm.ml[x][own_r] = make_float2(any ? m_ref : -INFINITY, any ? l : 0.f);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint32_t o[32];
+    // ---- the streams of a row tile: each finishes its share of the dimensions, and leaves the others' in shared memory for them
+    auto part_of = [&](int stream) { return reinterpret_cast<float*>(sm.k) + (stream * 128 + own_r) * 64; };
+    auto quad_at = [&](int quad) { return (quad ^ (own_r & 15)) << 2; };
+    auto join = [&](auto count) {
+      constexpr int N = decltype(count)::value, D = 64 / N, Q = D / 4;  // streams, dimensions of a share, their quads
+      const int y = first_of(x), x0 = x - y;
+      auto load = [&](int share, uint32_t* o) {
         if (any) {
-          tmem_ld32(to + 32 * h, o);
+          if constexpr (D == 32) tmem_ld32(to + share * D, o);
+          else tmem_ld16(to + share * D, o);
           tc_wait_ld();
         } else {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0u;
+          for (int k = 0; k < D; ++k) o[k] = 0u;
         }
+      };
+      if (owner) {
+        sm.ml[x][own_r] = make_float2(any ? m_ref : -INFINITY, any ? l : 0.f);
 #pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<uint4*>(part + (((8 * h + q) ^ (r & 15)) << 2)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        for (int s = 1; s < N; ++s) {
+          const int share = (y + s) % N;
+          uint32_t o[D];
+          load(share, o);
+#pragma unroll
+          for (int q = 0; q < Q; ++q)
+            *reinterpret_cast<uint4*>(part_of(x) + quad_at(share * Q + q)) = make_uint4(o[4 * q], o[4 * q + 1], o[4 * q + 2], o[4 * q + 3]);
+        }
       }
-    }
-    softmax_barrier();
-    // ---- the streams of this CTA: a weight for each row and stream, then four dimensions of a row a thread
-    const int streams = two ? 2 : 4;
-    if (tid < here) {
-      const int x0 = two ? (tid >> 7) * 2 : 0, pr = tid & 127;
-      float M = -INFINITY, L = 0.f;
-      for (int y = 0; y < streams; ++y) M = max_nan(M, sm.ml[x0 + y][pr].x);
-      float f[kStreams];
+      softmax_barrier();
+      if (!owner) return;
+      uint32_t o[D];
+      load(y, o);
+      float M = -INFINITY, L = 0.f, f[N];
 #pragma unroll
-      for (int y = 0; y < kStreams; ++y) {
-        if (y >= streams) continue;
-        const float2 ml = sm.ml[x0 + y][pr];
-        f[y] = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-        L = fmaf(ml.y, f[y], L);
+      for (int s = 0; s < N; ++s) M = max_nan(M, sm.ml[x0 + s][own_r].x);
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        const float2 ml = sm.ml[x0 + s][own_r];
+        f[s] = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
+        L = fmaf(ml.y, f[s], L);
       }
       const float unit_o = vref * Values::kUnit * 0.0078125f;  // 2^-kShift
       const float w = a.splits > 1 ? unit_o : M == -INFINITY ? 0.f : unit_o / L;
+      float v[D];
+      float own = 0.f;
 #pragma unroll
-      for (int y = 0; y < kStreams; ++y)
-        if (y < streams) sm.weight[x0 + y][pr] = f[y] * w;
-      if (a.splits > 1) sm.ml_cta[tid] = make_float2(M, L);
-    }
-    softmax_barrier();
+      for (int s = 0; s < N; ++s) {
+        f[s] *= w;
+        if (s == y) own = f[s];
+      }
+#pragma unroll
+      for (int k = 0; k < D; ++k) v[k] = __uint_as_float(o[k]) * own;
+#pragma unroll
+      for (int s = 0; s < N; ++s) {
+        if (s == y) continue;
+#pragma unroll
+        for (int q = 0; q < Q; ++q) {
+          const float4 t = *reinterpret_cast<const float4*>(part_of(x0 + s) + quad_at(y * Q + q));
+          v[4 * q] = fmaf(t.x, f[s], v[4 * q]);
+          v[4 * q + 1] = fmaf(t.y, f[s], v[4 * q + 1]);
+          v[4 * q + 2] = fmaf(t.z, f[s], v[4 * q + 2]);
+          v[4 * q + 3] = fmaf(t.w, f[s], v[4 * q + 3]);
+        }
+      }
+      if (a.splits > 1) {
+        if (y == 0) sm.ml_cta[(two ? (x >> 1) * 128 : 0) + own_r] = make_float2(M, L);
+#pragma unroll
+        for (int q = 0; q < Q; ++q)  // over what this thread has read
+          *reinterpret_cast<float4*>(part_of(x0) + quad_at(y * Q + q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+      } else {  // through the same places, so that a store covers whole sectors of few lines
+        constexpr int C = D / 8;
+#pragma unroll
+        for (int q = 0; q < C; ++q)
+          *reinterpret_cast<uint4*>(part_of(x0) + quad_at(y * Q + q)) = make_uint4(pack2<BF16>(v[8 * q], v[8 * q + 1]), pack2<BF16>(v[8 * q + 2], v[8 * q + 3]),
+                                                                                 pack2<BF16>(v[8 * q + 4], v[8 * q + 5]), pack2<BF16>(v[8 * q + 6], v[8 * q + 7]));
+        __syncwarp();
+        const int from = lane / C, q = lane % C;
+        RowWalk at(row - lane + from, 32 / C, a.group);
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int rr = own_r - lane + from + 32 / C * i;
+          const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(sm.k) + (x0 * 128 + rr) * 64 + (((y * Q + q) ^ (rr & 15)) << 2));
+          if (row - lane + from + 32 / C * i < row0 + here)
+            reinterpret_cast<uint4*>(a.out + (static_cast<int64_t>(sr.f0 + at.token) * a.heads + head * a.group + at.member) * 64 + y * D)[q] = t;
+          at.next();
+        }
+      }
+    };
+    if (two) join(std::integral_constant<int, 2>());
+    else join(std::integral_constant<int, 4>());
     auto store = [&](const RowWalk& to, int d, const float4& v) {
       *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(sr.f0 + to.token) * a.heads + head * a.group + to.member) * 64 + d) =
           make_uint2(pack2<BF16>(v.x, v.y), pack2<BF16>(v.z, v.w));
     };
-    auto merge = [&](auto count) {
-      constexpr int N = decltype(count)::value;
-      RowWalk to(row0 + (tid >> 4), kSoftmaxThreads / 16, a.group);
-#pragma unroll 4
-      for (int i = tid; i < here * 16; i += kSoftmaxThreads, to.next()) {
-        const int rr = i >> 4, quad = i & 15, x0 = N == 2 ? (rr >> 7) * 2 : 0, pr = rr & 127;
-        float* at = reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2);
-        float4 v = make_float4(0, 0, 0, 0);
-#pragma unroll
-        for (int y = 0; y < N; ++y) {
-          const float w = sm.weight[x0 + y][pr];
-          const float4 o = *reinterpret_cast<const float4*>(at + y * 128 * 64);
-          v.x = fmaf(o.x, w, v.x);
-          v.y = fmaf(o.y, w, v.y);
-          v.z = fmaf(o.z, w, v.z);
-          v.w = fmaf(o.w, w, v.w);
-        }
-        if (a.splits == 1) store(to, 4 * quad, v);
-        else *reinterpret_cast<float4*>(at) = v;
-      }
-    };
-    if (two) merge(std::integral_constant<int, 2>());
-    else merge(std::integral_constant<int, 4>());
     // ... then the CTAs of the cluster, each of which finishes its share of the tile; all parts are requested before one is used
     if (a.splits > 1) {
       __syncwarp();
