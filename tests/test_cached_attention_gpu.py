@@ -257,3 +257,19 @@ def test_a_run_together(ops):
         assert torch.equal(got.top_ids.long(), torch.sort(logits.float(), dim=1, descending=True, stable=True).indices[:, :4])
         x = emb[got.top_ids[:, 0].long()] * 4
     ops.check_device()
+
+
+@pytest.mark.parametrize("seed", range(10))
+def test_random_calls(ops, seed):
+    """Heads in groups of any size, ragged rows and contexts on both sides of every rule that chooses a kernel or a split."""
+    import random
+    rng = random.Random(seed)
+    for _ in range(6):
+        group, kv_heads, n = rng.choice([1, 1, 2, 3, 5, 7, 13]), rng.choice([1, 2, 3]), rng.choice([1, 1, 2, 3, 9, 40])
+        most = max(1, int(2 ** rng.uniform(0, 10 if n < 9 else 6)) // group)
+        counts = [rng.choice([most, rng.randint(0, most), rng.randint(1, most)]) for _ in range(n)]
+        context = [rng.choice([0, 1, rng.randint(1, 64), int(2 ** rng.uniform(5, 11))]) if rng.random() < 0.9 else c for c in counts]
+        if sum(counts) == 0:
+            continue
+        _case(ops, rng.choice(FORMATS), rng.choice(DTYPES), group * kv_heads, kv_heads, counts, context, rng.random() < 0.5,
+              spare_rows=rng.randint(0, 3), seed=seed)

@@ -278,3 +278,18 @@ def test_two_graphs_and_streams(ops):
     torch.cuda.synchronize()
     for _, r, b in graphs:
         assert all(torch.equal(x, y) for x, y in zip(r, want)) and torch.equal(b, d)
+
+
+def test_rows_far_apart(ops):
+    """Row offsets past 32 bits, read and written."""
+    vocab, pitch = 1000, 2300000001
+    z = torch.as_strided(torch.empty(2 * pitch + vocab, dtype=torch.float16, device="cuda"), (3, vocab), (pitch, 1))
+    x, t = _rows(3, vocab, torch.float16)
+    z.copy_(x)
+    got = ops.token_logprobs(z, t, top_k=4)
+    _check_forward(got, z, t, 4)
+    g = torch.ones(3, device="cuda")
+    want = ops.token_logprobs_backward(x, t, got.stats, grad_logp=g)
+    assert torch.equal(ops.token_logprobs_backward(z, t, got.stats, grad_logp=g, out=z), want)
+    assert torch.equal(z, want)
+    ops.check_device()
