@@ -163,13 +163,13 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
 }
 
 // grid: (block of the sequence, head) pairs of every sequence; warps 0 and 1 take the keys, 2 and 3 the values, 32 tokens each.
-// A tile is read once, and its largest value is known before the first code is: it stays in registers.  Two warps for a tile keep 32
-// warps an SM at that.  8 sequences of 1024 to 4096 tokens, 12 heads, f16 to int8 (95 MB): 20.0 us, 4.8 TB/s, bound by HBM and a CTA's chain of
-// index, load, maximum, store; one warp a tile, quotients by division and maxima in fp32 took 67.7.  A step's tokens (32 sequences, 12 heads) are that
+// A tile is read once, and its largest value is known before the first code is: it stays in registers.  Two warps for a tile keep 36
+// warps an SM at that (32: 19.9 us, 40: 21.3, they spill).  8 sequences of 1024 to 4096 tokens, 12 heads, f16 to int8 (95 MB): 19.2 us, 5.0 TB/s, bound by
+// HBM and a CTA's chain of index, load, maximum, store; one warp a tile, quotients by division and maxima in fp32 took 67.7.  A step's tokens (32 sequences, 12 heads) are that
 // chain alone, 2.8 us.
 constexpr int kWriteThreads = 128;
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(kWriteThreads, 8)
+__global__ void __launch_bounds__(kWriteThreads, 9)
 kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t token_stride, int64_t head_stride,
                 const int32_t* __restrict__ table, int table_stride, const int32_t* __restrict__ start,
                 const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
@@ -272,7 +272,7 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
 
 // The same grid and warps; out_k / out_v are token-major [tokens][heads * 64].  Bound by HBM: 249 MB in 42.4 us, 5.9 TB/s.
 template <bool BF16, bool INT8>
-__global__ void __launch_bounds__(kWriteThreads, 8)
+__global__ void __launch_bounds__(kWriteThreads, 9)
 kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, const int32_t* __restrict__ table,
                int table_stride, const int32_t* __restrict__ start, const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
   RT_PDL_WAIT();
