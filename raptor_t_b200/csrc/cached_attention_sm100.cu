@@ -14,8 +14,10 @@
 //                    tiles share is converted once.
 //   warps 20-23      issue the MMAs, one warp a stream: the next block's S = Q K^T (M 128, N 64, K 64) as soon as this one's scores have been read, and
 //                    O += P V when the probabilities are there.
-// A block's key scale multiplies its scores.  Its value scale goes into the probabilities, relative to the largest one of the keys that the CTA
-// visits: p' = p * scale / largest * 2^7 (2^7: halves keep all their bits down to p = 2^-21 of the row's maximum; p' <= 2^15).
+// A block's key scale multiplies its scores.  Its value scale goes into the probabilities as an exponent, p' = 2^(score + log2 scale - R + 7), with
+// R the row's own running maximum of score + log2 scale: halves keep all their bits down to 2^-21 of what counts most in the row's output, whatever
+// scales other rows see (2^7; p' <= 2^15).  The sum of the probabilities has the running maximum M of the scores as its reference and is taken from the
+// same exponentials, times 2^(R - M - log2 scale - 7); out = O 2^(R - M - 7) / sum.
 //
 // Bound by the softmax warps' issue slots (60 % used) and the exponentials (16 a clock and SM, 49 %): 0.85 us for 256 rows and a block of keys, 730 TFLOP/s
 // of the chip, after 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.2 us.  Before: two streams of 128
@@ -53,7 +55,8 @@ constexpr int kTmemCols = 512;
 constexpr int kColS = 0, kColO = 256;    // 4 x 64 scores, 4 x 64 outputs
 constexpr float kRescaleThreshold = 8.0f;
 constexpr int kPolyEvery = 8;            // pairs; 256 rows, 64 blocks: 73.4 us, with 4 78.6, 6 74.3, 16 76.2
-constexpr float kShift = 7.0f;           // p' is 2^7 times larger than p * scale / largest scale
+constexpr float kShift = 7.0f;           // p' is 2^7 times larger than its share of the output
+constexpr float kApart = 64.0f;          // p' of a block from which its sum is taken by itself
 // 16 x 96 + 4 x 56 + 4 x 40 = 24 x 80 registers a lane, what the launch has
 constexpr int kRegsSoftmax = 96, kRegsBring = 56, kRegsIssue = 40;
 
@@ -67,10 +70,11 @@ struct Smem {
   uint64_t raw_k[kRaw], raw_v[kRaw];
   uint64_t q_full[2], k_full[kStages], k_empty[kStages], v_full[kStages], v_empty[kStages];
   uint64_t s_full[kStreams], s_free[kStreams], p_full[kStreams], o_full[kStreams];
-  float2 scales[kRing];  // key and value scale of a block; a negative key scale: nobody sees its keys
-  float2 ml[kStreams][128];
+  float2 scales[kRing];  // of a block: key scale, base-2 logarithm of the value scale; a negative key scale: nobody sees its keys
+  float2 ml[kStreams][128];  // M and sum of a row
+  float ref[kStreams][128];  // R
   float2 ml_cta[256];
-  float vmax[kSoftmaxThreads / 32];
+  float ref_cta[256];
   int cost[kThreads + 1];
   uint32_t tmem_slot;
   int abort_flag;
@@ -282,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       const bool bad = page < 0 || page >= a.cache.blocks;
       if (bad) kv::index_error(a.err, kSiteCachedAttention);
       const int64_t slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
-      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], a.cache.v_scale[slot]);
+      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], __log2f(a.cache.v_scale[slot]));
       return slot;
     };
     auto request = [&](uint8_t* dst, const uint8_t* base, int64_t slot, uint64_t* bar) {
@@ -382,8 +386,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const int wmin = __reduce_min_sync(0xffffffffu, lim), wmax = __reduce_max_sync(0xffffffffu, lim);
     // ---- the query rows, as halves.  Eight lanes a row, so that a load covers whole lines (a row a lane took 4 us).  The streams of a row tile share
     // its operand tile; each brings its part of the rows and leaves a row's unit and bias for the others.
-    const int page0 = tid < n_blocks ? __ldg(table + tid) : -1;
-    float vref = 0.f;  // the largest value scale of the keys visited here
     float2* found = sm.ml_cta + (two ? (x >> 1) * 128 : 0);
     {
       // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
@@ -400,7 +402,6 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           t[i] = __ldg(reinterpret_cast<const uint4*>(a.q + (sr.f0 + at.token) * a.q_stride + (head * a.group + at.member) * 64) + chunk);
         at.next();
       }
-      if (page0 >= 0 && page0 < a.cache.blocks) vref = a.cache.v_scale[static_cast<int64_t>(page0) * a.cache.heads + head];
       uint8_t* tile_q = sm.q[two ? x >> 1 : 0];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -439,24 +440,13 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.q_full[two ? x >> 1 : 0]);
     }
-    for (int b = tid + kSoftmaxThreads; b < n_blocks; b += kSoftmaxThreads) {
-      const int page = __ldg(table + b);
-      if (page >= 0 && page < a.cache.blocks) vref = fmaxf(vref, a.cache.v_scale[static_cast<int64_t>(page) * a.cache.heads + head]);
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) vref = fmaxf(vref, __shfl_xor_sync(0xffffffffu, vref, o));
-    if (lane == 0) sm.vmax[warp] = vref;
     softmax_barrier();
     const float unit = found[r].x, bias = found[r].y;  // a score in base 2 is (product - bias) * unit * key scale
-#pragma unroll
-    for (int i = 0; i < kSoftmaxThreads / 32; ++i) vref = fmaxf(vref, sm.vmax[i]);
-    if (!(vref > 0.f)) vref = 1.f;
-    const float inv_vref = 1.f / vref;
 
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + x * 64, to = tmem + lanes + kColO + x * 64;
     uint8_t* p_row = sm.p[x] + r * 128;
-    float m_ref = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, ref = -INFINITY;
     bool ok = true;
     uint32_t c = 0;
     const int end = end_of(x);
@@ -481,20 +471,28 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           for (int i = 0; i < 64; ++i)
             if (i >= left) s[i] = 0xff800000u;
         }
+        const bool sees = lim > key0;  // a row that sees no key of the block is not touched by its scales
         const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
         const float off = bias * c0, m_new = max64(s) * c0 - off;
+        const float log_v = sees ? sc.y : 0.f, most = m_new + log_v;
+        const float m_was = m;
+        m = max_nan(m, m_new);
+        const float m_here = m == -INFINITY ? 0.f : m;
+        l *= ex2(m_was - m_here);
         float alpha = 1.f;
         bool fix = false;
-        if (m_ref == -INFINITY) {
-          m_ref = m_new;
-        } else if (m_new > m_ref + kRescaleThreshold) {
-          alpha = ex2(m_ref - m_new);
-          m_ref = m_new;
+        if (ref == -INFINITY) {  // no output yet, or none but zeros
+          ref = most;
+        } else if (most > ref + kRescaleThreshold) {
+          alpha = ex2(ref - most);
+          ref = most;
           fix = true;
         }
-        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-        const float e0 = __log2f(fmaxf(sc.y * inv_vref, 8.7e-19f)) + kShift;
-        l *= alpha;
+        const float ref_here = ref == -INFINITY ? 0.f : ref;
+        // Where the block's values are that much smaller than what the row has seen, its probabilities still count in the sum.
+        const bool apart = ref_here - most > kApart && m_new > m - kApart;
+        const bool any_apart = __any_sync(0xffffffffu, apart);
+        const float e0 = log_v + kShift;
         // the product of the step before is done: its probabilities may be written over, and the output tile is at rest
         if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 321);
         if (!ok) break;
@@ -513,11 +511,17 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           tc_fence_before_sync();
         }
         // half a row at a time: the registers hold 64 scores and 32 packed probabilities at once no more than barely
-        const float back = ex2(-e0);
+        float back = ex2(fminf(ref_here - m_here - e0, kApart));  // more than that: the block does not count in the sum
+        if (any_apart) {
+          uint32_t p[16];
+          l += exp_columns<false, 32, kPolyEvery>(s, p, c0, m_here + off);
+          l += exp_columns<false, 32, kPolyEvery>(s + 32, p, c0, m_here + off);
+          back = 0.f;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[16];
-          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref - e0 + off), back, l);
+          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref_here - e0 + off), back, l);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint4*>(p_row + (((4 * h + i) ^ (r & 7)) << 4)) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
@@ -543,6 +547,13 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     // ---- the streams of a row tile: each finishes its share of the dimensions, and leaves the others' in shared memory for them
     auto part_of = [&](int stream) { return reinterpret_cast<float*>(sm.k) + (stream * 128 + own_r) * 64; };
     auto quad_at = [&](int quad) { return (quad ^ (own_r & 15)) << 2; };
+    // of a partial result with reference x among results whose largest reference is `most`
+    auto weight = [](float x, float most) { return x == -INFINITY ? 0.f : ex2(x - most); };
+    // of the outputs with reference R; 2^(R - M) in two steps, since it may be as large as a value
+    auto factor = [](float R, float M, float L) {
+      const float half = ex2(0.5f * (R - M));
+      return L == 0.f ? 0.f : Values::kUnit * 0.0078125f / L * half * half;  // 2^-kShift
+    };
     auto join = [&](auto count) {
       constexpr int N = decltype(count)::value, D = 64 / N, Q = D / 4;  // streams, dimensions of a share, their quads
       const int y = first_of(x), x0 = x - y;
@@ -557,7 +568,8 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         }
       };
       if (owner) {
-        sm.ml[x][own_r] = make_float2(any ? m_ref : -INFINITY, any ? l : 0.f);
+        sm.ml[x][own_r] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
+        sm.ref[x][own_r] = any ? ref : -INFINITY;
 #pragma unroll
         for (int s = 1; s < N; ++s) {
           const int share = (y + s) % N;
@@ -572,17 +584,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       if (!owner) return;
       uint32_t o[D];
       load(y, o);
-      float M = -INFINITY, L = 0.f, f[N];
+      float M = -INFINITY, R = -INFINITY, L = 0.f, f[N];
 #pragma unroll
-      for (int s = 0; s < N; ++s) M = max_nan(M, sm.ml[x0 + s][own_r].x);
+      for (int s = 0; s < N; ++s) {
+        M = max_nan(M, sm.ml[x0 + s][own_r].x);
+        R = max_nan(R, sm.ref[x0 + s][own_r]);
+      }
 #pragma unroll
       for (int s = 0; s < N; ++s) {
         const float2 ml = sm.ml[x0 + s][own_r];
-        f[s] = ml.x == -INFINITY ? 0.f : ex2(ml.x - M);
-        L = fmaf(ml.y, f[s], L);
+        L = fmaf(ml.y, weight(ml.x, M), L);
+        f[s] = weight(sm.ref[x0 + s][own_r], R);
       }
-      const float unit_o = vref * Values::kUnit * 0.0078125f;  // 2^-kShift
-      const float w = a.splits > 1 ? unit_o : M == -INFINITY ? 0.f : unit_o / L;
+      const float w = a.splits > 1 ? 1.f : factor(R, M, L);
       float v[D];
       float own = 0.f;
 #pragma unroll
@@ -605,7 +619,10 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         }
       }
       if (a.splits > 1) {
-        if (y == 0) sm.ml_cta[(two ? (x >> 1) * 128 : 0) + own_r] = make_float2(M, L);
+        if (y == 0) {
+          sm.ml_cta[(two ? (x >> 1) * 128 : 0) + own_r] = make_float2(M, L);
+          sm.ref_cta[(two ? (x >> 1) * 128 : 0) + own_r] = R;
+        }
 #pragma unroll
         for (int q = 0; q < Q; ++q)  // over what this thread has read
           *reinterpret_cast<float4*>(part_of(x0) + quad_at(y * Q + q)) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -642,34 +659,40 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       RowWalk to(row0 + ((rank * kSoftmaxThreads + tid) >> 4), a.splits * kSoftmaxThreads / 16, a.group);
       for (int i = rank * kSoftmaxThreads + tid; i < here * 16; i += a.splits * kSoftmaxThreads, to.next()) {
         const int rr = i >> 4, quad = i & 15, x0 = two ? (rr >> 7) * 2 : 0, pr = rr & 127;
-        const uint32_t ml_at = smem_u32(&sm.ml_cta[rr]);
+        const uint32_t ml_at = smem_u32(&sm.ml_cta[rr]), ref_at = smem_u32(&sm.ref_cta[rr]);
         const uint32_t o_at = smem_u32(reinterpret_cast<float*>(sm.k) + (x0 * 128 + pr) * 64 + ((quad ^ (pr & 15)) << 2));
         float2 ml[kMaxSplits];
+        float ref[kMaxSplits];
         float4 o[kMaxSplits];
 #pragma unroll
         for (int w = 0; w < kMaxSplits; ++w) {
           ml[w] = make_float2(-INFINITY, 0.f);
+          ref[w] = -INFINITY;
           o[w] = make_float4(0, 0, 0, 0);
           if (w < a.splits) {
             ml[w] = kv::ld_cluster_f2(kv::peer_address(ml_at, w));
+            ref[w] = kv::ld_cluster_f1(kv::peer_address(ref_at, w));
             o[w] = kv::ld_cluster_f4(kv::peer_address(o_at, w));
           }
         }
-        float M = -INFINITY, L = 0.f;
+        float M = -INFINITY, R = -INFINITY, L = 0.f;
 #pragma unroll
-        for (int w = 0; w < kMaxSplits; ++w) M = max_nan(M, ml[w].x);
+        for (int w = 0; w < kMaxSplits; ++w) {
+          M = max_nan(M, ml[w].x);
+          R = max_nan(R, ref[w]);
+        }
         float4 v = make_float4(0, 0, 0, 0);
 #pragma unroll
         for (int w = 0; w < kMaxSplits; ++w) {
-          const float f = ml[w].x == -INFINITY ? 0.f : ex2(ml[w].x - M);
-          L = fmaf(ml[w].y, f, L);
+          const float f = weight(ref[w], R);
+          L = fmaf(ml[w].y, weight(ml[w].x, M), L);
           v.x = fmaf(o[w].x, f, v.x);
           v.y = fmaf(o[w].y, f, v.y);
           v.z = fmaf(o[w].z, f, v.z);
           v.w = fmaf(o[w].w, f, v.w);
         }
-        const float inv = M == -INFINITY ? 0.f : 1.f / L;
-        store(to, 4 * quad, make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv));
+        const float w = factor(R, M, L);
+        store(to, 4 * quad, make_float4(v.x * w, v.y * w, v.z * w, v.w * w));
       }
     }
     if (a.splits > 1) {
