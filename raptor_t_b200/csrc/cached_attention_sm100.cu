@@ -15,9 +15,9 @@
 //   warps 20-23      issue the MMAs, one warp a stream: the next block's S = Q K^T (M 128, N 64, K 64) as soon as this one's scores have been read, and
 //                    O += P V when the probabilities are there.
 // A block's key scale multiplies its scores.  Its value scale goes into the probabilities as an exponent, p' = 2^(score + log2 scale - R + 7), with
-// R the row's own running maximum of score + log2 scale: halves keep all their bits down to 2^-21 of what counts most in the row's output, whatever
-// scales other rows see (2^7; p' <= 2^15).  The sum of the probabilities has the running maximum M of the scores as its reference and is taken from the
-// same exponentials, times 2^(R - M - log2 scale - 7); out = O 2^(R - M - 7) / sum.
+// R the row's own running maximum of score + log2 scale (raised when that has grown by more than 8): halves keep all their bits down to 2^-21 of
+// what counts most in the row's output, whatever scales other rows see (2^7; p' <= 2^15).  The sum of the probabilities has a running maximum M of
+// the scores as its reference and is taken from the same exponentials, times 2^(R - M - log2 scale - 7); out = O 2^(R - M - 7) / sum.
 //
 // Bound by the softmax warps' issue slots (60 % used) and the exponentials (16 a clock and SM, 49 %): 0.85 us for 256 rows and a block of keys, 730 TFLOP/s
 // of the chip, after 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.2 us.  Before: two streams of 128
@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + x * 64, to = tmem + lanes + kColO + x * 64;
     uint8_t* p_row = sm.p[x] + r * 128;
-    float m = -INFINITY, l = 0.f, ref = -INFINITY;
+    float m = -INFINITY, ref = 0.f, gap = 0.f, l = 0.f;  // M, R, R - M - 7, sum
     bool ok = true;
     uint32_t c = 0;
     const int end = end_of(x);
@@ -475,28 +475,31 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
         const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
         const float off = bias * c0, m_new = max64(s) * c0 - off;
         const float log_v = sees ? sc.y : 0.f, most = m_new + log_v;
-        const float m_was = m;
-        m = max_nan(m, m_new);
-        const float m_here = m == -INFINITY ? 0.f : m;
-        l *= ex2(m_was - m_here);
         float alpha = 1.f;
-        bool fix = false;
-        if (ref == -INFINITY) {  // no output yet, or none but zeros
-          ref = most;
-        } else if (most > ref + kRescaleThreshold) {
-          alpha = ex2(ref - most);
-          ref = most;
-          fix = true;
+        bool fixes = false, apart = false;
+        const bool grown = !(m_new <= m + kRescaleThreshold), more = !(most <= ref + kRescaleThreshold);
+        if (__any_sync(0xffffffffu, grown || more || gap - log_v > kApart)) {
+          const bool none = m == -INFINITY;  // no output yet
+          if (grown) {
+            l *= none ? 0.f : ex2(m - m_new);
+            m = m_new;
+          }
+          if (none || more) {
+            // with value scales of 0 there is an output, but nothing in it: any other scale raises R
+            const float to = m == -INFINITY ? 0.f : most == -INFINITY ? m - 1000.f : most;
+            if (!none) alpha = ex2(ref - to);
+            ref = to;
+          }
+          gap = m == -INFINITY ? 0.f : ref - m - kShift;
+          // Where the block's values are that much smaller than what the row has seen, its probabilities still count in the sum: they are taken
+          // relative to M, and what they do to the output, nothing, is written over them.
+          apart = m != -INFINITY && gap - log_v > kApart;
+          fixes = __any_sync(0xffffffffu, !none && more);
         }
-        const float ref_here = ref == -INFINITY ? 0.f : ref;
-        // Where the block's values are that much smaller than what the row has seen, its probabilities still count in the sum.
-        const bool apart = ref_here - most > kApart && m_new > m - kApart;
-        const bool any_apart = __any_sync(0xffffffffu, apart);
-        const float e0 = log_v + kShift;
         // the product of the step before is done: its probabilities may be written over, and the output tile is at rest
         if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 321);
         if (!ok) break;
-        if (__any_sync(0xffffffffu, fix) && c > 0) {
+        if (fixes) {
           tc_fence_after_sync();
 #pragma unroll 1
           for (int i = 0; i < 64; i += 16) {
@@ -511,20 +514,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
           tc_fence_before_sync();
         }
         // half a row at a time: the registers hold 64 scores and 32 packed probabilities at once no more than barely
-        float back = ex2(fminf(ref_here - m_here - e0, kApart));  // more than that: the block does not count in the sum
-        if (any_apart) {
-          uint32_t p[16];
-          l += exp_columns<false, 32, kPolyEvery>(s, p, c0, m_here + off);
-          l += exp_columns<false, 32, kPolyEvery>(s + 32, p, c0, m_here + off);
-          back = 0.f;
-        }
+        // (not from `rel`, which may be rounded: what that does to the probabilities goes into sum and output alike)
+        const float rel = apart ? m : ref - kShift - log_v, back = ex2(apart ? 0.f : gap - log_v);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[16];
-          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, ref_here - e0 + off), back, l);
+          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, rel + off), back, l);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint4*>(p_row + (((4 * h + i) ^ (r & 7)) << 4)) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
+        }
+        if (apart) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) *reinterpret_cast<uint4*>(p_row + 16 * i) = make_uint4(0, 0, 0, 0);
         }
       } else {
         if (c > 0) ok = wait(&sm.o_full[x], (c - 1) & 1, 323);
@@ -569,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       };
       if (owner) {
         sm.ml[x][own_r] = make_float2(any ? m : -INFINITY, any ? l : 0.f);
-        sm.ref[x][own_r] = any ? ref : -INFINITY;
+        sm.ref[x][own_r] = any && m != -INFINITY ? ref : -INFINITY;
 #pragma unroll
         for (int s = 1; s < N; ++s) {
           const int share = (y + s) % N;
