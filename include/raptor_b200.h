@@ -276,7 +276,8 @@ rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* k_out_dev, void* v_ou
 /* out[row][head * 64 + d] = softmax(scale * q k^T) v over the cached tokens of the row's sequence.  Sequence s has the query rows
  * first_dev[s] .. first_dev[s + 1] - 1 (at most max_q, none allowed) and context_dev[s] tokens in the cache.  causal = 0: every row
  * sees all of them; 1: the query rows are the sequence's last tokens and row i of n sees the first context - n + i + 1.  A row
- * that sees nothing is 0.  q: 16-bit, element (row, head, d) at row * q_stride + head * 64 + d, q_stride a multiple of 8; out
+ * that sees nothing is 0, whatever its query holds.  Where a scale is NaN, rows that see one of the block's tokens are NaN, and no
+ * other row is touched.  q: 16-bit, element (row, head, d) at row * q_stride + head * 64 + d, q_stride a multiple of 8; out
  * [tokens][heads * 64] must not overlap q.  heads is a multiple of the cache's kv_heads: query head h reads
  * key head h / (heads / kv_heads).  Rows behind the last sequence stay as they are.  max_context (0: as wide as the table) only
  * guides how the work is split, a wrong one costs time. */

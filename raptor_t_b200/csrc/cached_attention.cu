@@ -185,7 +185,9 @@ struct RowTile {
         }
       }
     }
-    // The reference of a row follows its maximum when that has grown by more than 2^8.
+    // The reference of a row follows its maximum when that has grown by more than 2^8.  A row that sees no key of the block is touched neither by
+    // its scales nor by its own query, which may be no numbers.
+    auto blind = [&](int n, int e) { return edge && b * 64 >= lim[n][e]; };
     float u[NT][2], c[NT][2];
     bool grown = false;
 #pragma unroll
@@ -193,7 +195,7 @@ struct RowTile {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         u[n][e] = fmaxf(unit[n][e] * k_scale, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
-        c[n][e] = -bias[n][e] * k_scale;
+        c[n][e] = blind(n, e) ? 0.f : -bias[n][e] * k_scale;
         float x = fmaxf(fmaxf(sc[n][0][e], sc[n][0][e + 2]), fmaxf(sc[n][1][e], sc[n][1][e + 2]));
         x = fmaxf(x, fmaxf(fmaxf(sc[n][2][e], sc[n][2][e + 2]), fmaxf(sc[n][3][e], sc[n][3][e + 2])));
         grown |= fmaf(x, u[n][e], c[n][e]) > m[n][e] + kSlack;
@@ -284,10 +286,10 @@ struct RowTile {
       __syncwarp();
       values_read();
     }
-    const float vs = v_scale * C::kUnit;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const float off0 = -C::kBias * v_scale * sum[n][0], off1 = -C::kBias * v_scale * sum[n][1];
+      const float v0 = blind(n, 0) ? 0.f : v_scale, v1 = blind(n, 1) ? 0.f : v_scale, vs0 = v0 * C::kUnit, vs1 = v1 * C::kUnit;
+      const float off0 = -C::kBias * v0 * sum[n][0], off1 = -C::kBias * v1 * sum[n][1];
       l[n][0] += sum[n][0];
       l[n][1] += sum[n][1];
       if (change) {
@@ -301,10 +303,10 @@ struct RowTile {
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        o[n][j][0] += fmaf(acc[n][j][0], vs, off0);
-        o[n][j][1] += fmaf(acc[n][j][1], vs, off1);
-        o[n][j][2] += fmaf(acc[n][j][2], vs, off0);
-        o[n][j][3] += fmaf(acc[n][j][3], vs, off1);
+        o[n][j][0] += fmaf(acc[n][j][0], vs0, off0);
+        o[n][j][1] += fmaf(acc[n][j][1], vs1, off1);
+        o[n][j][2] += fmaf(acc[n][j][2], vs0, off0);
+        o[n][j][3] += fmaf(acc[n][j][3], vs1, off1);
       }
     }
     return true;

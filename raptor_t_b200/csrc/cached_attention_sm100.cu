@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       if (!ok) break;
       tc_fence_after_sync();
       const float2 sc = sm.scales[j % kRing];
-      const bool act = live && key0 < wmax && sc.x >= 0.f;
+      const bool act = live && key0 < wmax && !(sc.x < 0.f);
       uint32_t s[64];
       tmem_ld32(ts, s);
       tmem_ld32(ts + 32, s + 32);
@@ -465,16 +465,19 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.s_free[x]);  // the next block's scores may come
       if (act) {
+        float c0 = max_nan(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
+        float off = bias * c0, log_v = sc.y;
         if (key0 + 64 > wmin) {  // keys that some row of the warp does not see
           const int left = lim - key0;
 #pragma unroll
           for (int i = 0; i < 64; ++i)
             if (i >= left) s[i] = 0xff800000u;
+          if (left <= 0) {  // no key of the block: neither its scales nor the row's own query touch the row
+            c0 = 1.f;
+            off = log_v = 0.f;
+          }
         }
-        const bool sees = lim > key0;  // a row that sees no key of the block is not touched by its scales
-        const float c0 = fmaxf(unit * sc.x, 1.17549435e-38f);  // at least the smallest normal number: -inf * 0 would be NaN
-        const float off = bias * c0, m_new = max64(s) * c0 - off;
-        const float log_v = sees ? sc.y : 0.f, most = m_new + log_v;
+        const float m_new = max64(s) * c0 - off, most = m_new + log_v;
         float alpha = 1.f;
         bool fixes = false, apart = false;
         const bool grown = !(m_new <= m + kRescaleThreshold), more = !(most <= ref + kRescaleThreshold);

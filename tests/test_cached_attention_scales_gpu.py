@@ -137,3 +137,48 @@ def test_a_large_value_far_behind(ops):
         for causal in (False, True):
             _check(_attend(ops, q, cache, table, ctx, 160, causal), *_reference(q, cache, table[:-(-ctx // 64)], ctx, 0.125, causal))
     ops.check_device()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_scale_that_is_no_number(ops, fmt, rows, which):
+    """NaN as a scale of a block in use: NaN for the rows that see one of its tokens, nothing for the others."""
+    g = torch.Generator().manual_seed(rows)
+    cache = _filled(g, ops, 9, 2, fmt)
+    cache.k_scale.mul_(2.0 ** -2)
+    table, ctx = [7, 2, 8, 0, 5, 3, 1, 6], min(500, 448 + (rows + 1) // 2)
+    q = torch.randn(rows, 2, 64, generator=g).half().cuda()
+    for causal in (True, False):
+        want, tol = _reference(q, cache, table, ctx, 0.125, causal)
+        for block in (7, 5):
+            kept = getattr(cache, which + "_scale").clone()
+            getattr(cache, which + "_scale")[table[block], 0] = float("nan")  # of one head
+            first = max(0, 64 * block - (ctx - rows)) if causal else 0  # row that sees the block's first token
+            for copies in COPIES:
+                got = _attend(ops, q, cache, table, ctx, copies, causal)
+                assert got[first:, 0].isnan().all()
+                _check(got[:, 1], want[:, 1], tol[:, 1])
+                _check(got[:first, 0], want[:first, 0], tol[:first, 0])
+            getattr(cache, which + "_scale").copy_(kept)
+    ops.check_device()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("rows", ROWS[1:])
+def test_rows_that_see_nothing_hold_anything(ops, fmt, dtype, rows):
+    """Query rows without a key give 0, be they NaN or infinite; the other rows do not notice."""
+    g = torch.Generator().manual_seed(rows)
+    cache = _filled(g, ops, 6, 2, fmt)
+    cache.k_scale.mul_(2.0 ** -2)
+    table, ctx = [4, 0, 5, 2], rows // 2
+    q = torch.randn(rows, 2, 64, generator=g).to(dtype).cuda()
+    want, tol = _reference(q, cache, table[:-(-ctx // 64)], ctx, 0.125, True)
+    blind = rows - ctx
+    q[:blind:2], q[1:blind:2] = float("nan"), float("inf")
+    for copies in COPIES:
+        got = _attend(ops, q, cache, table, ctx, copies, True)
+        assert (got[:blind] == 0).all()
+        _check(got[blind:], want[blind:], tol[blind:])
+    ops.check_device()
