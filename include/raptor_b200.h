@@ -234,12 +234,13 @@ rt_status rt_sparse_attention_static(void* ctx_dev, const void* q_dev, const voi
  * tokens.  No counterpart in the reference, which stops at the encoder's hidden states.
  *
  * Indexes in device memory (table entries, lengths, token ids) are checked by the kernels: one that leaves its buffer is
- * skipped and reported by the next rt_check_device() as RT_ERR_INVALID.  The first call on a device allocates the
+ * skipped and reported by the next rt_check_device() as RT_ERR_INVALID; rt_cached_attention does the same with blocks that have a
+ * negative scale.  The first call on a device allocates the
  * word for that: make it before a stream capture.
  * ---------------------------------------------------------------------------------------- */
 
 /* Blocks of 64 tokens of one head, 64 dimensions each: k / v [blocks][kv_heads][64 tokens][64] code bytes (e4m3 or
- * int8), k_scale / v_scale fp32 [blocks][kv_heads]; value = code * scale.  Which blocks belong to a sequence, and in which order,
+ * int8), k_scale / v_scale fp32 [blocks][kv_heads], at least 0; value = code * scale.  Which blocks belong to a sequence, and in which order,
  * is the caller's block table: int32 [n_seq][table_stride], entry j = block of tokens 64 j .. 64 j + 63; entries behind a
  * sequence's last token are not read.  Sequences may share blocks that none of them writes to. */
 typedef struct rt_kv_cache {

@@ -104,6 +104,7 @@ struct RowTile {
   static constexpr int kRows = 8 * NT;
   int g, t;
   int ctx, least;         // keys of the sequence, and of those what the tile's first row sees
+  int* err;
   int lim[NT][2];         // and what this thread's rows see
   uint32_t q[NT][4][2];
   float unit[NT][2], bias[NT][2];  // a score in base 2 is (product * unit - bias) * key scale
@@ -112,6 +113,7 @@ struct RowTile {
 
   __device__ __forceinline__ void begin(const Args& a, const CachedRows& sr, int head, int row0) {
     ctx = sr.ctx;
+    err = a.err;
     least = sr.limit(a, row0);
     // a negative scale turns the scores around, and with it the queries; with a scale of 0 they are 0
     const float sign = a.scale_log2 > 0.f ? 1.f : a.scale_log2 < 0.f ? -1.f : 0.f;
@@ -144,7 +146,7 @@ struct RowTile {
     }
   }
 
-  // Block b of the sequence; k_scale < 0: no such block, nobody sees its keys.  keys_read(): the keys' codes are in registers;
+  // Block b of the sequence; a negative scale: no such block, nobody sees its keys.  keys_read(): the keys' codes are in registers;
   // values(): where the values' codes are, once they are there; values_read(): they are in registers.
   // Key kk of every 16 is row kk with its lowest bit turned where bit 1 is set, so that the value rows that four threads read at once are
   // even and odd: rows are 64 bytes, banks repeat after 128.
@@ -170,11 +172,16 @@ struct RowTile {
     }
     __syncwarp();
     keys_read();
-    const bool edge = b * 64 + 64 > least || k_scale < 0.f;  // keys that some row of the tile does not see
+    const bool missing = k_scale < 0.f || v_scale < 0.f;
+    const bool edge = b * 64 + 64 > least || missing;  // keys that some row of the tile does not see
     if (edge) {
+      if (missing) {
+        kv::index_error(err, kSiteCachedAttention);
+        k_scale = v_scale = 0.f;
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        const int e0 = k_scale < 0.f ? 0 : lim[n][0], e1 = k_scale < 0.f ? 0 : lim[n][1];
+        const int e0 = missing ? 0 : lim[n][0], e1 = missing ? 0 : lim[n][1];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int key = b * 64 + 16 * i + kg;
@@ -234,7 +241,7 @@ struct RowTile {
     }
     // keys 2 t, + 1, + 8, + 9 of key tile i, dimensions 8 g .. 8 g + 7.  With 16 rows a tile they are read as they are needed: all at once
     // would not fit the registers.
-    const int held = k_scale < 0.f ? 0 : ctx;
+    const int held = missing ? 0 : ctx;
     uint2 vw[NT == 1 ? 16 : 4];
     const uint8_t* vp = values();
     if (!vp) return false;
@@ -352,7 +359,7 @@ struct Feed {
   Look look;
   int slot = 0, done = 0;  // of the piece that is waited for next, pieces so far
   uint32_t phase = 0;
-  float ks[2], vs[2];      // scales of the present block and the next; a negative key scale: there is no such block
+  float ks[2], vs[2];      // scales of the present block and the next; a negative one: there is no such block
   int64_t next = 0;        // the next block's place in the cache
   int later = 0;           // table entry of the block after that
 
@@ -360,8 +367,7 @@ struct Feed {
       : a(args), ring(r), full(f), head(h), count(n), look(l) {}
 
   __device__ __forceinline__ int64_t resolve(int page, float* k, float* v) {
-    const bool bad = page < 0 || page >= a.cache.blocks;
-    if (bad) kv::index_error(a.err, kSiteCachedAttention);
+    const bool bad = page < 0 || page >= a.cache.blocks;  // reported where it is left out
     const int64_t at = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
     *k = bad ? -1.f : __ldg(a.cache.k_scale + at);
     *v = bad ? 0.f : __ldg(a.cache.v_scale + at);

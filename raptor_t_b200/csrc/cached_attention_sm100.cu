@@ -283,10 +283,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     uint8_t* raw = sm.raw[own];
     int64_t slot_k = 0, slot_v = 0;  // of the blocks whose keys and values are requested next
     auto find = [&](int page, int j) {
-      const bool bad = page < 0 || page >= a.cache.blocks;
+      const bool there = page >= 0 && page < a.cache.blocks;
+      const int64_t slot = static_cast<int64_t>(there ? page : 0) * a.cache.heads + head;
+      const float ks = there ? a.cache.k_scale[slot] : -1.f, vs = a.cache.v_scale[slot];
+      const bool bad = ks < 0.f || vs < 0.f;
       if (bad) kv::index_error(a.err, kSiteCachedAttention);
-      const int64_t slot = static_cast<int64_t>(bad ? 0 : page) * a.cache.heads + head;
-      sm.scales[j % kRing] = make_float2(bad ? -1.f : a.cache.k_scale[slot], __log2f(a.cache.v_scale[slot]));
+      sm.scales[j % kRing] = make_float2(bad ? -1.f : ks, __log2f(vs));
       return slot;
     };
     auto request = [&](uint8_t* dst, const uint8_t* base, int64_t slot, uint64_t* bar) {

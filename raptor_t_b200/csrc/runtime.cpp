@@ -78,7 +78,7 @@ rt_status check_device_error(const char* what) {
   if (h != 0) {
     cudaMemset(w, 0, sizeof(int));
     if (h >= kIndexSite)
-      return fail(RT_ERR_INVALID, "%s: an index or length in device memory is out of its range (site %d)", what, h);
+      return fail(RT_ERR_INVALID, "%s: an index, length or scale in device memory is out of its range (site %d)", what, h);
     return fail(RT_ERR_DEVICE_WAIT, "%s: a bounded device-side wait ran out at site %d", what, h);
   }
   return RT_OK;

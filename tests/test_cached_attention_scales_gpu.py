@@ -165,6 +165,29 @@ def test_a_scale_that_is_no_number(ops, fmt, rows, which):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", ROWS)
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_a_negative_scale_is_reported(ops, fmt, rows, which):
+    """Scales are at least 0: a block with a negative one is left out, as one that the cache does not have."""
+    from raptor_t_b200.capi import RtError
+    g = torch.Generator().manual_seed(rows)
+    cache = _filled(g, ops, 9, 1, fmt)
+    cache.k_scale.mul_(2.0 ** -2)
+    q = torch.randn(rows, 1, 64, generator=g).half().cuda()
+    want, tol = _reference(q, cache, [7, 8, 0], 172, 0.125, False)
+    getattr(cache, which + "_scale")[2] *= -1
+    if rows % 3 == 0:  # and the other one is NaN
+        getattr(cache, "kv"[which == "k"] + "_scale")[2] = float("nan")
+    for copies in COPIES:
+        got = _attend(ops, q, cache, [7, 2, 8, 0], 236, copies, False)
+        with pytest.raises(RtError) as e:
+            ops.check_device()
+        assert e.value.code == 1 and "1003" in str(e.value)
+        _check(got, want, tol)
+    ops.check_device()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("rows", ROWS[1:])
 def test_rows_that_see_nothing_hold_anything(ops, fmt, dtype, rows):
