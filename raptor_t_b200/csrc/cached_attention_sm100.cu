@@ -82,12 +82,6 @@ struct Smem {
 static_assert(kStages * 2 * kTile + kRaw * 2 * kBlock + kStreams * 2 * kTile >= kStreams * 128 * 64 * 4, "partial results fit");
 static_assert(sizeof(Smem) <= 227 * 1024, "one CTA per SM");
 
-__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 __device__ __forceinline__ void softmax_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 
 // Contiguous copy global -> shared (16-byte aligned), completion on an mbarrier.
@@ -524,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           uint32_t p[16];
-          l = fmaf(exp_columns<false, 32, kPolyEvery>(s + 32 * h, p, c0, rel + off), back, l);
+          l = fmaf(exp_columns<false, 32, kPolyEvery, true>(s + 32 * h, p, c0, rel + off), back, l);
 #pragma unroll
           for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint4*>(p_row + (((4 * h + i) ^ (r & 7)) << 4)) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);

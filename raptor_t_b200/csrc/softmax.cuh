@@ -35,6 +35,16 @@ __device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsig
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+__device__ __forceinline__ unsigned long long f2_mul(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
@@ -71,10 +81,16 @@ __device__ __forceinline__ float max64(const uint32_t* s) {
 // 2^x for a pair of arguments on the FMA pipe (the exponential unit is the kernel's bottleneck, a part of
 // the columns goes here instead): clamp, split x = n + f with |f| <= 0.5 by adding 1.5 * 2^23 (the integer
 // lands in the low mantissa bits), 2^f by a cubic (relative error 7.5e-5, below the 16-bit rounding of the
-// probabilities), n added to the exponent field.
+// probabilities), n added to the exponent field.  NAN_STAYS: NaN gives NaN (otherwise a small number); 2^n is then a factor.
+template <bool NAN_STAYS>
 __device__ __forceinline__ void ex2_fma_pair(float x0, float x1, float& r0, float& r1) {
-  x0 = fmaxf(x0, -126.f);
-  x1 = fmaxf(x1, -126.f);
+  if constexpr (NAN_STAYS) {
+    x0 = max_nan(x0, -126.f);
+    x1 = max_nan(x1, -126.f);
+  } else {
+    x0 = fmaxf(x0, -126.f);
+    x1 = fmaxf(x1, -126.f);
+  }
   const unsigned long long x = f2_pack(x0, x1);
   const unsigned long long xr = f2_add(x, f2_pack(12582912.f, 12582912.f));
   const unsigned long long n = f2_add(xr, f2_pack(-12582912.f, -12582912.f));
@@ -83,8 +99,13 @@ __device__ __forceinline__ void ex2_fma_pair(float x0, float x1, float& r0, floa
   r = f2_fma(r, f, f2_pack(0.69326099f, 0.69326099f));
   r = f2_fma(r, f, f2_pack(0.99992807f, 0.99992807f));
   float a0, a1, b0, b1;
-  f2_unpack(r, a0, a1);
   f2_unpack(xr, b0, b1);
+  if constexpr (NAN_STAYS) {
+    f2_unpack(f2_mul(r, f2_pack(__int_as_float((__float_as_int(b0) << 23) + 0x3f800000), __int_as_float((__float_as_int(b1) << 23) + 0x3f800000))),
+              r0, r1);
+    return;
+  }
+  f2_unpack(r, a0, a1);
   r0 = __int_as_float(__float_as_int(a0) + (__float_as_int(b0) << 23));
   r1 = __int_as_float(__float_as_int(a1) + (__float_as_int(b1) << 23));
 }
@@ -92,7 +113,7 @@ __device__ __forceinline__ void ex2_fma_pair(float x0, float x1, float& r0, floa
 // p[i] = 2^(s[2i] * c - m), 2^(s[2i+1] * c - m) packed to 16 bits, for N scores; returns their sum.
 // Every EVERY-th pair is computed on the FMA pipe.
 constexpr int kPolyEvery = 4;  // measured: 3 and 4 are equal within noise, 2 is slower (issue slots)
-template <bool BF16, int N, int EVERY = kPolyEvery>
+template <bool BF16, int N, int EVERY = kPolyEvery, bool NAN_STAYS = false>
 __device__ __forceinline__ float exp_columns(const uint32_t* s, uint32_t* p, float scale_log2, float m_ref) {
   static_assert(EVERY > 0, "every how many pairs");
   const unsigned long long c2 = f2_pack(scale_log2, scale_log2);
@@ -105,7 +126,7 @@ __device__ __forceinline__ float exp_columns(const uint32_t* s, uint32_t* p, flo
     f2_unpack(t, t0, t1);
     float p0, p1;
     if (i % EVERY == EVERY - 1) {
-      ex2_fma_pair(t0, t1, p0, p1);
+      ex2_fma_pair<NAN_STAYS>(t0, t1, p0, p1);
     } else {
       p0 = ex2(t0);
       p1 = ex2(t1);

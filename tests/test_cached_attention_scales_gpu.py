@@ -205,3 +205,21 @@ def test_rows_that_see_nothing_hold_anything(ops, fmt, dtype, rows):
         assert (got[:blind] == 0).all()
         _check(got[blind:], want[blind:], tol[blind:])
     ops.check_device()
+
+
+@pytest.mark.parametrize("rows", ROWS)
+def test_a_score_that_is_no_number(ops, rows):
+    """An infinite query entry on keys of 0 there: the scores of these keys are NaN, whichever they are, and so is the row; the other
+    scores are -inf."""
+    g = torch.Generator().manual_seed(rows)
+    cache = _filled(g, ops, 2, 1, torch.float8_e4m3fn)
+    q = torch.randn(rows, 1, 64, generator=g).half().cuda()
+    q[::2, :, 0] = float("inf")
+    for keys in ([0], [13], [14], [15], [30, 31], [47], [63], [64 + 15], [79, 80]):
+        cache.k[:, :, :, 0] = -2.0
+        for key in keys:
+            cache.k[key // 64, :, key % 64, 0] = 0.0
+        for copies in COPIES:
+            got = _attend(ops, q, cache, [0, 1], 81, copies, False)
+            assert got[::2].isnan().all() and got[1::2].isfinite().all(), keys
+    ops.check_device()
