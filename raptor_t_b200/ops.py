@@ -249,7 +249,7 @@ def cached_attention(q, cache, block_table, context, first, max_q=None, max_cont
 
 class TokenScores(NamedTuple):
     """What token_logprobs returns, fp32 (top_ids int32): logp and entropy [rows], stats [rows, 2], top_ids and top_logp
-    [rows, top_k]; None what was not asked for.  The tensors of a call share two allocations: clone one that outlives
+    [rows, top_k]; None what was not asked for.  The fp32 tensors of a call share an allocation: clone one that outlives
     the others by far."""
     logp: Optional[torch.Tensor]
     entropy: torch.Tensor
