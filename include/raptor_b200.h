@@ -262,7 +262,8 @@ typedef struct rt_kv_cache {
  *   need = e4m3: smallest power of two >= a / 448;  int8: a / 127 rounded up to 8 significant bits;  at least 2^-100.
  * Where the block holds earlier tokens (positions below start) and need <= its scale, the scale stays; else it becomes need and the
  * earlier codes c become round(c * old scale / scale).  New codes are round(x / scale), ties to even; infinities take
- * the largest code, NaN the code 0.  Codes of positions that hold no token stay as they are.  A call
+ * the largest code, NaN the code 0.  Quotients are rounded to fp32 first, which changes no code unless a scale that was not made here
+ * stays.  Codes of positions that hold no token stay as they are.  A call
  * may not write to one block twice, be it for two sequences or for two entries of one. */
 rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k_dev, const void* v_dev, int64_t token_stride,
                             int64_t head_stride, const int32_t* block_table_dev, int table_stride, const int32_t* start_dev,

@@ -7,7 +7,8 @@
 // The scale's few bits cost int8 at most 1/128 of its range and e4m3 none of its precision (a power of two moves the
 // exponent), and they make every code exact: x has at most 11 significant bits and the scale 8, so a quotient that is not itself on a border
 // between two codes is at least 2^-17 away from it, more than a correctly rounded fp32 division moves it (2^-18 at 127).  So every
-// implementation of the definition gets the same codes.
+// implementation of the definition gets the same codes.  Scales made elsewhere may have all 24 bits: there a code is that of the quotient as fp32 has
+// it.
 //
 // Both kernels move bytes: 2 in and 1 out a value, or the reverse.  Two warps take one block of one head, keys or values: its
 // 64 rows of 128 bytes stay in registers between the maximum and the rounding, one pass over the data.
@@ -113,30 +114,25 @@ __device__ __forceinline__ unsigned long long f2_add(unsigned long long a, unsig
   return r;
 }
 
-// Codes of x / scale.  int8: the quotient from the correctly rounded reciprocal y by Markstein's correction, q = x y,
-// q + (x - q s) y, which is the correctly rounded one (P. Markstein, IBM J. Res. Dev. 34, 1990); then rounded to a whole number by adding 1.5 * 2^23,
-// whose last byte is the code.  e4m3: the scale is a power of two, the product with its reciprocal exact.
+// Codes of x / scale: the quotient from the correctly rounded reciprocal y by Markstein's correction, q = x y,
+// q + (x - q s) y, which is the correctly rounded one (P. Markstein, IBM J. Res. Dev. 34, 1990), also for scales that were not made here.  int8: rounded to
+// a whole number by adding 1.5 * 2^23, whose last byte is the code.
 template <bool INT8>
 struct Coder {
   unsigned long long inv, neg;
-  float most;
   __device__ __forceinline__ explicit Coder(float scale) {
     const float y = __frcp_rn(scale);
     inv = f2(y, y);
     neg = f2(-scale, -scale);
-    most = INT8 ? kv::kInt8Max * scale : 0.f;  // what infinities become
   }
-  // x where it may be no number
-  __device__ __forceinline__ float number(float x) const {
-    if (x != x) return 0.f;
-    return INT8 ? fminf(fmaxf(x, -most), most) : x;
-  }
+  // what infinities become
+  static __device__ __forceinline__ uint32_t largest(bool negative) { return INT8 ? (negative ? 0x81u : 0x7fu) : (negative ? 0xfeu : 0x7eu); }
   __device__ __forceinline__ uint32_t four(const float* x) const {
     const unsigned long long a = f2(x[0], x[1]), b = f2(x[2], x[3]);
     unsigned long long p = f2_mul(a, inv), q = f2_mul(b, inv);
+    p = f2_fma(f2_fma(p, neg, a), inv, p);
+    q = f2_fma(f2_fma(q, neg, b), inv, q);
     if constexpr (INT8) {
-      p = f2_fma(f2_fma(p, neg, a), inv, p);
-      q = f2_fma(f2_fma(q, neg, b), inv, q);
       const unsigned long long magic = f2(12582912.f, 12582912.f);
       const float2 u = f2_split(f2_add(p, magic)), v = f2_split(f2_add(q, magic));
       const uint32_t lo = kv::prmt(__float_as_uint(u.x), __float_as_uint(u.y), 0x0040u);
@@ -261,11 +257,16 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
       f[2 * j] = t.x;
       f[2 * j + 1] = t.y;
     }
+    uint32_t infinite[2] = {0u, 0u};  // the codes of the infinities among them, whose quotients are 0 here
     if (strange) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = code.number(f[j]);
+      for (int j = 0; j < 8; ++j) {
+        if (fabsf(f[j]) < INFINITY) continue;
+        if (f[j] == f[j]) infinite[j >> 2] |= code.largest(f[j] < 0.f) << (8 * (j & 3));
+        f[j] = 0.f;
+      }
     }
-    *reinterpret_cast<uint2*>(dst + r * 64 + col) = make_uint2(code.four(f), code.four(f + 4));
+    *reinterpret_cast<uint2*>(dst + r * 64 + col) = make_uint2(code.four(f) | infinite[0], code.four(f + 4) | infinite[1]);
   }
   if ((warp & 1) == 0 && lane == 0 && !keep) *scale_at = scale;
 }
