@@ -303,7 +303,8 @@ rt_status rt_token_logprobs(const void* logits_dev, int64_t pitch, const int32_t
 /* The gradient with respect to the logits, rounded once to their type:
  *   dz_v = -p_v (g_logp + sum_j g_top_j + g_entropy (log p_v + entropy)) + [v = target] g_logp + sum_j [v = top_ids_j] g_top_j
  * g_logp_dev / g_entropy_dev fp32 [rows] or NULL (no such term; targets_dev / entropy_dev are then not read), g_top_dev fp32 [rows][top] for
- * top_ids_dev (top = 0: none; an id may stand there twice, a negative one counts for p alone).  dlogits_dev may be logits_dev itself, with the same
+ * top_ids_dev (top = 0: none; an id may stand there twice, a negative one counts for p alone).  A row of nothing but -inf has a gradient of 0, one
+ * with NaN or +inf a gradient of NaN.  dlogits_dev may be logits_dev itself, with the same
  * pitch; otherwise the two do not overlap.  Columns behind vocab stay as they are. */
 rt_status rt_token_logprobs_backward(void* dlogits_dev, int64_t out_pitch, const void* logits_dev, int64_t pitch,
                                      const int32_t* targets_dev, const float* stats_dev, const float* entropy_dev, int rows, int vocab,

@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(256) token_logprobs_grad_kernel(const GradArgs
   const float pull = g_t + (a.top > 0 ? warp_sum(g_alt) : 0.f);
   const float g_h = a.g_entropy ? a.g_entropy[row] : 0.f;
   const float h = a.g_entropy ? a.entropy[row] : 0.f;
-  const bool nothing = st.x == -INFINITY;
+  const bool nothing = st.x == -INFINITY && st.y == 0.f;  // a row of -inf; with a NaN among them its gradient is NaN
   constexpr float kLeast = -1e4f;  // of log p: p = 0 leaves nothing there, and with -inf it would be 0 * inf
   auto grad = [&](float z) {
     const float lp = max_nan((z - st.x) - st.y, kLeast);
