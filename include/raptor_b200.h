@@ -255,7 +255,7 @@ typedef struct rt_kv_cache {
 } rt_kv_cache;
 
 /* Quantises the keys and values of new tokens into the cache.  Sequence s has first_dev[s + 1] - first_dev[s] (at most max_tokens,
- * none allowed) new tokens, rows first_dev[s] .. of the batch of `tokens` rows; they take the positions from start_dev[s] on.
+ * none allowed; with max_tokens = 0 nothing is written) new tokens, rows first_dev[s] .. of the batch of `tokens` rows; they take the positions from start_dev[s] on.
  * k / v: 16-bit, element (row, head, d) at row * token_stride + head * head_stride + d (strides in elements, multiples of 8;
  * columns of a projection's output are fine); token_stride = 0: head-major per sequence, as rt_gemm_qkv and rt_qkv_bias_transpose
  * write them.  With a = the largest finite |value| that the call brings to a block and head:
@@ -270,13 +270,13 @@ rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k_dev, const v
                             const int32_t* first_dev, int n_seq, int tokens, int max_tokens, int dtype, void* stream);
 
 /* The reverse: values of the positions start_dev[s] .. of each sequence, rounded to 16 bits, into rows first_dev[s] .. of
- * k_out / v_out [tokens][kv_heads * 64]. */
+ * k_out / v_out [tokens][kv_heads * 64].  max_tokens = 0 counts as 1. */
 rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* k_out_dev, void* v_out_dev, const int32_t* block_table_dev,
                            int table_stride, const int32_t* start_dev, const int32_t* first_dev, int n_seq, int tokens,
                            int max_tokens, int dtype, void* stream);
 
 /* out[row][head * 64 + d] = softmax(scale * q k^T) v over the cached tokens of the row's sequence.  Sequence s has the query rows
- * first_dev[s] .. first_dev[s + 1] - 1 (at most max_q, none allowed) and context_dev[s] tokens in the cache.  causal = 0: every row
+ * first_dev[s] .. first_dev[s + 1] - 1 (at most max_q, 0 counts as 1; none allowed) and context_dev[s] tokens in the cache.  causal = 0: every row
  * sees all of them; 1: the query rows are the sequence's last tokens and row i of n sees the first context - n + i + 1.  A row
  * that sees nothing is 0, whatever its query holds.  Where a scale is NaN, rows that see one of the block's tokens are NaN, and no
  * other row is touched.  q: 16-bit, element (row, head, d) at row * q_stride + head * 64 + d, q_stride a multiple of 8; out

@@ -640,7 +640,8 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
              "cached_attention: bad sizes");
   RT_REQUIRE(heads % a.cache.heads == 0 && heads <= 4096, RT_ERR_UNSUPPORTED,
              "cached_attention: %d query heads over %d key heads (a multiple, at most 4096)", heads, a.cache.heads);
-  if (n_seq == 0 || tokens == 0 || max_q == 0) return RT_OK;
+  if (n_seq == 0 || tokens == 0) return RT_OK;
+  max_q += max_q == 0;
   RT_REQUIRE(out && q, RT_ERR_INVALID, "cached_attention: null pointer");
   RT_REQUIRE(((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) & 15u) == 0 && q_stride % 8 == 0 && q_stride >= 0,
              RT_ERR_INVALID, "cached_attention: queries and output must be 16-byte aligned, the query stride a multiple of 8 values");

@@ -363,6 +363,7 @@ extern "C" rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* out_k, voi
   KvView c;
   int64_t grid = 0;
   RT_TRY(check_kv_cache("kv_cache_read", cache, &c));
+  max_tokens += max_tokens == 0;
   RT_TRY(check_ragged("kv_cache_read", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &grid));
   if (grid == 0) return RT_OK;
   RT_REQUIRE(out_k && out_v, RT_ERR_INVALID, "kv_cache_read: null pointer");

@@ -72,6 +72,14 @@ void* stream_for(int device) {
   return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
 }
 
+int fits(int64_t v, const char* name) {
+  if (v < 0 || v > INT32_MAX) throw py::value_error(std::string(name) + ": " + std::to_string(v) + " is out of range");
+  return static_cast<int>(v);
+}
+
+// The most rows of one sequence: all rows where the caller does not say, and 0 counts as 1.
+int most_of(int64_t most, int rows, const char* name) { return most < 0 ? rows : std::max(1, fits(most, name)); }
+
 int index_of(const Tensor& t) { return t.is_cuda() ? t.get_device() : -1; }
 
 // Address of a contiguous tensor of that type and shape on that device.
@@ -83,11 +91,6 @@ void* flat(const Tensor& t, const char* name, at::ScalarType type, c10::IntArray
                           std::to_string(device) + ", got " + shape_of(t.sizes()) + " with strides " + shape_of(t.strides()) + " on " +
                           t.device().str());
   return t.data_ptr();
-}
-
-int fits(int64_t v, const char* name) {
-  if (v < 0 || v > INT32_MAX) throw py::value_error(std::string(name) + ": " + std::to_string(v) + " is out of range");
-  return static_cast<int>(v);
 }
 
 Tensor empty(c10::IntArrayRef shape, at::ScalarType type, int device) {
@@ -165,7 +168,7 @@ void kv_cache_write(const Cache& c, const Tensor& k, const Tensor& v, const Tens
   const Ragged r(table, start, first, c.device);
   const int n = fits(tokens, "tokens");
   check(entry.kv_cache_write(&c.c, k.data_ptr(), v.data_ptr(), ts, hs, r.table, r.width, r.lengths, r.first, r.n, n,
-                             max_tokens < 0 ? n : fits(max_tokens, "max_tokens"), dt, st));
+                             most_of(max_tokens, n, "max_tokens"), dt, st));
 }
 
 std::tuple<Tensor, Tensor> kv_cache_read(const Cache& c, const Tensor& table, const Tensor& start, const Tensor& first, int64_t tokens,
@@ -186,7 +189,7 @@ std::tuple<Tensor, Tensor> kv_cache_read(const Cache& c, const Tensor& table, co
   const int dt = dtype16(k);
   const Ragged r(table, start, first, c.device);
   check(entry.kv_cache_read(&c.c, flat(k, "k", type, shape, c.device), flat(v, "v", type, shape, c.device), r.table, r.width, r.lengths,
-                            r.first, r.n, n, max_tokens < 0 ? n : fits(max_tokens, "max_tokens"), dt, st));
+                            r.first, r.n, n, most_of(max_tokens, n, "max_tokens"), dt, st));
   return {k, v};
 }
 
@@ -200,7 +203,7 @@ Tensor cached_attention(const Tensor& q, const Cache& c, const Tensor& table, co
   const Ragged r(table, context, first, c.device);
   const int n = fits(q.size(0), "tokens");
   check(entry.cached_attention(flat(o, "out", q.scalar_type(), q.sizes(), c.device), q.data_ptr(), q.stride(0), &c.c, r.table, r.width,
-                               r.lengths, r.first, r.n, n, max_q < 0 ? n : fits(max_q, "max_q"), fits(max_context, "max_context"),
+                               r.lengths, r.first, r.n, n, most_of(max_q, n, "max_q"), fits(max_context, "max_context"),
                                fits(q.size(1), "heads"), static_cast<float>(scale), causal, dt, st));
   return o;
 }

@@ -227,7 +227,7 @@ def kv_cache_write(cache, k, v, block_table, start, first, max_tokens=None, head
     """Quantises new tokens into the cache (rt_kv_cache_write; the rule for the scales stands there).
     k, v [tokens, kv_heads, 64] 16-bit, rows may be strided (columns of a projection); head_major: the buffers of
     gemm_qkv / qkv_bias_transpose instead, [tokens, kv_heads * 64] storage.  Sequence s writes rows first[s] .. first[s + 1] - 1 to
-    its positions from start[s] on (int32 device tensors).  max_tokens: the most new tokens of one sequence (default: all rows)."""
+    its positions from start[s] on (int32 device tensors).  max_tokens: the most new tokens of one sequence (default: all rows; 0 counts as 1)."""
     _native().kv_cache_write(cache._c, k, v, block_table, start, first, -1 if max_tokens is None else max_tokens, head_major)
 
 
@@ -242,7 +242,7 @@ def cached_attention(q, cache, block_table, context, first, max_q=None, max_cont
     """softmax(scale * q k^T) v over the cached tokens (rt_cached_attention): q [tokens, heads, 64], rows may be strided; returns
     [tokens, heads, 64].  Sequence s has the query rows first[s] .. first[s + 1] - 1 and context[s] cached tokens; causal: its
     rows are its last tokens, row i of n sees the first context - n + i + 1.  max_q: the most query rows of one sequence (default:
-    all rows); max_context only guides how the work is split."""
+    all rows; 0 counts as 1); max_context only guides how the work is split."""
     return _native().cached_attention(q, cache._c, block_table, context, first, -1 if max_q is None else max_q, max_context, scale, causal,
                                       out)
 

@@ -1,0 +1,54 @@
+"""Bounds that the caller states (max_tokens, max_q), and tensors whose strides say nothing because there is one row or one head."""
+import pytest
+import torch
+
+from test_kv_cache_gpu import FORMATS, _filled, _first, _i32, _tables
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a CUDA device")
+    from raptor_t_b200 import ops as _ops
+    return _ops
+
+
+def test_a_bound_of_zero(ops):
+    """A caller who says that no sequence has a token gets one token done all the same, and more than one reported."""
+    from raptor_t_b200.capi import RtError
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(3, 2, 64, generator=g).half().cuda()
+    table, context = _i32([[0], [2], [1]]), _i32([5, 6, 7])
+    one, three = _i32([0, 1, 1, 2]), _i32([0, 0, 3, 3])
+    for first, fails in ((one, False), (three, True), (_i32([0, 0, 0, 0]), False)):
+        a, b = _filled(g, ops, 3, 2, torch.int8), None
+        b = ops.KvCache(*(t.clone() for t in (a.k, a.v, a.k_scale, a.v_scale)))
+        ops.kv_cache_write(a, x, x, table, context, first, max_tokens=0)
+        if fails:
+            with pytest.raises(RtError):
+                ops.check_device()
+        else:
+            ops.kv_cache_write(b, x, x, table, context, first)
+        assert torch.equal(a.k, b.k) and torch.equal(a.v_scale, b.v_scale)
+        outs = []
+        for bound in (0, None):
+            if fails and bound is None:
+                continue
+            back = [torch.full((3, 2, 64), 7.0, dtype=torch.float16, device="cuda") for _ in range(2)]
+            ops.kv_cache_read(a, table, _i32([0, 0, 0]), first, 3, torch.float16, max_tokens=bound, out=back)
+            if fails:
+                with pytest.raises(RtError):
+                    ops.check_device()
+            got = torch.full((3, 2, 64), 7.0, dtype=torch.float16, device="cuda")
+            ops.cached_attention(x, a, table, context, first, max_q=bound, scale=0.125, out=got)
+            if fails:
+                with pytest.raises(RtError):
+                    ops.check_device()
+            outs.append([*back, got])
+        if fails:
+            assert all((t == 7.0).all() for t in outs[0])
+        else:
+            assert all(torch.equal(s, t) for s, t in zip(*outs))
+    ops.check_device()
