@@ -11,6 +11,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <array>
 #include <cstdint>
 #include <optional>
 #include <string>
@@ -155,15 +156,16 @@ void kv_cache_write(const Cache& c, const Tensor& k, const Tensor& v, const Tens
     flat(k, "k", k.scalar_type(), {tokens, heads * 64}, c.device);
     flat(v, "v", k.scalar_type(), {tokens, heads * 64}, c.device);
   } else {
-    if (k.dim() != 3 || k.size(1) != heads || k.size(2) != 64 || k.sizes() != v.sizes() || k.strides() != v.strides() ||
-        k.stride(2) != 1 || v.scalar_type() != k.scalar_type() || index_of(k) != c.device || index_of(v) != c.device)
+    // the stride over one token or one head says nothing
+    auto strides = [&](const Tensor& t) {
+      return std::array<int64_t, 2>{tokens > 1 ? t.stride(0) : 64 * heads, heads > 1 ? t.stride(1) : 64};
+    };
+    if (k.dim() != 3 || k.size(1) != heads || k.size(2) != 64 || k.sizes() != v.sizes() || strides(k) != strides(v) ||
+        k.stride(2) != 1 || v.stride(2) != 1 || v.scalar_type() != k.scalar_type() || index_of(k) != c.device || index_of(v) != c.device)
       throw py::value_error("k and v: expected [tokens, kv_heads, 64] of the same type and strides, on the cache's device");
-    ts = k.stride(0);
-    hs = k.stride(1);
-    if (ts == 0) {
-      if (tokens > 1) throw py::value_error("k and v: rows without a stride");
-      ts = 64 * heads;
-    }
+    ts = strides(k)[0];
+    hs = strides(k)[1];
+    if (ts == 0) throw py::value_error("k and v: rows without a stride");
   }
   const Ragged r(table, start, first, c.device);
   const int n = fits(tokens, "tokens");
@@ -202,7 +204,7 @@ Tensor cached_attention(const Tensor& q, const Cache& c, const Tensor& table, co
   Tensor o = out ? *out : empty(q.sizes(), q.scalar_type(), c.device);
   const Ragged r(table, context, first, c.device);
   const int n = fits(q.size(0), "tokens");
-  check(entry.cached_attention(flat(o, "out", q.scalar_type(), q.sizes(), c.device), q.data_ptr(), q.stride(0), &c.c, r.table, r.width,
+  check(entry.cached_attention(flat(o, "out", q.scalar_type(), q.sizes(), c.device), q.data_ptr(), n > 1 ? q.stride(0) : 64 * q.size(1), &c.c, r.table, r.width,
                                r.lengths, r.first, r.n, n, most_of(max_q, n, "max_q"), fits(max_context, "max_context"),
                                fits(q.size(1), "heads"), static_cast<float>(scale), causal, dt, st));
   return o;

@@ -52,3 +52,33 @@ def test_a_bound_of_zero(ops):
         else:
             assert all(torch.equal(s, t) for s, t in zip(*outs))
     ops.check_device()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_strides_that_say_nothing(ops, fmt):
+    """One token, or one head: the stride over it may be any number."""
+    g = torch.Generator().manual_seed(3)
+    base = torch.randn(5000, generator=g).half().cuda()
+    table, first = _i32([[1, 0]]), _i32([0, 1])
+    # one token
+    x = base[:192].view(1, 3, 64)
+    odd = torch.as_strided(base, (1, 3, 64), (7, 64, 1))
+    zero = torch.as_strided(base, (1, 3, 64), (0, 64, 1))
+    caches = [_filled(torch.Generator().manual_seed(4), ops, 2, 3, fmt) for _ in range(4)]
+    for cache, k, v in zip(caches, (x, odd, zero, odd), (x, odd, zero, x)):
+        ops.kv_cache_write(cache, k, v, table, _i32([70]), first)
+    outs = [ops.cached_attention(q, cache, table, _i32([71]), first, scale=0.125) for cache, q in zip(caches, (x, odd, zero, x))]
+    for cache, o in zip(caches[1:], outs[1:]):
+        assert torch.equal(cache.k.view(torch.int8), caches[0].k.view(torch.int8)) and torch.equal(cache.v_scale, caches[0].v_scale)
+        assert torch.equal(o, outs[0])
+    # one head
+    y = base[:640].view(10, 1, 64)
+    odd = torch.as_strided(base, (10, 1, 64), (64, 3, 1))
+    caches = [_filled(torch.Generator().manual_seed(4), ops, 2, 1, fmt) for _ in range(3)]
+    first = _i32([0, 10])
+    for cache, k, v in zip(caches, (y, odd, odd), (y, odd, y)):
+        ops.kv_cache_write(cache, k, v, table, _i32([60]), first)
+    outs = [ops.cached_attention(q, cache, table, _i32([70]), first, scale=0.125) for cache, q in zip(caches, (y, odd, y))]
+    for cache, o in zip(caches[1:], outs[1:]):
+        assert torch.equal(cache.k.view(torch.int8), caches[0].k.view(torch.int8)) and torch.equal(o, outs[0])
+    ops.check_device()
