@@ -629,6 +629,19 @@ rt_status launch_by_rows(const Args& a, cudaStream_t st) {
 
 using namespace rt;
 
+namespace {
+
+// Does the output [tokens][width] share memory with the rows of the queries (`width` values each, `stride` apart)?
+bool overlaps(const void* out, const void* q, int64_t stride, int64_t tokens, int64_t width) {
+  const int64_t row = 2 * width, step = 2 * stride, begin = reinterpret_cast<intptr_t>(out) - reinterpret_cast<intptr_t>(q), end = begin + tokens * row;
+  if (end <= 0 || begin >= (tokens - 1) * step + row) return false;
+  // the first row that ends behind the output's beginning
+  const int64_t i = begin < row ? 0 : step == 0 ? tokens : std::min(tokens, (begin - row) / step + 1);
+  return i < tokens && i * step < end;
+}
+
+}  // namespace
+
 extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_stride, const rt_kv_cache* cache, const int32_t* table,
                                          int table_stride, const int32_t* context, const int32_t* first, int n_seq, int tokens,
                                          int max_q, int max_context, int heads, float scale, int causal, int dtype, void* stream) {
@@ -664,6 +677,7 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
   RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * (rows / 8 + 1) < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
              "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
+  RT_REQUIRE(!overlaps(out, q, q_stride, tokens, int64_t{64} * heads), RT_ERR_INVALID, "cached_attention: the output overlaps the queries");
   const int64_t widest = static_cast<int64_t>(table_stride) * 64;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
   // Which kernel: the one of few rows pays for every 16 rows that there are (1.65 ns a tile and block of keys on the full chip), the one of many

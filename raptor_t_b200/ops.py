@@ -242,7 +242,7 @@ def cached_attention(q, cache, block_table, context, first, max_q=None, max_cont
     """softmax(scale * q k^T) v over the cached tokens (rt_cached_attention): q [tokens, heads, 64], rows may be strided; returns
     [tokens, heads, 64].  Sequence s has the query rows first[s] .. first[s + 1] - 1 and context[s] cached tokens; causal: its
     rows are its last tokens, row i of n sees the first context - n + i + 1.  max_q: the most query rows of one sequence (default:
-    all rows; 0 counts as 1); max_context only guides how the work is split."""
+    all rows; 0 counts as 1); max_context only guides how the work is split.  out must not overlap q."""
     return _native().cached_attention(q, cache._c, block_table, context, first, -1 if max_q is None else max_q, max_context, scale, causal,
                                       out)
 

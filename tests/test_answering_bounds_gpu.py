@@ -82,3 +82,25 @@ def test_strides_that_say_nothing(ops, fmt):
     for cache, o in zip(caches[1:], outs[1:]):
         assert torch.equal(cache.k.view(torch.int8), caches[0].k.view(torch.int8)) and torch.equal(o, outs[0])
     ops.check_device()
+
+
+def test_output_over_the_queries_is_refused(ops):
+    """Every row's keys are read after other rows have been written."""
+    from raptor_t_b200.capi import RtError
+    g = torch.Generator().manual_seed(5)
+    cache = _filled(g, ops, 2, 2, torch.int8)
+    store = torch.randn(40, 2, 64, generator=g).half().cuda()
+    args = cache, _i32([[0, 1]]), _i32([100]), _i32([0, 20])
+    want = ops.cached_attention(store[:20], *args, scale=0.125)
+    for out in (store[:20], store[19:39]):
+        with pytest.raises(RtError) as e:
+            ops.cached_attention(store[:20], *args, scale=0.125, out=out)
+        assert e.value.code == 1
+    assert torch.equal(ops.cached_attention(store[:20], *args, scale=0.125, out=store[20:]), want)
+    # between the rows of wider ones: one row of output in the gap of the queries' buffer
+    wide = torch.randn(20, 3 * 128, generator=g).half().cuda()
+    q = wide[:1, :128].unflatten(1, (2, 64))
+    one = cache, _i32([[0, 1]]), _i32([100]), _i32([0, 1])
+    want = ops.cached_attention(q, *one, scale=0.125)
+    assert torch.equal(ops.cached_attention(q, *one, scale=0.125, out=wide[:1, 128:256].view(1, 2, 64)), want)
+    ops.check_device()
