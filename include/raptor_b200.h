@@ -282,7 +282,7 @@ rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* k_out_dev, void* v_ou
  * other row is touched.  q: 16-bit, element (row, head, d) at row * q_stride + head * 64 + d, q_stride a multiple of 8; out
  * [tokens][heads * 64] must not overlap q.  heads is a multiple of the cache's kv_heads: query head h reads
  * key head h / (heads / kv_heads).  Rows behind the last sequence stay as they are.  max_context (0: as wide as the table) only
- * guides how the work is split, a wrong one costs time. */
+ * guides how the work is split, a wrong one costs time.  scale is a number. */
 rt_status rt_cached_attention(void* out_dev, const void* q_dev, int64_t q_stride, const rt_kv_cache* cache,
                               const int32_t* block_table_dev, int table_stride, const int32_t* context_dev,
                               const int32_t* first_dev, int n_seq, int tokens, int max_q, int max_context, int heads, float scale,

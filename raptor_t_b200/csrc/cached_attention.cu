@@ -23,6 +23,7 @@
 #include "cached_attention.h"
 
 #include <algorithm>
+#include <cmath>
 
 #include "device_error.h"
 #include "launch.h"
@@ -677,6 +678,7 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
   RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * (rows / 8 + 1) < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
              "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
+  RT_REQUIRE(std::isfinite(a.scale_log2), RT_ERR_INVALID, "cached_attention: the scale is no number, or too large for one");
   RT_REQUIRE(!overlaps(out, q, q_stride, tokens, int64_t{64} * heads), RT_ERR_INVALID, "cached_attention: the output overlaps the queries");
   const int64_t widest = static_cast<int64_t>(table_stride) * 64;
   const int64_t keys = max_context > 0 ? std::min<int64_t>(max_context, widest) : widest;
