@@ -14,6 +14,9 @@
 // 64 rows of 128 bytes stay in registers between the maximum and the rounding, one pass over the data.
 #include "kv_cache.cuh"
 
+#include <algorithm>
+#include <type_traits>
+
 #include "device_error.h"
 #include "launch.h"
 #include "launch_count.h"
@@ -71,6 +74,34 @@ __device__ __forceinline__ Span span_of(int seq, int nth, const int32_t* __restr
   }
   s.page = page;
   return s;
+}
+
+// Which sequence and which of its blocks a CTA takes.  Direct: every sequence has `spans` places, as many as its longest one may need.  From a list:
+// sequence s has the places first[s] / 64 + 2 s .. first[s + 1] / 64 + 2 s + 1, never fewer than it needs (a sequence of n tokens touches at
+// most (n + 62) / 64 + 1 blocks), tokens / 64 + 2 n_seq in all; each CTA looks for the sequence that has its place.
+struct Place {
+  int seq, nth;
+};
+template <bool LISTED>
+__device__ __forceinline__ Place place_of(int at, int spans, const int32_t* __restrict__ first, int n_seq, int tokens, int max_tokens, int* err, int site) {
+  if constexpr (!LISTED) return Place{at / spans, at % spans};
+  __shared__ int s_seq, s_nth, s_found;
+  if (threadIdx.x == 0) s_found = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < n_seq; s += blockDim.x) {
+    const int f0 = first[s], f1 = first[s + 1];
+    if (f1 <= f0) continue;
+    const int64_t lo = (f0 >> 6) + 2ll * s, hi = (f1 >> 6) + 2ll * s + 2;
+    if (f0 < 0 || f1 > tokens || static_cast<int64_t>(f1) - f0 > max_tokens) {
+      kv::index_error(err, site);
+    } else if (lo <= at && at < hi) {
+      s_seq = s;
+      s_nth = static_cast<int>(at - lo);
+      if (atomicAdd(&s_found, 1)) kv::index_error(err, site);  // rows of two sequences
+    }
+  }
+  __syncthreads();
+  return Place{s_found == 1 ? s_seq : -1, s_nth};
 }
 
 // The packed row of 64 values of token `t` (row of the batch): token-major with strides, or head-major per sequence
@@ -164,20 +195,20 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
 // HBM and a CTA's chain of index, load, maximum, store; one warp a tile, quotients by division and maxima in fp32 took 67.7.  A step's tokens (32 sequences, 12 heads) are that
 // chain alone, 2.8 us.
 constexpr int kWriteThreads = 128;
-template <bool BF16, bool INT8>
+template <bool BF16, bool INT8, bool LISTED>
 __global__ void __launch_bounds__(kWriteThreads, 9)
 kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t token_stride, int64_t head_stride,
                 const int32_t* __restrict__ table, int table_stride, const int32_t* __restrict__ start,
-                const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
+                const int32_t* __restrict__ first, int n_seq, int tokens, int max_tokens, int spans, int* err) {
   __shared__ uint32_t s_most[kWriteThreads / 32];
   RT_PDL_WAIT();
   RT_PDL_LAUNCH_DEPENDENTS();  // not before the wait: launches would queue up on the SMs
   const int head = blockIdx.x % c.heads;
-  const int nth = blockIdx.x / c.heads % spans;
-  const int seq = blockIdx.x / c.heads / spans;
+  const Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheWrite);
+  if (place.seq < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool values = warp >= 2;
-  const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheWrite);
+  const Span s = span_of(place.seq, place.nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheWrite);
   if (s.page < 0) return;
   const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
   uint8_t* dst = (values ? c.v : c.k) + slot * 4096;
@@ -272,18 +303,19 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
 }
 
 // The same grid and warps; out_k / out_v are token-major [tokens][heads * 64].  Bound by HBM: 249 MB in 42.4 us, 5.9 TB/s.
-template <bool BF16, bool INT8>
+template <bool BF16, bool INT8, bool LISTED>
 __global__ void __launch_bounds__(kWriteThreads, 9)
 kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ out_v, const int32_t* __restrict__ table,
-               int table_stride, const int32_t* __restrict__ start, const int32_t* __restrict__ first, int tokens, int max_tokens, int spans, int* err) {
+               int table_stride, const int32_t* __restrict__ start, const int32_t* __restrict__ first, int n_seq, int tokens, int max_tokens, int spans,
+               int* err) {
   RT_PDL_WAIT();
   RT_PDL_LAUNCH_DEPENDENTS();
   const int head = blockIdx.x % c.heads;
-  const int nth = blockIdx.x / c.heads % spans;
-  const int seq = blockIdx.x / c.heads / spans;
+  const Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheRead);
+  if (place.seq < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool values = warp >= 2;
-  const Span s = span_of(seq, nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheRead);
+  const Span s = span_of(place.seq, place.nth, table, table_stride, start, first, tokens, max_tokens, c.blocks, err, kSiteCacheRead);
   if (s.page < 0) return;
   const int64_t slot = static_cast<int64_t>(s.page) * c.heads + head;
   const int row0 = (warp & 1) * 32 + (lane >> 3), col = (lane & 7) * 8;
@@ -313,18 +345,40 @@ kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ ou
 }
 
 // Blocks that `max_tokens` new tokens of a sequence touch at most, wherever they start.
-int64_t spans_of(int max_tokens) { return (static_cast<int64_t>(max_tokens) + 62) / 64 + 1; }
+int spans_of(int max_tokens) { return static_cast<int>((static_cast<int64_t>(max_tokens) + 62) / 64 + 1); }
+
+// How a call's CTAs find their work, and how many there are.
+struct Plan {
+  int64_t grid;
+  bool listed;
+};
 
 rt_status check_ragged(const char* what, const int32_t* table, int table_stride, const int32_t* start, const int32_t* first, int n_seq,
-                       int tokens, int max_tokens, int kv_heads, int dtype, int64_t* grid) {
+                       int tokens, int max_tokens, int kv_heads, int dtype, Plan* plan) {
   RT_REQUIRE(table && start && first, RT_ERR_INVALID, "%s: null pointer", what);
   RT_REQUIRE(dtype == RT_F16 || dtype == RT_BF16, RT_ERR_INVALID, "%s: unknown dtype %d", what, dtype);
   RT_REQUIRE(n_seq >= 0 && tokens >= 0 && table_stride > 0 && max_tokens >= 0, RT_ERR_INVALID, "%s: bad sizes", what);
-  *grid = static_cast<int64_t>(n_seq) * kv_heads;  // under 2^41
-  if (tokens == 0 || max_tokens == 0) *grid = 0;
-  RT_REQUIRE(*grid < (int64_t{1} << 31) && (*grid *= spans_of(max_tokens)) < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "%s: %d sequences of up to %d tokens are too many for one call", what,
-             n_seq, max_tokens);
+  *plan = Plan{0, false};
+  if (n_seq == 0 || tokens == 0 || max_tokens == 0) return RT_OK;
+  const int64_t direct = static_cast<int64_t>(n_seq) * spans_of(std::min(max_tokens, tokens)), places = tokens / 64 + int64_t{2} * n_seq;  // under 2^57
+  // A CTA without work costs 10 to 15 ns of a call, a CTA that looks for its sequence 7 % more and as much again for each 1000 sequences.  12 heads, int8,
+  // us direct and listed: 8 x 4096 tokens with 1.0 CTAs for each place 24.8 and 26.6, with 2.0 27.2 and 26.6, with 7.8 (any of them may bring all) 55.8 and
+  // 26.6; 64 x 2048, 60: 1632 and 96; 300 x 40, 2.3: 25.0 and 21.6; 1000 x 65, 2.0: 98 and 127, 11: 424 and 127; 5000 x 1, 1.0: 152 and 948.
+  plan->listed = static_cast<double>(direct) > static_cast<double>(places) * (2.0 + n_seq * 1e-3);
+  const int64_t ctas = plan->listed ? places : direct;
+  RT_REQUIRE(ctas < (int64_t{1} << 31) && ctas * kv_heads < (int64_t{1} << 31), RT_ERR_UNSUPPORTED,
+             "%s: %d sequences of up to %d tokens are too many for one call", what, n_seq, max_tokens);
+  plan->grid = ctas * kv_heads;
   return RT_OK;
+}
+
+// The kernel for the 16-bit type, the cache's format and the plan.
+template <typename F>
+auto choose(bool bf16, bool int8, bool listed, F kernel) {
+  using T = std::true_type;
+  using N = std::false_type;
+  auto with = [&](auto b, auto i) { return listed ? kernel(b, i, T()) : kernel(b, i, N()); };
+  return bf16 ? (int8 ? with(T(), T()) : with(T(), N())) : (int8 ? with(N(), T()) : with(N(), N()));
 }
 
 }  // namespace
@@ -336,22 +390,22 @@ extern "C" rt_status rt_kv_cache_write(const rt_kv_cache* cache, const void* k, 
                                        int64_t head_stride, const int32_t* table, int table_stride, const int32_t* start,
                                        const int32_t* first, int n_seq, int tokens, int max_tokens, int dtype, void* stream) {
   KvView c;
-  int64_t grid = 0;
+  Plan plan;
   RT_TRY(check_kv_cache("kv_cache_write", cache, &c));
-  RT_TRY(check_ragged("kv_cache_write", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &grid));
-  if (grid == 0) return RT_OK;
+  RT_TRY(check_ragged("kv_cache_write", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &plan));
+  if (plan.grid == 0) return RT_OK;
   RT_REQUIRE(k && v, RT_ERR_INVALID, "kv_cache_write: null pointer");
   RT_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15u) == 0 && token_stride % 8 == 0 &&
                  head_stride % 8 == 0 && token_stride >= 0 && head_stride >= 0,
              RT_ERR_INVALID, "kv_cache_write: keys and values must be 16-byte aligned, with strides that are multiples of 8 values");
   int* err = device_error_word();
   RT_REQUIRE(err != nullptr, RT_ERR_CUDA, "kv_cache_write: cannot allocate the device error word");
-  const bool int8 = cache->format == RT_KV_INT8;
-  auto kern = dtype == RT_BF16 ? (int8 ? kv_write_kernel<true, true> : kv_write_kernel<true, false>)
-                               : (int8 ? kv_write_kernel<false, true> : kv_write_kernel<false, false>);
-  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
+  auto kern = choose(dtype == RT_BF16, cache->format == RT_KV_INT8, plan.listed, [](auto bf16, auto int8, auto listed) {
+    return kv_write_kernel<decltype(bf16)::value, decltype(int8)::value, decltype(listed)::value>;
+  });
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(plan.grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
                               static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), token_stride, head_stride, table,
-                              table_stride, start, first, tokens, max_tokens, static_cast<int>(spans_of(max_tokens)), err));
+                              table_stride, start, first, n_seq, tokens, max_tokens, spans_of(std::min(max_tokens, tokens)), err));
   count_launch();
   RT_CHECK_CUDA(cudaGetLastError());
   return RT_OK;
@@ -361,22 +415,22 @@ extern "C" rt_status rt_kv_cache_read(const rt_kv_cache* cache, void* out_k, voi
                                       const int32_t* start, const int32_t* first, int n_seq, int tokens, int max_tokens, int dtype,
                                       void* stream) {
   KvView c;
-  int64_t grid = 0;
+  Plan plan;
   RT_TRY(check_kv_cache("kv_cache_read", cache, &c));
   max_tokens += max_tokens == 0;
-  RT_TRY(check_ragged("kv_cache_read", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &grid));
-  if (grid == 0) return RT_OK;
+  RT_TRY(check_ragged("kv_cache_read", table, table_stride, start, first, n_seq, tokens, max_tokens, c.heads, dtype, &plan));
+  if (plan.grid == 0) return RT_OK;
   RT_REQUIRE(out_k && out_v, RT_ERR_INVALID, "kv_cache_read: null pointer");
   RT_REQUIRE(((reinterpret_cast<uintptr_t>(out_k) | reinterpret_cast<uintptr_t>(out_v)) & 15u) == 0, RT_ERR_INVALID,
              "kv_cache_read: outputs must be 16-byte aligned");
   int* err = device_error_word();
   RT_REQUIRE(err != nullptr, RT_ERR_CUDA, "kv_cache_read: cannot allocate the device error word");
-  const bool int8 = cache->format == RT_KV_INT8;
-  auto kern = dtype == RT_BF16 ? (int8 ? kv_read_kernel<true, true> : kv_read_kernel<true, false>)
-                               : (int8 ? kv_read_kernel<false, true> : kv_read_kernel<false, false>);
-  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
-                              static_cast<uint16_t*>(out_k), static_cast<uint16_t*>(out_v), table, table_stride, start, first, tokens,
-                              max_tokens, static_cast<int>(spans_of(max_tokens)), err));
+  auto kern = choose(dtype == RT_BF16, cache->format == RT_KV_INT8, plan.listed, [](auto bf16, auto int8, auto listed) {
+    return kv_read_kernel<decltype(bf16)::value, decltype(int8)::value, decltype(listed)::value>;
+  });
+  RT_CHECK_CUDA(launch_kernel(kern, dim3(static_cast<unsigned>(plan.grid)), dim3(kWriteThreads), 0, static_cast<cudaStream_t>(stream), c,
+                              static_cast<uint16_t*>(out_k), static_cast<uint16_t*>(out_v), table, table_stride, start, first, n_seq,
+                              tokens, max_tokens, spans_of(std::min(max_tokens, tokens)), err));
   count_launch();
   RT_CHECK_CUDA(cudaGetLastError());
   return RT_OK;
