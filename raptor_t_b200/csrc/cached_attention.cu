@@ -441,7 +441,7 @@ struct Smem {
   float2 part_ml[kMaxSplits][16];
   float2 ml[kWarps][16];
   uint64_t full[kWarps][kSlots];
-  int cost[kWarps * 32 + 1];
+  alignas(16) int cost[kRanked + 4];
   int abort_flag;
 };
 static_assert(4 * (sizeof(Smem) + 1024) <= 228 * 1024, "four CTAs share an SM");

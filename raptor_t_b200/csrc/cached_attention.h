@@ -1,5 +1,7 @@
 // Arguments of the kernels behind rt_cached_attention (cached_attention.cu: few query rows, cached_attention_sm100.cu: many).
 #pragma once
+#include <limits.h>
+
 #include "device_error.h"
 #include "kv_cache.cuh"
 
@@ -53,20 +55,30 @@ struct CachedRows {
   }
 };
 
-// The `place`-th largest of `n` costs (equal ones in order of their index), n at most the CTA's threads; cost[] in shared memory, n + 1 ints.
-// All threads of the CTA call it; `mine` is the cost of the calling thread's index.
-// CTAs start in order of their index: with the longest work first the last ones to end are short.
-__device__ __forceinline__ int index_by_cost(int* cost, int n, int mine, int place) {
+// The `place`-th largest of `n` costs (in keys; by whole blocks, equal ones in order of their index), n at most kRanked and at most the CTA's
+// threads; key[] in shared memory, kRanked + 4 ints, 16-byte aligned.  All threads of the CTA call it; `mine` is the cost of the calling
+// thread's index.  CTAs start in order of their index: with the longest work first the last ones to end are short.
+constexpr int kRanked = 256;
+__device__ __forceinline__ int index_by_cost(int* key, int n, int mine, int place) {
   const int tid = threadIdx.x;
-  if (tid < n) cost[tid] = mine;
+  const int own = min(mine >> 6, (1 << 23) - 1) * kRanked + (kRanked - 1 - tid);  // no two are equal
+  if (tid < n) key[tid] = own;
+  if (tid < 4) key[n + tid] = INT_MIN;
   __syncthreads();
+  int before = 0;
   if (tid < n) {
-    int before = 0;
-    for (int i = 0; i < n; ++i) before += cost[i] > mine || (cost[i] == mine && i < tid);
-    if (before == place) cost[n] = tid;
+    for (int i = 0; i < n; i += 4) {
+      const int4 k = *reinterpret_cast<const int4*>(key + i);
+      before += k.x > own;
+      before += k.y > own;
+      before += k.z > own;
+      before += k.w > own;
+    }
   }
   __syncthreads();
-  return cost[n];
+  if (tid < n && before == place) key[0] = tid;
+  __syncthreads();
+  return key[0];
 }
 
 namespace kv {

@@ -46,6 +46,7 @@ constexpr int kThreads = 768;
 constexpr int kSoftmaxThreads = 512;
 constexpr int kStreams = 4;
 constexpr int kMaxSplits = 8;            // CTAs of a cluster
+constexpr int kSms = 148;
 constexpr int kStages = 4;               // operand tiles of keys, and of values: one for each warp that fills them
 constexpr int kRaw = 4;                  // blocks of codes on their way, one for each of these warps
 constexpr int kBlock = 4096;             // codes of a block's keys, or values
@@ -75,7 +76,7 @@ struct Smem {
   float ref[kStreams][128];  // R
   float2 ml_cta[256];
   float ref_cta[256];
-  int cost[kThreads + 1];
+  alignas(16) int cost[kRanked + 4];
   uint32_t tmem_slot;
   int abort_flag;
 };
@@ -715,7 +716,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
 
 rt_status launch_cached_attention_many_rows(const Args& args, bool bf16, bool int8, cudaStream_t st) {
   Args a = args;
-  a.sorted = a.n_seq * a.tiles > 1 && a.n_seq * a.tiles <= kThreads;
+  // Longest tiles first where there are more CTAs than run at once, but not so many that the last round hardly counts or that ranking them, which
+  // every CTA does for itself, costs more than it saves.  Sequences of 65 to 256 rows over 64 to 4096 keys, us in order and ranked: 200 with one key head
+  // (200 CTAs) 70.6 and 54.9, 128 with four (512) 95.5 and 73.7, 200 with four (800) 137.7 and 113.3, 256 with four (1024) 157.4 and 152.4, 256 with
+  // twelve (3072) 414 and 456; equal lengths lose 3 to 6 %.  Ranking 768 of them took 110 us of a call of 160.
+  const int64_t items = static_cast<int64_t>(a.n_seq) * a.tiles, ctas = items * a.cache.heads * a.splits;
+  a.sorted = items <= kRanked && ctas > kSms && ctas <= 6 * kSms;
   auto kern = bf16 ? (int8 ? many_rows_kernel<true, true> : many_rows_kernel<true, false>)
                    : (int8 ? many_rows_kernel<false, true> : many_rows_kernel<false, false>);
   RT_TRY(ensure_kernel_smem(reinterpret_cast<const void*>(kern), sizeof(Smem), true));
