@@ -676,7 +676,7 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   RT_REQUIRE(static_cast<int64_t>(a.max_q) * a.group < (int64_t{1} << 30), RT_ERR_UNSUPPORTED, "cached_attention: too many query rows");
   const int rows = a.max_q * a.group;
   const int64_t heads_of_all = static_cast<int64_t>(n_seq) * a.cache.heads;  // under 2^41
-  RT_REQUIRE(heads_of_all < (int64_t{1} << 26) && heads_of_all * (rows / 8 + 1) < (int64_t{1} << 28), RT_ERR_UNSUPPORTED,
+  RT_REQUIRE(heads_of_all < (int64_t{1} << 26), RT_ERR_UNSUPPORTED,
              "cached_attention: %d sequences of up to %d query tokens are too many for one call", n_seq, max_q);
   RT_REQUIRE(std::isfinite(a.scale_log2), RT_ERR_INVALID, "cached_attention: the scale is no number, or too large for one");
   RT_REQUIRE(!overlaps(out, q, q_stride, tokens, int64_t{64} * heads), RT_ERR_INVALID, "cached_attention: the output overlaps the queries");
@@ -686,9 +686,15 @@ extern "C" rt_status rt_cached_attention(void* out, const void* q, int64_t q_str
   // rows for whole tiles.  12 x 4096 keys, 12 heads, 64 rows each: 60.5 and 39.8 us; 16 x 2000 keys 45.7 and 47.3; 16 x 512 to 4096 keys, 5 to
   // 64 rows: 41 and 53.
   const int64_t few_tiles = std::min(n_seq * static_cast<int64_t>((rows + 15) / 16), static_cast<int64_t>(tokens) * a.group / 16 + n_seq / 2);
-  const int64_t big = heads_of_all * ((rows + 255) / 256);
+  // Tiles of the kernel of many rows: as many for each sequence as the longest one has, or, where that is much more than the rows of the call
+  // make, by a search for each CTA's sequence.  12 heads, causal, us: 8 sequences of 2048 rows with 64 tiles each 525 (most CTAs had no work and
+  // were ranked all the same), searched for 133; 64 x 512 with 128 each 1038 and 237; with 2 each 227.
+  a.tiles = (rows + 255) / 256;
+  const int64_t direct = many_rows_items(a);
+  a.listed = true;
+  a.listed = static_cast<double>(direct) > static_cast<double>(many_rows_items(a)) * (1.5 + n_seq * 1e-3);
   double many_us = 0;
-  const int many_splits = many_rows_splits(big, rows, keys, &many_us);
+  const int many_splits = many_rows_splits(many_rows_items(a) * a.cache.heads, rows, keys, &many_us);
   const bool many = rows > kFewRows ||
                     (rows > 32 && many_us < 5.0 + 1.65e-3 * static_cast<double>(few_tiles * a.cache.heads) * ((keys + 63) / 64));
   a.tile_rows = many ? 256 : rows <= 8 ? 8 : 16;

@@ -20,6 +20,7 @@ struct CachedAttentionArgs {
   int tile_rows, tiles;                    // rows of a tile, tiles of the longest sequence
   int splits;                              // CTAs of a cluster that share a tile's keys
   int sorted;                              // long sequences first
+  int listed;                              // many rows: tiles by kv::find_place, at most `tiles` of a sequence otherwise
   float scale_log2;
   int causal;
   int* err;
@@ -136,6 +137,10 @@ __device__ __forceinline__ uint32_t peer_address(uint32_t addr, int rank) {
 
 }  // namespace kv
 
+// Tiles that the kernel of many rows has a place for.
+inline int64_t many_rows_items(const CachedAttentionArgs& a) {
+  return a.listed ? (static_cast<int64_t>(a.tokens) * a.group >> 8) + a.n_seq : static_cast<int64_t>(a.n_seq) * a.tiles;
+}
 rt_status launch_cached_attention_many_rows(const CachedAttentionArgs& a, bool bf16, bool int8, cudaStream_t st);
 
 }  // namespace rt

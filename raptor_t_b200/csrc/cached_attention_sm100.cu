@@ -79,6 +79,8 @@ struct Smem {
   alignas(16) int cost[kRanked + 4];
   uint32_t tmem_slot;
   int abort_flag;
+  kv::Place place;
+  int places;
 };
 static_assert(kStages * 2 * kTile + kRaw * 2 * kBlock + kStreams * 2 * kTile >= kStreams * 128 * 64 * 4, "partial results fit");
 static_assert(sizeof(Smem) <= 227 * 1024, "one CTA per SM");
@@ -136,8 +138,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
   const int rank = blockIdx.x % a.splits;
   const int head = blockIdx.x / a.splits % a.cache.heads;
   int item = blockIdx.x / a.splits / a.cache.heads;  // (sequence, tile), the last tiles first
-  const int items = a.n_seq * a.tiles;
-  if (a.sorted) {
+  kv::Place place{-1, 0};
+  if (a.listed) {
+    place = kv::find_place(item, a.first, a.n_seq, a.group, 8, 1, a.tokens, a.max_q, &sm.place, &sm.places, a.err, kSiteCachedAttention);
+    if (place.seq < 0) return;
+  } else if (a.sorted) {
+    const int items = a.n_seq * a.tiles;
     int cost = -1;
     if (tid < items) {
       const int s = tid % a.n_seq, first_row = (a.tiles - 1 - tid / a.n_seq) * 256;
@@ -146,11 +152,12 @@ __global__ void __launch_bounds__(kThreads, 1) many_rows_kernel(const Args a) {
     }
     item = index_by_cost(sm.cost, items, cost, item);
   }
-  const int tile = a.tiles - 1 - item / a.n_seq, seq = item % a.n_seq;
+  const int seq = a.listed ? place.seq : item % a.n_seq;
   const CachedRows sr(a, seq);
   if (!sr.ok) return;
+  const int tile = a.listed ? (sr.rows - 1) / 256 - place.nth : a.tiles - 1 - item / a.n_seq;
   const int row0 = tile * 256, here = min(256, sr.rows - row0);
-  if (here <= 0) return;
+  if (tile < 0 || here <= 0) return;
   const bool two = here > 128;  // two row tiles, each with two streams; otherwise one with four
   const int most = sr.limit(a, row0 + here - 1);
   const int all_blocks = (most + 63) / 64, each = (all_blocks + a.splits - 1) / a.splits;
@@ -720,13 +727,15 @@ rt_status launch_cached_attention_many_rows(const Args& args, bool bf16, bool in
   // every CTA does for itself, costs more than it saves.  Sequences of 65 to 256 rows over 64 to 4096 keys, us in order and ranked: 200 with one key head
   // (200 CTAs) 70.6 and 54.9, 128 with four (512) 95.5 and 73.7, 200 with four (800) 137.7 and 113.3, 256 with four (1024) 157.4 and 152.4, 256 with
   // twelve (3072) 414 and 456; equal lengths lose 3 to 6 %.  Ranking 768 of them took 110 us of a call of 160.
-  const int64_t items = static_cast<int64_t>(a.n_seq) * a.tiles, ctas = items * a.cache.heads * a.splits;
-  a.sorted = items <= kRanked && ctas > kSms && ctas <= 6 * kSms;
+  const int64_t items = many_rows_items(a), ctas = items * a.cache.heads * a.splits;
+  RT_REQUIRE(ctas < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "cached_attention: %d sequences of up to %d query tokens are too many for one call", a.n_seq,
+             a.max_q);
+  a.sorted = !a.listed && items <= kRanked && ctas > kSms && ctas <= 6 * kSms;
   auto kern = bf16 ? (int8 ? many_rows_kernel<true, true> : many_rows_kernel<true, false>)
                    : (int8 ? many_rows_kernel<false, true> : many_rows_kernel<false, false>);
   RT_TRY(ensure_kernel_smem(reinterpret_cast<const void*>(kern), sizeof(Smem), true));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<int64_t>(a.n_seq) * a.cache.heads * a.tiles * a.splits));
+  cfg.gridDim = dim3(static_cast<unsigned>(ctas));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = sizeof(Smem);
   cfg.stream = st;

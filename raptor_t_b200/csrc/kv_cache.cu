@@ -76,32 +76,15 @@ __device__ __forceinline__ Span span_of(int seq, int nth, const int32_t* __restr
   return s;
 }
 
-// Which sequence and which of its blocks a CTA takes.  Direct: every sequence has `spans` places, as many as its longest one may need.  From a list:
-// sequence s has the places first[s] / 64 + 2 s .. first[s + 1] / 64 + 2 s + 1, never fewer than it needs (a sequence of n tokens touches at
-// most (n + 62) / 64 + 1 blocks), tokens / 64 + 2 n_seq in all; each CTA looks for the sequence that has its place.
-struct Place {
-  int seq, nth;
-};
+// Which sequence and which of its blocks a CTA takes.  Direct: every sequence has `spans` places, as many as its longest one may need.  From a list
+// (kv::find_place): a sequence of n tokens touches at most (n + 62) / 64 + 1 blocks, never more than n / 64 + 2.
 template <bool LISTED>
-__device__ __forceinline__ Place place_of(int at, int spans, const int32_t* __restrict__ first, int n_seq, int tokens, int max_tokens, int* err, int site) {
-  if constexpr (!LISTED) return Place{at / spans, at % spans};
-  __shared__ int s_seq, s_nth, s_found;
-  if (threadIdx.x == 0) s_found = 0;
-  __syncthreads();
-  for (int s = threadIdx.x; s < n_seq; s += blockDim.x) {
-    const int f0 = first[s], f1 = first[s + 1];
-    if (f1 <= f0) continue;
-    const int64_t lo = (f0 >> 6) + 2ll * s, hi = (f1 >> 6) + 2ll * s + 2;
-    if (f0 < 0 || f1 > tokens || static_cast<int64_t>(f1) - f0 > max_tokens) {
-      kv::index_error(err, site);
-    } else if (lo <= at && at < hi) {
-      s_seq = s;
-      s_nth = static_cast<int>(at - lo);
-      if (atomicAdd(&s_found, 1)) kv::index_error(err, site);  // rows of two sequences
-    }
-  }
-  __syncthreads();
-  return Place{s_found == 1 ? s_seq : -1, s_nth};
+__device__ __forceinline__ kv::Place place_of(int at, int spans, const int32_t* __restrict__ first, int n_seq, int tokens, int max_tokens, int* err,
+                                              int site) {
+  if constexpr (!LISTED) return kv::Place{at / spans, at % spans};
+  __shared__ kv::Place found;
+  __shared__ int count;
+  return kv::find_place(at, first, n_seq, 1, 6, 2, tokens, max_tokens, &found, &count, err, site);
 }
 
 // The packed row of 64 values of token `t` (row of the batch): token-major with strides, or head-major per sequence
@@ -204,7 +187,7 @@ kv_write_kernel(KvView c, const uint16_t* __restrict__ k, const uint16_t* __rest
   RT_PDL_WAIT();
   RT_PDL_LAUNCH_DEPENDENTS();  // not before the wait: launches would queue up on the SMs
   const int head = blockIdx.x % c.heads;
-  const Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheWrite);
+  const kv::Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheWrite);
   if (place.seq < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool values = warp >= 2;
@@ -311,7 +294,7 @@ kv_read_kernel(KvView c, uint16_t* __restrict__ out_k, uint16_t* __restrict__ ou
   RT_PDL_WAIT();
   RT_PDL_LAUNCH_DEPENDENTS();
   const int head = blockIdx.x % c.heads;
-  const Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheRead);
+  const kv::Place place = place_of<LISTED>(blockIdx.x / c.heads, spans, first, n_seq, tokens, max_tokens, err, kSiteCacheRead);
   if (place.seq < 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const bool values = warp >= 2;

@@ -30,6 +30,34 @@ constexpr float kMinScale = 7.888609052210118e-31f;  // 2^-100: 1 / scale stays 
 
 __device__ __forceinline__ void index_error(int* err, int site) { atomicCAS(err, 0, site); }
 
+// Which part of which sequence a CTA takes, where nobody knows the longest one: sequence s has the places
+// (first[s] * group >> shift) + spare * s up to where those of s + 1 begin, at least (n * group >> shift) + spare for n tokens.  Each CTA looks for
+// the sequence that has place `at`; none: seq = -1.  All threads call it; found and count are in shared memory.
+struct Place {
+  int seq, nth;
+};
+__device__ __forceinline__ Place find_place(int at, const int32_t* __restrict__ first, int n_seq, int group, int shift, int spare, int tokens,
+                                            int most, Place* found, int* count, int* err, int site) {
+  if (threadIdx.x == 0) *count = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < n_seq; s += blockDim.x) {
+    const int f0 = first[s], f1 = first[s + 1];
+    if (f1 <= f0) continue;
+    if (f0 < 0 || f1 > tokens || f1 - f0 > most) {
+      index_error(err, site);
+      continue;
+    }
+    const int64_t lo = (static_cast<int64_t>(f0) * group >> shift) + static_cast<int64_t>(spare) * s;
+    const int64_t hi = (static_cast<int64_t>(f1) * group >> shift) + static_cast<int64_t>(spare) * (s + 1);
+    if (lo <= at && at < hi) {
+      if (atomicAdd(count, 1)) index_error(err, site);  // rows of two sequences
+      *found = Place{s, static_cast<int>(at - lo)};
+    }
+  }
+  __syncthreads();
+  return *count == 1 ? *found : Place{-1, 0};
+}
+
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
   uint32_t r;
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));

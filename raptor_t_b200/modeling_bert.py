@@ -94,8 +94,8 @@ class BertCachedAttention:
 
     def __call__(self, hidden, cache, block_table, start, context, first, max_tokens=None, max_context=0):
         """hidden [tokens, H]: rows first[s] .. first[s + 1] - 1 are new tokens of sequence s, which has start[s] tokens in the cache and
-        context[s] with them.  max_tokens: the most new tokens of one sequence; give it for single tokens and for batches of many
-        sequences (without it the attention plans for one that has all rows).  Returns LayerNorm(attention output + hidden)."""
+        context[s] with them.  max_tokens: the most new tokens of one sequence; give it for single tokens
+        (without it the attention plans for one sequence that has all rows).  Returns LayerNorm(attention output + hidden)."""
         qkv = ops.gemm(hidden, self.qkv_w, self.qkv_b, ops.capi.RT_EPI_BIAS)
         q, k, v = (t.unflatten(1, (self.heads, 64)) for t in qkv.split(self.H, 1))
         ops.kv_cache_write(cache, k, v, block_table, start, first, max_tokens)
