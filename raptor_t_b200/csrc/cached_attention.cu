@@ -565,14 +565,18 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_per_sm(NT)) few_rows_kernel(
 
 constexpr int kSms = 148;
 
-// CTAs that share a tile's keys, a power of two (clusters of 3 or 6 run slower than of 2 or 4): as many as have a block for every warp and do not
-// make more than 1.35 rounds of CTAs.  One round is best for equal lengths (8 x 4096 tokens, 12 heads: 16.3 us with 4, 20.1 with 8),
-// two with the long sequences first for ragged ones (24 x 1000 to 16384 tokens, 4 key heads: 38.6 us with 4, 31 with 8).
+// CTAs that share a tile's keys, a power of two (clusters of 3 or 6 run slower than of 2 or 4): as many as have a block for every warp, do not
+// make more than 1.35 rounds of CTAs, and, beyond two CTAs an SM, leave a warp of the longest sequence four blocks.
+// More than one round, with the long sequences first, is for ragged lengths, which a batch of answers has.  us by CTAs of a tile, all lengths equal and from 1/16 of
+// that on at random: 96 tiles x 16384 keys 4: 42.9 and 34.2, 8: 45.3 and 27.4; 384 x 4096 1: 41.5 and 34.4, 2: 45.6 and 25.0; 384 x 8192 1: 76.0 and 63.8,
+// 2: 80.3 and 43.7.  Fewer than four blocks a warp do not pay for the join: 96 x 4096 4: 14.7 and 13.1, 8: 17.5 and 15.4; 192 x 2048 2: 14.6 and 12.5, 4: 16.6 and
+// 14.9; but while few CTAs run, they shorten the chain: 24 x 4096 4: 9.0 and 9.0, 8: 7.7 and 7.9.
 // With 16 rows a tile results weigh more, and one round it is.
 int splits_of(int64_t units, int tile_rows, int64_t keys) {
   const int64_t slots = kSms * ctas_per_sm(tile_rows / 8), room = tile_rows == 8 ? slots * 135 / 100 : slots;
+  auto pays = [&](int64_t splits) { return tile_rows != 8 || units * splits <= 2 * kSms || keys >= 64 * kWarps * 4 * splits; };
   int splits = 1;
-  while (splits < kMaxSplits && units * splits * 2 <= room && keys > 64 * kWarps * splits) splits *= 2;
+  while (splits < kMaxSplits && units * splits * 2 <= room && keys > 64 * kWarps * splits && pays(2 * splits)) splits *= 2;
   return splits;
 }
 
