@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Sc
   const int rank = blockIdx.x % a.ranks, row = blockIdx.x / a.ranks;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Share<TYPE> share(static_cast<const typename L::T*>(a.logits) + row * a.pitch, a.vocab, rank, a.ranks);
-  static_assert(kMaxRanks * kMaxTop <= kThreads && kRowWarps <= 64, "");
+  static_assert(kMaxRanks * kMaxTop <= kThreads && kRowWarps <= 32, "one warp joins what the row's warps have found");
   if (tid < kMaxRanks * kMaxTop) s_all[tid] = 0;
   if (tid == 0) s_count = s_flags = 0;
   if (a.ranks > 1) ptx::cluster_arrive();  // waited for before another CTA's shared memory is written
@@ -539,20 +539,11 @@ __global__ void __launch_bounds__(kThreads, CTAS) token_logprobs_kernel(const Sc
   }
   if (warp == kThreads / 32 - 1) {
     const int n = a.ranks * (kThreads / 32);
-    Stats x, y;
+    Stats x;
     float most = -INFINITY;
     if (lane < n) {
       x = s_warp[lane];
       most = s_warp_max[lane];
-    }
-    if (lane + 32 < n) {
-      y = s_warp[lane + 32];
-      most = fmaxf(most, s_warp_max[lane + 32]);
-      const float to = fmaxf(x.r, y.r);
-      if (to != x.r) x.raise(to);
-      if (to != y.r) y.raise(to);
-      x.s += y.s;
-      x.w += y.w;
     }
     join_warp(x);
     most = warp_max(most);
