@@ -62,7 +62,7 @@ struct CachedRows {
 constexpr int kRanked = 256;
 __device__ __forceinline__ int index_by_cost(int* key, int n, int mine, int place) {
   const int tid = threadIdx.x;
-  const int own = min(mine >> 6, (1 << 23) - 1) * kRanked + (kRanked - 1 - tid);  // no two are equal
+  const int own = max(-1, min(mine >> 6, (1 << 23) - 1)) * kRanked + (kRanked - 1 - tid);  // no two are equal
   if (tid < n) key[tid] = own;
   if (tid < 4) key[n + tid] = INT_MIN;
   __syncthreads();
