@@ -240,7 +240,8 @@ rt_status rt_sparse_attention_static(void* ctx_dev, const void* q_dev, const voi
  * ---------------------------------------------------------------------------------------- */
 
 /* Blocks of 64 tokens of one head, 64 dimensions each: k / v [blocks][kv_heads][64 tokens][64] code bytes (e4m3 or
- * int8), k_scale / v_scale fp32 [blocks][kv_heads], at least 0; value = code * scale.  Which blocks belong to a sequence, and in which order,
+ * int8), k_scale / v_scale fp32 [blocks][kv_heads], at least 0; value = code * scale (the codes of tokens are numbers:
+ * rt_kv_cache_write stores no NaN of e4m3, and one in a value makes rows NaN that do not see it).  Which blocks belong to a sequence, and in which order,
  * is the caller's block table: int32 [n_seq][table_stride], entry j = block of tokens 64 j .. 64 j + 63; entries behind a
  * sequence's last token are not read.  Sequences may share blocks that none of them writes to. */
 typedef struct rt_kv_cache {

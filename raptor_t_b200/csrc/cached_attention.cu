@@ -16,10 +16,10 @@
 // entries 2^-28 below the row's largest.  Probabilities are rounded to halves (2^-11 relative) for the second product; their
 // sum is that of the rounded ones, in fp32.
 //
-// Measured (int8, 12 heads): one token over 4,096 cached ones 6.7 us, of which 2 are a launch and the rest the chain context, block table, codes,
-// products, join; 64 x 4096 tokens 77.6 us, 5.2 TB/s of codes; ragged calls lose the last CTAs' time.  From 16 rows on the warps' instructions count:
+// Measured (int8, 12 heads): one token over 4,096 cached ones 6.6 us, of which 2 are a launch and the rest the chain context, block table, codes,
+// products, join; 64 x 4096 tokens 78.6 us, 5.1 TB/s of codes; ragged calls lose the last CTAs' time.  From 16 rows on the warps' instructions count:
 // 1.65 ns a tile of 16 rows and block of keys on the full chip.  Tiles of 32 rows (255 registers, two CTAs an SM) run slower: 16 x 4096 keys, 32 rows
-// 53.4 us, 42.5 with two tiles of 16.
+// 53.4 us, 43.4 with two tiles of 16.
 #include "cached_attention.h"
 
 #include <algorithm>

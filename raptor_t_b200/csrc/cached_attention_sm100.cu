@@ -19,9 +19,10 @@
 // what counts most in the row's output, whatever scales other rows see (2^7; p' <= 2^15).  The sum of the probabilities has a running maximum M of
 // the scores as its reference and is taken from the same exponentials, times 2^(R - M - log2 scale - 7); out = O 2^(R - M - 7) / sum.
 //
-// Bound by the softmax warps' issue slots (60 % used) and the exponentials (16 a clock and SM, 49 %): 0.85 us for 256 rows and a block of keys, 730 TFLOP/s
-// of the chip, after 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144 heads: 66.2 us.  Before: two streams of 128
-// keys a step, eight softmax warps an SM, 2.0 us for 256 rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
+// No unit is full: the issue slots are 60 % used, the exponentials (16 a clock and SM) 49 %.  What bounds a stream is the chain of its step: scores, maximum,
+// the wait for the product before, exponentials, store, fence, product; four streams overlap it as far as the registers of their softmax warps go.  0.86 us for
+// 256 rows and a block of keys, 720 TFLOP/s of the chip, after 10 to 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144
+// heads, device time in a captured graph: 65.7 us (int8), 64.2 (e4m3).  Before: two streams of 128 keys a step, eight softmax warps an SM, 2.0 us for 256 rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
 // 77.8 us for the whole.
 // Few tiles over many keys are split over the CTAs of a cluster; partial results, of streams and of CTAs, meet in (distributed) shared memory.
 #include "cached_attention.h"

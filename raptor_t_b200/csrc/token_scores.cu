@@ -9,9 +9,9 @@
 // logits, still in L2) and list what does.  A list that does not fit (thousands of equal logits) is replaced by k
 // searches over the row.
 //
-// Measured (50,358 logits a row): forward of 2,048 rows of fp16 with 8 alternatives 47.7 us, 4.3 TB/s (41 without alternatives: the list costs four
+// Measured (50,358 logits a row, device time in a captured graph; 0.3 to 0.5 us more a call in a loop, and up to 4 % between GPUs): forward of 2,048 rows of fp16 with 8 alternatives 47.7 us, 4.3 TB/s (41 without alternatives: the list costs four
 // barriers and a round trip to L2 a row); 4,096 rows 83, 5.0 TB/s; 19 rows 7.0, a launch and the chain of one row.  Gradient of 4,096 rows of bf16
-// with 4 alternatives 137 us, 6.0 TB/s; with one value at a time instead of packed pairs 144.
+// with 4 alternatives 135 to 137 us, 6.0 TB/s; with one value at a time instead of packed pairs 144.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
