@@ -22,7 +22,8 @@
 // No unit is full: the issue slots are 60 % used, the exponentials (16 a clock and SM) 49 %.  What bounds a stream is the chain of its step: scores, maximum,
 // the wait for the product before, exponentials, store, fence, product; four streams overlap it as far as the registers of their softmax warps go.  0.86 us for
 // 256 rows and a block of keys, 720 TFLOP/s of the chip, after 10 to 12 us for the start, the queries, the join and the end of a CTA.  256 rows x 64 blocks x 144
-// heads, device time in a captured graph: 65.7 us (int8), 64.2 (e4m3).  Before: two streams of 128 keys a step, eight softmax warps an SM, 2.0 us for 256 rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
+// heads, device time in a captured graph: 65.7 us (int8), 64.2 (e4m3).  Before: two streams of 128 keys a step, eight softmax warps an SM, 2.0 us for 256
+// rows x 128 keys; probabilities over the scores' TMEM columns, which the next scores wait for,
 // 77.8 us for the whole.
 // Few tiles over many keys are split over the CTAs of a cluster; partial results, of streams and of CTAs, meet in (distributed) shared memory.
 #include "cached_attention.h"
@@ -727,7 +728,7 @@ rt_status launch_cached_attention_many_rows(const Args& args, bool bf16, bool in
   // Longest tiles first where there are more CTAs than run at once, but not so many that the last round hardly counts or that ranking them, which
   // every CTA does for itself, costs more than it saves.  Sequences of 65 to 256 rows over 64 to 4096 keys, us in order and ranked: 200 with one key head
   // (200 CTAs) 70.6 and 54.9, 128 with four (512) 95.5 and 73.7, 200 with four (800) 137.7 and 113.3, 256 with four (1024) 157.4 and 152.4, 256 with
-  // twelve (3072) 414 and 456; equal lengths lose 3 to 6 %.  Ranking 768 of them took 110 us of a call of 160.
+  // twelve 414 and 456; equal lengths lose 3 to 6 %.  Ranking 768 of them took 110 us of a call of 160.
   const int64_t items = many_rows_items(a), ctas = items * a.cache.heads * a.splits;
   RT_REQUIRE(ctas < (int64_t{1} << 31), RT_ERR_UNSUPPORTED, "cached_attention: %d sequences of up to %d query tokens are too many for one call", a.n_seq,
              a.max_q);

@@ -174,8 +174,8 @@ __device__ __forceinline__ void values4(uint32_t w, float scale, float* x) {
 
 // grid: (block of the sequence, head) pairs of every sequence; warps 0 and 1 take the keys, 2 and 3 the values, 32 tokens each.
 // A tile is read once, and its largest value is known before the first code is: it stays in registers.  Two warps for a tile keep 36
-// warps an SM at that (32: 19.9 us, 40: 21.3, they spill).  8 sequences of 1024 to 4096 tokens, 12 heads, f16 to int8 (95 MB): 19.5 us of device time, 20.1 a call, 4.9 TB/s, bound by
-// HBM and a CTA's chain of index, load, maximum, store; one warp a tile, quotients by division and maxima in fp32 took 67.7.  A step's tokens (32 sequences, 12 heads) are that
+// warps an SM at that (32: 19.9 us, 40: 21.3, they spill).  8 sequences of 1024 to 4096 tokens, 12 heads, f16 to int8 (95 MB): 19.5 us of device time, 20.1 a call, 4.9 TB/s,
+// bound by HBM and a CTA's chain of index, load, maximum, store; one warp a tile, quotients by division and maxima in fp32 took 67.7.  A step's tokens (32 sequences, 12 heads) are that
 // chain alone, 2.8 us.
 constexpr int kWriteThreads = 128;
 template <bool BF16, bool INT8, bool LISTED>
